@@ -508,6 +508,122 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
                                        int32_t max_tokens, int32_t dims[7],
                                        char symbol[LF_FP8_SYMBOL_BYTES]);
 
+/* ---- attention between the projections ----------------------------------- */
+/*
+ * The steps from the packed Q|K|V rows of a QKV projection to the rows the
+ * output projection reads, over a paged key / value cache:
+ *  lf_attn_qk_norm_rope_{bf16,e4m3}
+ *      (counts, positions, row_offsets, lengths, page_offsets, page_indices,
+ *       attn, qkv, gq, gk, q, k_cache, v_cache, status)
+ *  lf_attn_decode_d{64,128,256}_{bf16,e4m3}
+ *      (counts, row_offsets, lengths, page_offsets, page_indices, attn, q,
+ *       out, k_cache, v_cache, ws)
+ *  lf_attn_join_d{64,128,256}
+ *      (counts, row_offsets, attn, out, ws)   after lf_attn_decode
+ *
+ * Runtime inputs, int32, in the vocabulary of a paged step (model/plan
+ * runtime inputs): counts = StepCounts; row_offsets [total_rows + 1], the
+ * rows of sequence s being row_offsets[s] .. row_offsets[s + 1] - 1; lengths
+ * [total_rows], the tokens of sequence s once this step's rows are in the
+ * cache; page_offsets [total_rows + 1] into page_indices, the pages of
+ * sequence s in order; positions [query_tokens, axes], what the rotation
+ * turns by (a row's place in the cache comes from lengths and row_offsets, so
+ * positions of images or shifted ones need not be places). attn: the
+ * descriptor region below, a model constant.
+ *
+ * qk_norm_rope, every row m < query_tokens that belongs to a sequence: each
+ * query and key head u of the packed row qkv [M, Hq + 2 Hkv, D] (bf16) is
+ * normalized, u = u (g / sqrt(mean(u^2) + epsilon)) (norm 0: not; gq, gk bf16
+ * [D]), and the pairs of its first rotary_dim values are turned by 2 pi
+ * positions[m, axis[i]] turns[i], the angle in 64 bits. Pair i is (u[i],
+ * u[i + rotary_dim / 2]) (pairing 0) or (u[2 i], u[2 i + 1]) (pairing 1).
+ * Everything is fp32 up to one rounding at the store: query heads to q
+ * [M, Hq, D] bf16, keys and values to the row's place in the cache, as bf16 or
+ * as e4m3 codes of x * (1 / scale[head]), saturated to +-448 (NaN stays NaN).
+ *
+ * decode, the sequences prefill_rows .. prefill_rows + decode_rows - 1, one
+ * row each (the first of its range): out[row] = sum_j p_j v_j over the keys j
+ * of [max(0, length - window), length) (window 0: all), p = softmax of
+ * softmax_scale q.k_j. Query head h reads key head h / (Hq / Hkv). The scores
+ * and the softmax statistics are fp32; the weights p go to the second product
+ * as bf16 and are summed as what they were rounded to. A row without keys (or
+ * all of whose scores are -inf) gives zeros; values at keys that do not count
+ * are not read into the sum, whatever they hold. Other rows of out stay as
+ * they were.
+ *
+ * The cache regions hold, for page p, head h and slot i, D elements at
+ * p * page_stride + h * head_stride + i * token_stride (elements; any order of
+ * the three dimensions without overlap). Page indices outside [0, pages) are
+ * not followed: the append drops the row, the attention leaves the page's keys
+ * out. Offsets and lengths that leave the descriptor's bounds or the
+ * sequence's pages are cut to them. Each sets the int32 error word at the
+ * start of status / ws to nonzero (it stays set until the caller clears it).
+ */
+#define LF_FP8_ATTN_MAGIC 0x4E54414Cu /* bytes "LATN" */
+#define LF_FP8_ATTN_DESC_BYTES 256
+#define LF_FP8_ATTN_MAX_SEQUENCES 2048
+#define LF_FP8_ATTN_STATUS_BYTES 256
+
+enum lf_fp8_attn_cache { LF_FP8_CACHE_BF16 = 1, LF_FP8_CACHE_E4M3 = 2 };
+enum lf_fp8_attn_pairing { LF_FP8_PAIR_HALF = 0, LF_FP8_PAIR_NEIGHBOUR = 1 };
+
+/* The descriptor region: this structure, then (offsets from its start) the
+ * cache scales fp32 [2][kv_heads] (keys, values), turns fp64 [rotary_dim / 2]
+ * (turns per position) and axis int32 [rotary_dim / 2]. */
+typedef struct lf_fp8_attn_desc {
+  uint32_t magic;
+  int32_t query_heads;   /* a multiple of kv_heads */
+  int32_t kv_heads;
+  int32_t head_dim;      /* 64, 128 or 256 */
+  int32_t cache;         /* enum lf_fp8_attn_cache */
+  int32_t page_size;     /* a power of two, 8 .. 1024 */
+  int32_t pages;
+  int32_t max_tokens;    /* rows of qkv, q and out */
+  int32_t max_sequences; /* at most LF_FP8_ATTN_MAX_SEQUENCES */
+  int32_t table_entries; /* capacity of page_indices */
+  int32_t window;        /* 0: none */
+  int32_t rotary_dim;    /* 0 (no rotation) or a multiple of 16, at most head_dim */
+  int32_t axes;          /* 1 .. 4: positions of a row */
+  int32_t pairing;       /* enum lf_fp8_attn_pairing */
+  int32_t norm;          /* 0 or 1 */
+  float norm_epsilon;
+  float softmax_scale;
+  int32_t reserved;
+  int64_t page_stride;   /* elements; all three 0: [page][head][slot][D] */
+  int64_t head_stride;
+  int64_t token_stride;
+  int64_t scale_offset;  /* bytes, written by lunaflux_fp8_attn_descriptor */
+  int64_t turns_offset;
+  int64_t axis_offset;
+  int64_t region_bytes;
+  uint8_t padding[128];
+} lf_fp8_attn_desc;
+
+/* Checks the fields of *desc, and writes its magic, default strides and the
+ * region offsets. LF_INVALID_ARGUMENT for values outside the ranges above,
+ * strides that overlap or are not multiples of 16 bytes, or bounds past 32
+ * bits (table_entries * page_size, the 128-key tiles of a step times heads). */
+int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *desc);
+/* Writes the descriptor region (desc->region_bytes bytes). scales: 2 kv_heads
+ * values, finite and above zero (null for a bf16 cache: ones); turns and axis:
+ * rotary_dim / 2 each, turns finite, 0 <= axis < axes (null without rotation). */
+int32_t lunaflux_fp8_attn_region(const lf_fp8_attn_desc *desc, const float *scales,
+                                 int64_t scale_count, const double *turns, const int32_t *axis,
+                                 int64_t pair_count, uint8_t *region, int64_t region_bytes);
+/* Bytes one cache region (keys or values) spans; -1 if invalid. */
+int64_t lunaflux_fp8_attn_cache_bytes(const lf_fp8_attn_desc *desc);
+
+enum lf_fp8_attn_entry {
+  LF_FP8_ATTN_QK_NORM_ROPE = 1,
+  LF_FP8_ATTN_DECODE = 2,
+  LF_FP8_ATTN_JOIN = 3 /* runs after DECODE, on its workspace */
+};
+/* Workspace of DECODE and JOIN (ws) or of QK_NORM_ROPE (status): zero-filled
+ * once when allocated; launches sharing one must not overlap. -1 if invalid. */
+int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc *desc);
+int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc *desc,
+                                          int32_t dims[7], char symbol[LF_FP8_SYMBOL_BYTES]);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,7 @@ _i32p = ctypes.POINTER(ctypes.c_int32)
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _f32p = ctypes.POINTER(ctypes.c_float)
+_f64p = ctypes.POINTER(ctypes.c_double)
 
 SIGNATURES = {
     "lunaflux_hip_probe": (_i32, [_i64p]),
@@ -139,10 +140,19 @@ SIGNATURES = {
     "lunaflux_fp8_moe_workspace_layout": (_i32, [_vp, _i32, _i64p]),
     "lunaflux_fp8_moe_launch_geometry": (_i32, [_i32, _vp, _i32, _i32p, ctypes.c_char_p]),
     "lunaflux_fp8_moe_step_geometry": (_i32, [_i32, _vp, _i32, _i32p, ctypes.c_char_p]),
+    "lunaflux_fp8_attn_descriptor": (_i32, [_vp]),
+    "lunaflux_fp8_attn_region": (_i32, [_vp, _f32p, _i64, _f64p, _i32p, _i64, _u8p, _i64]),
+    "lunaflux_fp8_attn_cache_bytes": (_i64, [_vp]),
+    "lunaflux_fp8_attn_workspace_bytes": (_i64, [_i32, _vp]),
+    "lunaflux_fp8_attn_launch_geometry": (_i32, [_i32, _vp, _i32p, ctypes.c_char_p]),
 }
 
 MOE_ROUTE, MOE_SORT, MOE_QUANT_TOKENS, MOE_GATE_UP, MOE_QUANT_HIDDEN, MOE_DOWN, MOE_COMBINE = range(1, 8)
 MOE_SORT_COUNT = 8
+LF_FP8_CACHE_BF16, LF_FP8_CACHE_E4M3 = 1, 2
+LF_FP8_PAIR_HALF, LF_FP8_PAIR_NEIGHBOUR = 0, 1
+LF_FP8_ATTN_MAX_SEQUENCES = 2048
+ATTN_QK_NORM_ROPE, ATTN_DECODE, ATTN_JOIN = 1, 2, 3
 
 
 class NativeLibraryMissing(RuntimeError):

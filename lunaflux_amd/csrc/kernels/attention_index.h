@@ -1,0 +1,153 @@
+// attention_index.h - which memory the attention kernels touch and how their
+// work is cut: the descriptor as the device sees it, a sequence's pages and
+// live keys, and the split of a step's key tiles over blocks. Integer code
+// only, no device builtins, so it also compiles for the host.
+#pragma once
+
+#include <stdint.h>
+
+namespace attn {
+
+// Mirror of lf_fp8_attn_desc.
+struct Desc {
+  uint32_t magic;
+  int32_t query_heads, kv_heads, head_dim, cache, page_size, pages;
+  int32_t max_tokens, max_sequences, table_entries, window;
+  int32_t rotary_dim, axes, pairing, norm;
+  float norm_epsilon, softmax_scale;
+  int32_t reserved;
+  int64_t page_stride, head_stride, token_stride;
+  int64_t scale_offset, turns_offset, axis_offset, region_bytes;
+};
+constexpr uint32_t kMagic = 0x4E54414Cu;
+
+// Entries of sequence s in the page table; none where the offsets leave it.
+struct Pages {
+  int first, count;
+};
+LF_DEVICE Pages pages_of(const Desc &d, const int32_t *offsets, int s, bool &bad) {
+  const int first = offsets[s], end = offsets[s + 1];
+  if (first < 0 || end < first || end > d.table_entries) {
+    bad = true;
+    return {0, 0};
+  }
+  return {first, end - first};
+}
+
+// Byte of (page, head, slot) in a cache region. Strides fit 31 bits, so each
+// product is one 32 x 32 -> 64 multiplication.
+template <bool E4M3>
+LF_DEVICE uint64_t cache_byte(const Desc &d, int page, int head, int slot) {
+  constexpr uint64_t size = E4M3 ? 1 : 2;
+  return size * (static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(d.page_stride) +
+                 static_cast<uint64_t>(static_cast<uint32_t>(head)) * static_cast<uint32_t>(d.head_stride) +
+                 static_cast<uint64_t>(static_cast<uint32_t>(slot)) * static_cast<uint32_t>(d.token_stride));
+}
+
+// ---- append ---------------------------------------------------------------------
+
+// Page and slot of a row of sequence s; page -1 where there is none.
+struct Place {
+  int page, slot;
+};
+LF_DEVICE Place place_of(const Desc &d, const int32_t *row_offsets, const int32_t *lengths,
+                         const int32_t *page_offsets, const int32_t *page_indices, int s, int row) {
+  bool bad = false;
+  const Pages pages = pages_of(d, page_offsets, s, bad);
+  const int64_t token = static_cast<int64_t>(lengths[s]) - row_offsets[s + 1] + row;
+  const int shift = __builtin_ctz(static_cast<uint32_t>(d.page_size));
+  if (token < 0 || (token >> shift) >= pages.count) return {-1, 0};
+  const int page = page_indices[pages.first + static_cast<int>(token >> shift)];
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(d.pages)) return {-1, 0};
+  return {page, static_cast<int>(token & (d.page_size - 1))};
+}
+
+// ---- single-token attention -------------------------------------------------------
+
+constexpr int kTileKeys = 128;
+constexpr int kHeadTile = 16;
+
+// Keys [lo, len) of a sequence, in `tiles` tiles from the one that holds lo;
+// a sequence without keys has one tile, whose block writes its zeros.
+struct Span {
+  int first_tile, tiles, lo, len;
+};
+LF_DEVICE Span span_of(const Desc &d, const int32_t *lengths, const int32_t *page_offsets, int s, bool &bad) {
+  const Pages p = pages_of(d, page_offsets, s, bad);
+  int len = lengths[s];
+  const int most = p.count * d.page_size;
+  if (len < 0 || len > most) {
+    bad = true;
+    len = len < 0 ? 0 : most;
+  }
+  const int lo = d.window > 0 && len > d.window ? len - d.window : 0;
+  const int first = lo / kTileKeys;
+  const int end = (len + kTileKeys - 1) / kTileKeys;
+  return {first, end > first ? end - first : 1, lo, len};
+}
+
+// Page of key j, or -1: outside the entries [first, end) that hold keys which
+// count (a released page before the window, an unused one behind the length),
+// or outside the cache.
+LF_DEVICE int page_of(const Desc &d, const int32_t *table, int first, int end, int shift, int j, bool &bad) {
+  const int e = j >> shift;
+  if (e < first || e >= end) return -1;
+  const int page = table[e];
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(d.pages)) {
+    bad = true;
+    return -1;
+  }
+  return page;
+}
+
+LF_DEVICE int head_tiles_of(const Desc &d) {
+  const int group = d.query_heads / d.kv_heads;
+  return d.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
+}
+
+// The step's sequences s0 .. s0 + n - 1 that are decoded.
+struct Decoded {
+  int s0, n;
+};
+LF_DEVICE Decoded decoded_of(const Desc &d, const int32_t *counts) {
+  int total = counts[2], s0 = counts[0], n = counts[1];
+  total = total < 0 ? 0 : total > d.max_sequences ? d.max_sequences : total;
+  s0 = s0 < 0 ? 0 : s0 > total ? total : s0;
+  n = n < 0 ? 0 : n > total - s0 ? total - s0 : n;
+  return {s0, n};
+}
+
+// The step's items are the tiles of every (sequence, head tile) pair in turn:
+// pair (i, ht) starts at prefix[i] head_tiles + ht tiles(i), where prefix adds
+// up the tiles of the sequences before i. Block b holds the items
+// [b share, (b + 1) share).
+LF_DEVICE int share_of(int items, int blocks) { return (items + blocks - 1) / blocks; }
+
+// The sequence that item u belongs to (prefix rises by at least 1 a sequence).
+LF_DEVICE int sequence_at(const int *prefix, int n, int head_tiles, int u) {
+  int i = 0;
+  for (int lo = 0, hi = n; lo < hi;) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] * head_tiles <= u) {
+      i = mid;
+      lo = mid + 1;
+    } else {
+      hi = mid;
+    }
+  }
+  return i;
+}
+
+// The blocks first .. last that hold parts of the pair whose items are [begin,
+// begin + tiles), and where block b leaves its part: partial result 2 b if the
+// pair is the first thing in the block's range, 2 b + 1 if it comes after
+// another (only the pair's first block can, so no two parts share a place).
+struct Parts {
+  int first, last;
+};
+LF_DEVICE Parts parts_of(int begin, int tiles, int share) {
+  return {begin / share, (begin + tiles - 1) / share};
+}
+LF_DEVICE int part_slot(int block, int begin, int share) { return 2 * block + (begin > block * share ? 1 : 0); }
+
+}  // namespace attn

@@ -4,4 +4,5 @@
 #include "w8a16.hip"
 #include "w8a16_gemm.hip"
 #include "moe.hip"
+#include "attention.hip"
 #include "calibrate.hip"

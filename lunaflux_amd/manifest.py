@@ -70,6 +70,9 @@ FAMILIES = (
     (9, "lf_moe_"),
     (10, "lf_fp8_w8a16_gated_mlp_"),
     (11, "lf_fp8_w8a8_gated_mlp_"),
+    (23, "lf_attn_qk_norm_rope_"),
+    (24, "lf_attn_decode_"),
+    (25, "lf_attn_join_"),
 )
 
 

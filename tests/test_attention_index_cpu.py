@@ -1,0 +1,150 @@
+"""The attention kernels' index arithmetic (csrc/kernels/attention_index.h), run
+on the CPU: for descriptors and steps of any kind, also ones whose offsets,
+lengths and page indices are garbage, no place read or written lies outside
+the regions the descriptor bounds; and for sound steps the cut of the key tiles
+over blocks covers every tile once, and the join reads exactly the partial
+results that the blocks leave."""
+import os
+import subprocess
+
+
+from lunaflux_amd import build as native_build
+
+KERNELS = os.path.join(native_build.CSRC, "kernels")
+
+PROGRAM = r"""
+#include <cstdint>
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <set>
+#include <vector>
+#define LF_DEVICE static inline
+#include "attention_index.h"
+using namespace attn;
+#define CHECK(x) do { if (!(x)) { std::printf("FAIL line %d: %s\n", __LINE__, #x); std::exit(1); } } while (0)
+static std::mt19937 rng(7);
+static int pick(int lo, int hi) { return lo + static_cast<int>(rng() % static_cast<unsigned>(hi - lo + 1)); }
+
+static Desc desc() {
+  Desc d{};
+  d.kv_heads = pick(1, 8);
+  d.query_heads = d.kv_heads * pick(1, 40);
+  d.head_dim = 64 << pick(0, 2);
+  d.page_size = 8 << pick(0, 7);
+  d.pages = pick(1, 50);
+  d.max_tokens = pick(1, 60);
+  d.max_sequences = pick(1, 20);
+  d.table_entries = pick(1, 100);
+  d.window = pick(0, 2) ? 0 : pick(1, 700);
+  d.token_stride = d.head_dim;
+  d.head_stride = d.token_stride * d.page_size;
+  d.page_stride = d.head_stride * d.kv_heads;
+  return d;
+}
+static int64_t elements(const Desc &d) {
+  return (d.pages - 1) * d.page_stride + (d.kv_heads - 1) * d.head_stride + (d.page_size - 1) * d.token_stride +
+         d.head_dim;
+}
+
+static void hostile() {
+  const Desc d = desc();
+  auto garbage = [&](size_t n) {
+    std::vector<int32_t> v(n);
+    for (auto &x : v) {
+      const int kind = pick(0, 3);
+      x = kind == 0 ? pick(-5, 5) : kind == 1 ? pick(0, 3000) : kind == 2 ? static_cast<int32_t>(rng()) : pick(0, 40);
+    }
+    return v;
+  };
+  // regions of exactly the descriptor's sizes; .at() faults outside them
+  auto counts = garbage(5), row_offsets = garbage(d.max_sequences + 1), lengths = garbage(d.max_sequences);
+  auto page_offsets = garbage(d.max_sequences + 1), table = garbage(d.table_entries);
+  const Decoded dec = decoded_of(d, counts.data());
+  CHECK(dec.s0 >= 0 && dec.n >= 0 && dec.s0 + dec.n <= d.max_sequences);
+  for (int s = 0; s < d.max_sequences; ++s) {
+    bool bad = false;
+    const Pages p = pages_of(d, page_offsets.data(), s, bad);
+    CHECK(p.first >= 0 && p.count >= 0 && p.first + p.count <= d.table_entries);
+    const Span span = span_of(d, lengths.data(), page_offsets.data(), s, bad);
+    CHECK(span.len >= 0 && span.len <= int64_t(p.count) * d.page_size && span.lo >= 0 && span.lo <= span.len);
+    CHECK(span.tiles >= 1);
+    const int shift = __builtin_ctz(d.page_size), first = span.lo >> shift, end = (span.len + d.page_size - 1) >> shift;
+    CHECK(end <= p.count);
+    for (int t = 0; t < span.tiles; ++t) {
+      for (int j = (span.first_tile + t) * kTileKeys; j < (span.first_tile + t + 1) * kTileKeys; ++j) {
+        const int e = j >> shift;
+        if (e >= first && e < end) CHECK(p.first + e >= 0 && p.first + e < d.table_entries);
+        const int page = page_of(d, table.data() + p.first, first, end, shift, j, bad);
+        CHECK(page >= -1 && page < d.pages);
+        // the kernel reads page 0 where there is none
+        for (int h = 0; h < d.kv_heads; ++h) {
+          const uint64_t at = cache_byte<true>(d, page < 0 ? 0 : page, h, j & (d.page_size - 1));
+          CHECK(at + d.head_dim <= static_cast<uint64_t>(elements(d)));
+          CHECK(cache_byte<false>(d, page < 0 ? 0 : page, h, j & (d.page_size - 1)) == 2 * at);
+        }
+      }
+    }
+    for (int row = 0; row < d.max_tokens; ++row) {
+      const Place place = place_of(d, row_offsets.data(), lengths.data(), page_offsets.data(), table.data(), s, row);
+      CHECK(place.page >= -1 && place.page < d.pages && place.slot >= 0 && place.slot < d.page_size);
+    }
+  }
+}
+
+static void cut(int blocks) {
+  Desc d = desc();
+  const int n = pick(0, d.max_sequences), head_tiles = head_tiles_of(d);
+  std::vector<int> prefix(n + 1, 0), tiles(n);
+  for (int i = 0; i < n; ++i) {
+    tiles[i] = pick(0, 4) ? pick(1, 5) : pick(1, 400);
+    prefix[i + 1] = prefix[i] + tiles[i];
+  }
+  const int items = prefix[n] * head_tiles, share = share_of(items, blocks);
+  std::vector<int> seen(items, 0);
+  std::set<int> left, read;
+  for (int b = 0; b < blocks; ++b) {
+    const int begin = b * share, end = begin + share < items ? begin + share : items;
+    for (int u = begin; u < end;) {
+      const int i = sequence_at(prefix.data(), n, head_tiles, u);
+      CHECK(prefix[i] * head_tiles <= u && u < prefix[i + 1] * head_tiles);
+      const int within = u - prefix[i] * head_tiles, ht = within / tiles[i], t0 = within - ht * tiles[i];
+      const int t1 = tiles[i] - t0 < end - u ? tiles[i] : t0 + (end - u);
+      CHECK(t1 > t0 && ht < head_tiles);
+      for (int t = t0; t < t1; ++t) seen[prefix[i] * head_tiles + ht * tiles[i] + t]++;
+      if (t0 != 0 || t1 != tiles[i]) {
+        const int slot = part_slot(b, u - t0, share);
+        CHECK(slot >= 0 && slot < 2 * blocks && left.insert(slot).second);
+      }
+      u += t1 - t0;
+    }
+  }
+  for (int x : seen) CHECK(x == 1);
+  for (int i = 0; i < n; ++i) {
+    for (int ht = 0; ht < head_tiles; ++ht) {
+      const int begin = prefix[i] * head_tiles + ht * tiles[i];
+      const Parts parts = parts_of(begin, tiles[i], share);
+      if (parts.first == parts.last) continue;
+      for (int b = parts.first; b <= parts.last; ++b) CHECK(read.insert(part_slot(b, begin, share)).second);
+    }
+  }
+  CHECK(left == read);
+}
+
+int main() {
+  for (int i = 0; i < 300; ++i) hostile();
+  const int blocks[] = {1, 2, 7, 256, 1024};
+  for (int i = 0; i < 400; ++i) cut(blocks[i % 5]);
+  std::printf("ok\n");
+}
+"""
+
+
+def test_places_stay_in_bounds_and_tiles_are_covered_once(tmp_path):
+    src = tmp_path / "index.cpp"
+    src.write_text(PROGRAM)
+    exe = str(tmp_path / "index")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", KERNELS,
+                    str(src), "-o", exe], check=True)
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
