@@ -145,6 +145,9 @@ SIGNATURES = {
     "lunaflux_fp8_attn_cache_bytes": (_i64, [_vp]),
     "lunaflux_fp8_attn_workspace_bytes": (_i64, [_i32, _vp]),
     "lunaflux_fp8_attn_launch_geometry": (_i32, [_i32, _vp, _i32p, ctypes.c_char_p]),
+    "lunaflux_fp8_low_rank_descriptor": (_i32, [_i32, _i32, _i64, _i64p, _i32, _i32, _vp]),
+    "lunaflux_fp8_low_rank_workspace_bytes": (_i64, [_vp]),
+    "lunaflux_fp8_low_rank_launch_geometry": (_i32, [_i32, _vp, _i32p, ctypes.c_char_p]),
 }
 
 MOE_ROUTE, MOE_SORT, MOE_QUANT_TOKENS, MOE_GATE_UP, MOE_QUANT_HIDDEN, MOE_DOWN, MOE_COMBINE = range(1, 8)
@@ -153,6 +156,7 @@ LF_FP8_CACHE_BF16, LF_FP8_CACHE_E4M3 = 1, 2
 LF_FP8_PAIR_HALF, LF_FP8_PAIR_NEIGHBOUR = 0, 1
 LF_FP8_ATTN_MAX_SEQUENCES = 2048
 ATTN_QK_NORM_ROPE, ATTN_DECODE, ATTN_JOIN = 1, 2, 3
+LOW_RANK_SHRINK, LOW_RANK_EXPAND = 1, 2
 
 
 class NativeLibraryMissing(RuntimeError):

@@ -49,11 +49,13 @@ def build_code_object(out=CODE_OBJECT):
 
 
 def build_library(out=LIBRARY):
-    """Host code (runtime.cpp, pack.cpp, attention.cpp) plus scratch.hip, the one source with
-    device code of its own: the scratch array and its clearing kernel, built
-    for gfx950 into the library's embedded code object."""
+    """Host code (runtime.cpp, pack.cpp, attention.cpp, low_rank.cpp) plus
+    scratch.hip, the one source with device code of its own: the scratch array
+    and its clearing kernel, built for gfx950 into the library's embedded code
+    object."""
     sources = [os.path.join(CSRC, "runtime.cpp"), os.path.join(CSRC, "pack.cpp"),
-               os.path.join(CSRC, "attention.cpp"), os.path.join(CSRC, "scratch.hip")]
+               os.path.join(CSRC, "attention.cpp"), os.path.join(CSRC, "low_rank.cpp"),
+               os.path.join(CSRC, "scratch.hip")]
     tmp = out + ".tmp"
     _run([HIPCC, *HOST_FLAGS, f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
           "-packed-fp32-ops", "-shared", "-I", INCLUDE, "-I", CSRC, *sources, "-o", tmp])

@@ -5,4 +5,5 @@
 #include "w8a16_gemm.hip"
 #include "moe.hip"
 #include "attention.hip"
+#include "low_rank.hip"
 #include "calibrate.hip"
