@@ -518,8 +518,6 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
  *  lf_attn_decode_d{64,128,256}_{bf16,e4m3}
  *      (counts, row_offsets, lengths, page_offsets, page_indices, attn, q,
  *       out, k_cache, v_cache, ws)
- *  lf_attn_join_d{64,128,256}
- *      (counts, row_offsets, attn, out, ws)   after lf_attn_decode
  *
  * Runtime inputs, int32, in the vocabulary of a paged step (model/plan
  * runtime inputs): counts = StepCounts; row_offsets [total_rows + 1], the
@@ -615,11 +613,11 @@ int64_t lunaflux_fp8_attn_cache_bytes(const lf_fp8_attn_desc *desc);
 
 enum lf_fp8_attn_entry {
   LF_FP8_ATTN_QK_NORM_ROPE = 1,
-  LF_FP8_ATTN_DECODE = 2,
-  LF_FP8_ATTN_JOIN = 3 /* runs after DECODE, on its workspace */
+  LF_FP8_ATTN_DECODE = 2
 };
-/* Workspace of DECODE and JOIN (ws) or of QK_NORM_ROPE (status): zero-filled
- * once when allocated; launches sharing one must not overlap. -1 if invalid. */
+/* Workspace of DECODE (ws) or of QK_NORM_ROPE (status): zero-filled once when
+ * allocated (its counters return to zero at the end of every launch; launches
+ * sharing one must not overlap). -1 if invalid. */
 int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc *desc);
 int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc *desc,
                                           int32_t dims[7], char symbol[LF_FP8_SYMBOL_BYTES]);

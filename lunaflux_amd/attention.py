@@ -261,6 +261,14 @@ def _holds(what: str, region: KernelArgument, byte_count: int):
         raise _invalid(f"{what}: {byte_count} bytes aligned to 16 are wanted")
 
 
+def _apart(what: str, *regions: KernelArgument):
+    """Refuses regions of one allocation that overlap."""
+    for i, p in enumerate(regions):
+        for q in regions[:i]:
+            if p.allocation is q.allocation and p.offset < q.offset + q.byte_count and q.offset < p.offset + p.byte_count:
+                raise _invalid(f"{what} overlap")
+
+
 def _step_fits(layer: AttentionLayer, step: PagedStep):
     d = layer.desc
     if (step.max_tokens, step.max_sequences, step.table_entries, step.page_size) != \
@@ -281,9 +289,10 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     """Packed rows qkv [max_tokens, Hq + 2 Hkv, D] (a QKV projection's output)
     to rotated queries q [max_tokens, Hq, D] and, in the cache, keys and values
     of every row of the step. gq, gk: the norm weights [D], given if and only if
-    the layer normalizes its heads. q may not overlap qkv."""
+    the layer normalizes its heads. The regions may not overlap."""
     d = layer.desc
     _step_fits(layer, step)
+    _apart("qkv, q and the caches", qkv, q, k_cache, v_cache)
     heads = d.query_heads + 2 * d.kv_heads
     _holds("qkv", qkv, 2 * d.max_tokens * heads * d.head_dim)
     _holds("q", q, 2 * d.max_tokens * d.query_heads * d.head_dim)
@@ -309,24 +318,20 @@ def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
                       out: KernelArgument, k_cache: KernelArgument, v_cache: KernelArgument) -> BoundAttention:
     """Attention of the step's decoded sequences: q [max_tokens, Hq, D] (bf16,
     rotated) against the cached keys of each, out [max_tokens, Hq D] as the
-    output projection reads it. Rows of other sequences stay as they were."""
+    output projection reads it. Rows of other sequences stay as they were. out
+    may not overlap what is read."""
     d = layer.desc
     _step_fits(layer, step)
+    for region in (q, k_cache, v_cache):
+        _apart("out and what is read", out, region)
     _holds("q", q, 2 * d.max_tokens * d.query_heads * d.head_dim)
     _holds("out", out, 2 * d.max_tokens * d.query_heads * d.head_dim)
     _holds("k_cache", k_cache, layer.cache_bytes)
     _holds("v_cache", v_cache, layer.cache_bytes)
     ws = _workspace(rt, _abi.ATTN_DECODE, d)
-    counts, rows = _region(step.counts, alignment=4), _region(step.row_offsets, alignment=4)
-    wsr = _region(ws, alignment=256)
-
-    def launch(entry, args):
-        dims, symbol = launch_geometry(entry, d)
-        return LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)
-
-    return BoundAttention([
-        launch(_abi.ATTN_DECODE, [counts, rows, _region(step.lengths, alignment=4),
-                                  _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4),
-                                  layer.region, q, out, k_cache, v_cache, wsr]),
-        launch(_abi.ATTN_JOIN, [counts, rows, layer.region, out, wsr]),
-    ], workspace=ws, keep=[layer, step])
+    dims, symbol = launch_geometry(_abi.ATTN_DECODE, d)
+    args = [_region(step.counts, alignment=4), _region(step.row_offsets, alignment=4), _region(step.lengths, alignment=4),
+            _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4), layer.region, q, out,
+            k_cache, v_cache, _region(ws, alignment=256)]
+    return BoundAttention([LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)], workspace=ws,
+                          keep=[layer, step])

@@ -14,8 +14,8 @@ namespace {
 
 constexpr int64_t kLimit32 = (int64_t(1) << 31) - 1;
 // kernels/attention.hip
-constexpr int64_t kTileKeys = 128;
-constexpr int64_t kDecodeBlocks = 1024;
+constexpr int64_t kTileKeys = 32;
+constexpr int64_t kGroup = 32;
 constexpr int64_t kHeadTile = 16;
 constexpr int64_t kWaves = 4;
 
@@ -69,7 +69,7 @@ bool fields_ok(const lf_fp8_attn_desc *d) {
     return false;
   }
   if (d->norm == 1 && !(d->norm_epsilon >= 0.0f && std::isfinite(d->norm_epsilon))) return false;
-  // The kernels count cached tokens, rows of positions and (tile, head) items in 32 bits.
+  // The kernels count cached tokens, positions and (key tile, head tile) items in 31 bits.
   if (int64_t(d->table_entries) * d->page_size > kLimit32 - 1024 ||
       int64_t(d->max_tokens) * d->axes > kLimit32 || int64_t(d->max_tokens) > (1 << 24) ||
       (int64_t(d->table_entries) * d->page_size / kTileKeys + 2 * d->max_sequences) * head_tiles(d) > kLimit32) {
@@ -82,11 +82,21 @@ bool desc_ok(const lf_fp8_attn_desc *d) {
   return d != nullptr && d->magic == LF_FP8_ATTN_MAGIC && fields_ok(d) && strides_ok(d);
 }
 
-// The decode workspace: a 256-byte header (error word, the step's plan), the
-// tile prefix of the step's sequences, then two partial results per block:
-// fp32 [16][D] sums, 16 maxima and 16 weight sums.
-int64_t prefix_bytes(const lf_fp8_attn_desc *d) { return align_up((int64_t(d->max_sequences) + 1) * 4, 256); }
-int64_t slot_bytes(const lf_fp8_attn_desc *d) { return (kHeadTile * d->head_dim + 2 * kHeadTile) * 4; }
+int64_t tile_rows(const lf_fp8_attn_desc *d) {
+  return std::min<int64_t>(d->query_heads / d->kv_heads, kHeadTile);
+}
+
+// kernels/attention.hip, blocks: blocks of the decode grid.
+int64_t decode_blocks(const lf_fp8_attn_desc *d) { return d->head_dim == 64 ? 512 : 256; }
+
+// The decode workspace: a line with the error word, two arrival counters per
+// partial result, two partial results per block (fp32 [rows][D] sums, maxima
+// and weight sums of a head tile's rows) and the groups' sums.
+int64_t decode_bytes(const lf_fp8_attn_desc *d) {
+  const int64_t places = 2 * decode_blocks(d);
+  return LF_FP8_ATTN_STATUS_BYTES + 2 * places * 4 +
+         (places + places / kGroup + 2) * tile_rows(d) * (d->head_dim + 2) * 4;
+}
 
 }  // namespace
 
@@ -150,9 +160,7 @@ int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc 
   if (!desc_ok(d)) return -1;
   switch (entry) {
     case LF_FP8_ATTN_QK_NORM_ROPE: return LF_FP8_ATTN_STATUS_BYTES;
-    case LF_FP8_ATTN_DECODE:
-    case LF_FP8_ATTN_JOIN:
-      return LF_FP8_ATTN_STATUS_BYTES + prefix_bytes(d) + 2 * kDecodeBlocks * slot_bytes(d);
+    case LF_FP8_ATTN_DECODE: return decode_bytes(d);
     default: return -1;
   }
 }
@@ -167,16 +175,10 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
       gx = d->max_tokens;
       std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_qk_norm_rope_%s", type);
       break;
-    case LF_FP8_ATTN_DECODE: {
-      const int64_t rows = std::min<int64_t>(d->query_heads / d->kv_heads, kHeadTile);
-      gx = kDecodeBlocks;
-      lds = align_up((int64_t(d->max_sequences) + 1) * 4, 16) + kWaves * rows * (d->head_dim + 2) * 4;
+    case LF_FP8_ATTN_DECODE:
+      gx = decode_blocks(d);
+      lds = align_up((int64_t(d->max_sequences) + 1) * 4, 16) + kWaves * tile_rows(d) * (d->head_dim + 4) * 4;
       std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_decode_d%d_%s", d->head_dim, type);
-      break;
-    }
-    case LF_FP8_ATTN_JOIN:
-      gx = (int64_t(d->max_sequences) * d->query_heads + kWaves - 1) / kWaves;
-      std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_join_d%d", d->head_dim);
       break;
     default: return LF_INVALID_ARGUMENT;
   }

@@ -5,6 +5,7 @@
 #include "device_common.h"
 
 #include "attention_index.h"
+#include "phases.h"
 
 namespace attn {
 
@@ -178,31 +179,138 @@ LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, con
 
 // ---- attention of one new token per sequence -------------------------------
 
-// The step's work in tiles of 128 keys: (sequence, head tile, key tile), key
-// tiles innermost, cut into equal ranges of `share` tiles, one per block. A
-// pair (sequence, head tile) that one block holds whole is finished there;
-// others leave a partial result per block (fp32 sums, maximum and weight sum
-// of each of its 16 rows), which the join adds up in block order.
+// The step's work is cut into tiles of 32 keys, (sequence, head tile, key tile)
+// with key tiles innermost, and the tiles into equal ranges, one per block,
+// whose four waves take a pair's tiles in turn and join through LDS. A pair
+// (sequence, head tile) that one block holds whole is finished there. Other
+// blocks leave a partial result (fp32 sums, maximum and weight sum of each of
+// the tile's rows) in the workspace; of every kGroup neighbours the last to
+// arrive adds the group's up in order, and the last group to arrive the
+// groups'. Partial results are stored and loaded at agent scope (past the XCD's
+// L2), and a block counts itself only once its stores have completed.
 constexpr int kWaves = 4;
-constexpr int kBlocks = 1024;
 
-// Workspace: error word, live sequences, share, then the tile prefix and two
-// partial results per block (first range of the block, last one).
+// Blocks of the grid: one per CU, two with heads of 64 values (half the bytes in
+// flight per wave).
+template <int D>
+LF_DEVICE constexpr int blocks() { return D == 64 ? 512 : 256; }
+
+// Workspace: a line with the error word, arrival counters of groups (at their
+// first part's place) and of pairs (at theirs), the partial results, two per
+// block, and the groups' sums.
 struct Ws {
-  int *head;
-  int *prefix;
-  float *slots;
+  int *error, *group_arrivals, *pair_arrivals;
+  float *parts, *groups;
+  int floats;  // of a partial result: [rows][D] sums, rows maxima, rows weight sums
 };
-LF_DEVICE Ws ws_of(const Desc &d, uint8_t *ws) {
+template <int D>
+LF_DEVICE Ws ws_of(uint8_t *ws, int tile_rows) {
+  constexpr int places = 2 * blocks<D>();
   Ws w;
-  w.head = reinterpret_cast<int *>(ws);
-  w.prefix = reinterpret_cast<int *>(ws + 256);
-  w.slots = reinterpret_cast<float *>(ws + 256 + align256((static_cast<uint64_t>(d.max_sequences) + 1) * 4));
+  w.error = reinterpret_cast<int *>(ws);
+  w.group_arrivals = reinterpret_cast<int *>(ws + 256);
+  w.pair_arrivals = w.group_arrivals + places;
+  w.parts = reinterpret_cast<float *>(w.pair_arrivals + places);
+  w.floats = tile_rows * (D + 2);
+  w.groups = w.parts + static_cast<uint64_t>(places) * w.floats;
   return w;
 }
-template <int D>
-LF_DEVICE float *slot_of(const Ws &w, int slot) {
-  return w.slots + static_cast<uint64_t>(slot) * (kHeadTile * D + 2 * kHeadTile);
+
+LF_DEVICE float load_agent(const float *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+LF_DEVICE void store_agent(float *p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Counts this block, whose stores at agent scope came before; true for the last
+// of `total`, which puts the counter back to zero.
+LF_DEVICE bool arrive(int *counter, int total, int *flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (before == total - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = before == total - 1 ? 1 : 0;
+  }
+  __syncthreads();
+  const bool last = __builtin_amdgcn_readfirstlane(*flag) != 0;
+  asm volatile("" ::: "memory");
+  return last;
+}
+
+// The block adds up `count` partial results of `rows` rows in their order, the
+// first at float `first` of `from` and the p-th of the others at rest + p step,
+// and hands every value on: write(row, column, sum, weight sum, maximum).
+// kGroup results of a few values per thread are in flight at a time. stats:
+// LDS, the maxima and weight sums of kGroup results. (The empty asm keeps the
+// compiler from holding an address per result and thread.)
+template <int D, class W>
+LF_DEVICE void add_parts(const float *from, int first, int rest, int step, int count, int rows, int tile_rows,
+                         float (*stats)[kGroup][kHeadTile], W &&write) {
+  constexpr int kThreads = 64 * kWaves, kAtOnce = 2;
+  static_assert(2 * kThreads == kGroup * kHeadTile, "two statistics per thread");
+  for (int x0 = 0; x0 < rows * D; x0 += kAtOnce * kThreads) {
+    float acc[kAtOnce], sum[kAtOnce], top[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) acc[i] = sum[i] = 0.0f, top[i] = -INFINITY;
+    for (int p0 = 0; p0 < count; p0 += kGroup) {
+      float v[kGroup][kAtOnce];
+#pragma unroll
+      for (int p = 0; p < kGroup; ++p) {
+        const int part = p0 + p < count ? p0 + p : p0;
+        uint32_t at = static_cast<uint32_t>(part == 0 ? first : rest + part * step);
+        asm("" : "+s"(at));
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int x = x0 + i * kThreads + static_cast<int>(threadIdx.x);
+          v[p][i] = load_agent(from + at + static_cast<uint32_t>(x < rows * D ? x : 0));
+        }
+      }
+      const int sr = threadIdx.x % kHeadTile;
+      float m[2], l[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int sp = p0 + static_cast<int>(threadIdx.x) / kHeadTile + i * (kGroup / 2);
+        const bool some = sp < count && sr < rows;
+        const float *src = from + (sp == 0 || !some ? first : rest + sp * step) + tile_rows * D + (some ? sr : 0);
+        m[i] = load_agent(src);
+        l[i] = load_agent(src + tile_rows);
+        m[i] = some ? m[i] : -INFINITY;
+        l[i] = some ? l[i] : 0.0f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        stats[0][threadIdx.x / kHeadTile + i * (kGroup / 2)][sr] = m[i];
+        stats[1][threadIdx.x / kHeadTile + i * (kGroup / 2)][sr] = l[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int x = x0 + i * kThreads + static_cast<int>(threadIdx.x), r = x < rows * D ? x / D : 0;
+        float next = top[i];
+#pragma unroll
+        for (int p = 0; p < kGroup; ++p) next = fmaxf(next, stats[0][p][r]);
+        const float base = next == -INFINITY ? 0.0f : next;
+        const float keep = __builtin_amdgcn_exp2f(top[i] - base);
+        top[i] = next;
+        acc[i] *= keep;
+        sum[i] *= keep;
+#pragma unroll
+        for (int p = 0; p < kGroup; ++p) {
+          const float f = __builtin_amdgcn_exp2f(stats[0][p][r] - base);
+          sum[i] += f * stats[1][p][r];
+          acc[i] += p0 + p < count ? f * v[p][i] : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int x = x0 + i * kThreads + static_cast<int>(threadIdx.x);
+      if (x < rows * D) write(x / D, x % D, acc[i], sum[i], top[i]);
+    }
+  }
 }
 
 // Keys and values of 32 consecutive keys in a wave's registers.
@@ -239,9 +347,86 @@ LF_DEVICE void load_words(uint32_t (&dst)[WORDS], const uint8_t *src) {
   }
 }
 
+template <int WORDS>
+LF_DEVICE void store_words(uint16_t *dst, const uint32_t (&src)[WORDS]) {
+  if constexpr (WORDS == 2) {
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(src[0], src[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4)
+      *reinterpret_cast<u32x4 *>(dst + 2 * i) = u32x4{src[i], src[i + 1], src[i + 2], src[i + 3]};
+  }
+}
+
 LF_DEVICE bf16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_bit_cast(bf16x8, u32x4{a, b, c, d});
 }
+
+// Where a tile's four groups of keys are: byte offsets of their first rows from
+// the head's first, and which of them lie in the cache.
+struct Groups {
+  uint64_t at0, at1, at2, at3;
+  int in;
+};
+// page: the groups' page indices in lanes 0 .. 3.
+LF_DEVICE Groups groups_of(int page, int pages, uint32_t page_bytes, uint32_t token_bytes, int slot_mask, int base) {
+  int in = 0;
+  auto at = [&](int p, int k) {
+    const bool ok = static_cast<uint32_t>(p) < static_cast<uint32_t>(pages);
+    in |= ok ? 1 << k : 0;
+    return static_cast<uint64_t>(static_cast<uint32_t>(ok ? p : 0)) * page_bytes +
+           static_cast<uint64_t>(static_cast<uint32_t>((base + 8 * k) & slot_mask)) * token_bytes;
+  };
+  const uint64_t a = at(__builtin_amdgcn_readlane(page, 0), 0), b = at(__builtin_amdgcn_readlane(page, 1), 1);
+  const uint64_t c = at(__builtin_amdgcn_readlane(page, 2), 2), d = at(__builtin_amdgcn_readlane(page, 3), 3);
+  return {a, b, c, d, in};
+}
+LF_DEVICE uint64_t pick(bool first, uint64_t a, uint64_t b) { return first ? a : b; }
+
+// keys: this lane's part of the first row of its group of eight (c % 8 rows
+// further, chunk g); values: that of row 4 g of its half.
+template <int D, bool E4M3>
+LF_DEVICE void load_keys(Tile<D, E4M3> &x, const uint8_t *keys, const Groups &at, int c) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint8_t *src = keys + pick(c < 8, half == 0 ? +at.at0 : +at.at2, half == 0 ? +at.at1 : +at.at3);
+#pragma unroll
+    for (int k = 0; k < Tile<D, E4M3>::kChunks; ++k) x.k[half][k] = *reinterpret_cast<const u32x4 *>(src + 64 * k);
+  }
+}
+template <int D, bool E4M3>
+LF_DEVICE void load_values(Tile<D, E4M3> &x, const uint8_t *values, const Groups &at, uint32_t token_bytes, int g) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint8_t *src = values + pick(g < 2, half == 0 ? +at.at0 : +at.at2, half == 0 ? +at.at1 : +at.at3);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) load_words(x.v[4 * half + e], src + static_cast<uint64_t>(e) * token_bytes);
+  }
+}
+
+// The larger of a value over the four lane groups, in all of them.
+LF_DEVICE float max_over_groups(float v) {
+  const uint32_t a = __float_as_uint(v);
+  const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const uint32_t b = __float_as_uint(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+  const auto y = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
+// A part of a pair: the tiles of keys [base, stop) of a sequence whose keys [lo,
+// len) count, stop at most len, for `live` query heads from head `row0` of key head h's group on.
+struct Piece {
+  const int32_t *table;
+  int lo, len, base, stop;
+  int h, row0, live, row;  // row of q and out, or -1
+  int pair, tiles;         // its pair's first item and tiles
+};
+
+// What a block keeps of each of the first sequences in LDS.
+struct Sequence {
+  Span span;
+  int entry, row;  // first page table entry, row of q and out
+};
 
 template <int D, bool E4M3>
 LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths,
@@ -249,19 +434,36 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
                       const uint16_t *q, uint16_t *out, const uint8_t *kc, const uint8_t *vc, uint8_t *ws) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ int wave_total[kWaves];
+  __shared__ int arrived;
+  __shared__ float stats[2][kGroup][kHeadTile];
+  __shared__ Sequence near[64 * kWaves];
   const Desc &d = desc_of(attn);
-  if (d.magic != kMagic) return;
-  const Ws w = ws_of(d, ws);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rows = live_rows(counts, d.max_tokens);
-  const int s0 = decoded_of(d, counts).s0, n = decoded_of(d, counts).n;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // (the loads before the first wait: each further round trip to memory delays
+  // every block's first keys)
+  const int magic = d.magic, count0 = counts[0], count1 = counts[1], count2 = counts[2];
+  int rows = counts[kQueryTokensIndex];
+  rows = rows < 0 ? 0 : rows > d.max_tokens ? d.max_tokens : rows;
+  if (magic != static_cast<int>(kMagic)) return;
+  const Decoded decoded = decoded_of(d, count0, count1, count2);
+  const int s0 = decoded.s0, n = decoded.n;
+  auto load_sequence = [&](int s, bool &is_bad) {
+    const int len = lengths[s], first = page_offsets[s], end = page_offsets[s + 1], row = row_offsets[s];
+    const Pages pages = pages_of(d, first, end, is_bad);
+    return Sequence{span_of(d, len, pages, is_bad), pages.first, row};
+  };
 
   int *prefix = reinterpret_cast<int *>(lds);
   bool bad = false;
   int64_t carry = 0;
   for (int base = 0; base < n; base += 256) {
     const int i = base + static_cast<int>(threadIdx.x);
-    const int tiles = i < n ? span_of(d, lengths, page_offsets, s0 + i, bad).tiles : 0;
+    int tiles = 0;
+    if (i < n) {
+      const Sequence q1 = load_sequence(s0 + i, bad);
+      tiles = q1.span.tiles;
+      if (base == 0) near[i] = q1;
+    }
     int sum = tiles;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -287,91 +489,126 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   // (page ranges that overlap may add up to more than the descriptor's bound)
   const bool counted = carry * head_tiles <= INT32_MAX;
   if (!counted) bad = true;
-  const int items = counted ? static_cast<int>(carry) * head_tiles : 0;
-  const int share = share_of(items, kBlocks);
-  if (blockIdx.x == 0) {
-    if (threadIdx.x == 0) {
-      w.head[1] = n;
-      w.head[2] = share;
-      w.head[3] = s0;
-    }
-    for (int i = threadIdx.x; i <= n; i += 256) w.prefix[i] = prefix[i];
-  }
-  if (bad) flag_error(w.head);
-  if (share == 0) return;
-  const int begin = static_cast<int>(blockIdx.x) * share;
-  const int end = begin + share < items ? begin + share : items;
+  const int items = __builtin_amdgcn_readfirstlane(counted ? static_cast<int>(carry) * head_tiles : 0);
+  const int share = share_of(items, n * head_tiles, blocks<D>());
+  const int tile_rows = group < kHeadTile ? group : kHeadTile;
+  const Ws w = ws_of<D>(ws, tile_rows);
+  if (bad) flag_error(w.error);
 
   const int shift = __builtin_ctz(d.page_size);
+  constexpr uint32_t kSize = E4M3 ? 1 : 2;
+  const uint32_t page_bytes = static_cast<uint32_t>(d.page_stride) * kSize;
+  const uint32_t token_bytes = static_cast<uint32_t>(d.token_stride) * kSize;
+  const int slot_mask = d.page_size - 1, pages = d.pages;
   const float *scales = reinterpret_cast<const float *>(attn + d.scale_offset);
   const int g = lane >> 4, c = lane & 15;
-  const int tile_rows = group < kHeadTile ? group : kHeadTile;
-  float *join = reinterpret_cast<float *>(lds + ((static_cast<uint64_t>(d.max_sequences) * 4 + 4 + 15) & ~uint64_t(15)));
 
-  for (int u = begin; u < end;) {
-    const int i = sequence_at(prefix, n, head_tiles, u);
-    const int s = s0 + i;
-    bool unused = false;
-    const Span span = span_of(d, lengths, page_offsets, s, unused);
-    const Pages pages = pages_of(d, page_offsets, s, unused);
-    const int32_t *table = page_indices + pages.first;
-    const int first_page = span.lo >> shift, end_page = (span.len + d.page_size - 1) >> shift;
-    const int within = u - prefix[i] * head_tiles;
-    const int ht = within / span.tiles, t0 = within - ht * span.tiles;
-    const int t1 = span.tiles - t0 < end - u ? span.tiles : t0 + (end - u);
-    const int h = ht / group_tiles;
-    const int row0 = (ht - h * group_tiles) * kHeadTile;  // first query head of the tile in its group
-    const int tile_live = group - row0 < kHeadTile ? group - row0 : kHeadTile;
-    const int row = row_offsets[s];
-    const bool row_ok = row >= 0 && row < rows;
-    if (!row_ok) bad = true;
+  const int block = blockIdx.x;
+  const int64_t begin64 = static_cast<int64_t>(block) * share;
+  if (begin64 >= items) return;
+  int u = static_cast<int>(begin64);
+  const int end = items - u < share ? items : u + share;
 
-    // B operand of the first product: query head c, the values of its key chunk
-    bf16x8 qv[D / 32];
-    {
-      const uint16_t *src = q + (static_cast<uint64_t>(row_ok ? row : 0) * Hq + h * group + row0 + c) * D;
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        // bf16 keys: chunk k holds values 32 k + 8 g ..; e4m3: 64 (k / 2) + 16 g + 8 (k % 2) ..
-        const int at = E4M3 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 32 * k + 8 * g;
-        qv[k] = c < tile_live && row_ok ? *reinterpret_cast<const bf16x8 *>(src + at) : operand(0, 0, 0, 0);
+  // the next part of a pair in the block's range
+  auto take = [&](Piece &x) {
+    while (u < end) {
+      const int i = __builtin_amdgcn_readfirstlane(sequence_at(prefix, n, head_tiles, u));
+      bool unused = false;
+      const Sequence seq = i < 64 * kWaves ? near[i] : load_sequence(s0 + i, unused);
+      const Span span = {__builtin_amdgcn_readfirstlane(seq.span.first_tile), __builtin_amdgcn_readfirstlane(seq.span.tiles),
+                         __builtin_amdgcn_readfirstlane(seq.span.lo), __builtin_amdgcn_readfirstlane(seq.span.len)};
+      const int within = u - __builtin_amdgcn_readfirstlane(prefix[i]) * head_tiles;
+      const int ht = within / span.tiles, t0 = within - ht * span.tiles;
+      const int t1 = span.tiles - t0 < end - u ? span.tiles : t0 + (end - u);
+      x.pair = u - t0;
+      x.tiles = span.tiles;
+      x.h = ht / group_tiles;
+      x.row0 = (ht - x.h * group_tiles) * kHeadTile;
+      x.live = group - x.row0 < kHeadTile ? group - x.row0 : kHeadTile;
+      x.row = __builtin_amdgcn_readfirstlane(seq.row);
+      if (x.row < 0 || x.row >= rows) {
+        x.row = -1;
+        bad = true;
+      }
+      x.table = page_indices + __builtin_amdgcn_readfirstlane(seq.entry);
+      x.lo = span.lo;
+      x.len = span.len;
+      x.base = (span.first_tile + t0) * kTileKeys;
+      x.stop = (span.first_tile + t1) * kTileKeys < span.len ? (span.first_tile + t1) * kTileKeys : span.len;
+      u += t1 - t0;
+      if (span.len > 0) return true;
+      if (x.row >= 0) {  // no keys
+        uint16_t *dst = out + (static_cast<uint64_t>(x.row) * Hq + x.h * group + x.row0) * D;
+        for (int k = threadIdx.x; k < x.live * D; k += 64 * kWaves) dst[k] = 0;
       }
     }
-    const float factor = d.softmax_scale * 1.44269504088896341f * (E4M3 ? scales[h] : 1.0f);
-    const uint8_t *kh = kc + cache_byte<E4M3>(d, 0, h, 0);
-    const uint8_t *vh = vc + cache_byte<E4M3>(d, 0, h, 0);
+    return false;
+  };
+  auto indices = [&](const int32_t *table, int lo, int len, int base) {
+    return table[entry_of(lo >> shift, (len + slot_mask) >> shift, shift, base + 8 * (lane & 3))];
+  };
+  auto tile_groups = [&](int page, int base) { return groups_of(page, pages, page_bytes, token_bytes, slot_mask, base); };
+  // this lane's part of a head's rows: of keys, row c % 8 of a group of eight,
+  // chunk g; of values, row 4 g of a half
+  const uint32_t key_lane = (c & 7) * token_bytes + 16 * g;
+  const uint32_t value_lane = (4 * g & 7) * token_bytes + c * (D / 16 * kSize);
+  const uint32_t head_bytes = static_cast<uint32_t>(d.head_stride) * kSize;
+  auto keys_of = [&](uint32_t h) { return kc + static_cast<uint64_t>(h) * head_bytes + key_lane; };
+  auto values_of = [&](uint32_t h) { return vc + static_cast<uint64_t>(h) * head_bytes + value_lane; };
+  // B operand of the first product: query head c, the values of its key chunk
+  bf16x8 qv[D / 32];
+  auto load_queries = [&](const Piece &x) {
+    const uint16_t *src =
+        q + (static_cast<uint64_t>(x.row < 0 ? 0 : x.row) * Hq + x.h * group + x.row0 + (c < x.live ? c : 0)) * D;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      // bf16 keys: chunk k holds values 32 k + 8 g ..; e4m3: 64 (k / 2) + 16 g + 8 (k % 2) ..
+      const int at = E4M3 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 32 * k + 8 * g;
+      qv[k] = *reinterpret_cast<const bf16x8 *>(src + at);
+    }
+  };
 
+  // Loads run one tile ahead, over the ends of pieces too: keys, values and
+  // queries each into the registers just consumed, page indices one further.
+  // The wave's tiles of a piece are its own-th of every four; a piece without one
+  // for it gives it one tile of keys that are all masked.
+  constexpr int kStep = kWaves * kTileKeys;
+  auto take_mine = [&](Piece &x) {
+    const bool some = take(x);
+    x.base += wave * kTileKeys;
+    return some;
+  };
+  Piece now, next;
+  if (!take_mine(now)) {
+    if (bad) flag_error(w.error);
+    return;
+  }
+  Tile<D, E4M3> x;
+  Groups at = tile_groups(indices(now.table, now.lo, now.len, now.base), now.base);
+  load_keys(x, keys_of(now.h), at, c);
+  load_queries(now);
+  int ahead = indices(now.table, now.lo, now.len, now.base + kStep);
+  asm volatile("" ::: "memory");  // values last, as in the loop
+  load_values(x, values_of(now.h), at, token_bytes, g);
+  bool has_next = take_mine(next);
+  if (!has_next) next = now;  // what is loaded behind the last tile
+  auto after_one_tile = [&]() {  // a piece of one tile: the tile ahead is the next piece's
+    if (now.base + kStep >= now.stop) {
+      ahead = indices(next.table, next.lo, next.len, next.base);
+      asm volatile("" : "+v"(ahead));  // waited for here, not where every tile's is
+    }
+  };
+  after_one_tile();
+
+  for (;;) {
+    const float factor = d.softmax_scale * 1.44269504088896341f * (E4M3 ? scales[now.h] : 1.0f);
     f32x4 o[D / 16];
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     f32x4 sum4 = {0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY;
-
-    for (int t = t0; t < t1; ++t) {
-      const int base = (span.first_tile + t) * kTileKeys + 32 * wave;
-      if (base >= span.len || base + 32 <= span.lo) continue;
-      Tile<D, E4M3> x;
-      int vpage[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int j = base + 16 * half + c;
-        const int page = page_of(d, table, first_page, end_page, shift, j, bad);
-        const uint8_t *src = kh + cache_byte<E4M3>(d, page < 0 ? 0 : page, 0, j & (d.page_size - 1)) + 16 * g;
-#pragma unroll
-        for (int k = 0; k < Tile<D, E4M3>::kChunks; ++k) x.k[half][k] = *reinterpret_cast<const u32x4 *>(src + 64 * k);
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int j = base + 16 * half + 4 * g;  // four keys of one page
-        vpage[half] = page_of(d, table, first_page, end_page, shift, j, bad);
-        const uint8_t *src = vh + cache_byte<E4M3>(d, vpage[half] < 0 ? 0 : vpage[half], 0, j & (d.page_size - 1)) +
-                             c * (D / 16 * Tile<D, E4M3>::kSize);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          load_words(x.v[4 * half + e], src + static_cast<uint64_t>(e) * static_cast<uint32_t>(d.token_stride) *
-                                                  Tile<D, E4M3>::kSize);
-        }
-      }
+    int base = now.base;
+    do {
       // scores: rows = keys 16 half + 4 g + r, column = query head c
       f32x4 sc[2];
 #pragma unroll
@@ -393,16 +630,28 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
           }
         }
       }
+      // The tile after this one, in this piece or the next; behind the last, any.
+      // (All loads are issued on every path: a load that a branch may skip makes
+      // the wait for an older one a wait for all.)
+      const bool more = base + kStep < now.stop;
+      const Groups then = tile_groups(ahead, more ? base + kStep : next.base);
+      const uint32_t then_h = more ? now.h : next.h;
+      load_keys(x, keys_of(then_h), then, c);
+      if (!more) load_queries(next);
+      {
+        const bool same = base + 2 * kStep < now.stop;
+        ahead = indices(same ? now.table : next.table, same ? now.lo : next.lo, same ? now.len : next.len,
+                        same ? base + 2 * kStep : more ? next.base : next.base + kStep);
+      }
       float z[8];
-      const bool edge = base < span.lo || base + 32 > span.len;
-      const bool masked = __any(edge || vpage[0] < 0 || vpage[1] < 0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = sc[e >> 2][e & 3] * factor;
-      if (masked) {
+      if (at.in != 15 && base < now.stop) bad = true;
+      if (base < now.lo || base + kTileKeys > now.stop || at.in != 15) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = base + 16 * (e >> 2) + 4 * g + (e & 3);
-          const bool live = j >= span.lo && j < span.len && vpage[e >> 2] >= 0;
+          const bool live = j >= now.lo && j < now.stop && ((at.in >> (2 * (e >> 2) + (g >> 1))) & 1) != 0;
           z[e] = live ? z[e] : -INFINITY;
           // a weight of zero times what the place holds would let an infinity or NaN through
 #pragma unroll
@@ -412,17 +661,14 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       float most = z[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) most = fmaxf(most, z[e]);
-      most = fmaxf(most, __shfl_xor(most, 16));
-      most = fmaxf(most, __shfl_xor(most, 32));
-      if (__any(most > top)) {
-        const float next = fmaxf(top, most);
-        const float shrink = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.0f : next));
-        top = next;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) o[k] *= shrink;
-        sum4 *= shrink;
-      }
+      most = max_over_groups(most);
+      const float before = top;
+      top = fmaxf(top, most);
       const float from = top == -INFINITY ? 0.0f : top;
+      const float shrink = __builtin_amdgcn_exp2f(before - from);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) o[k] *= shrink;
+      sum4 *= shrink;
       uint32_t pw[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -454,17 +700,23 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
         for (int e = 0; e < 4; ++e) a[e] = __builtin_amdgcn_perm(vp[2 * e + 1][k >> 1], vp[2 * e][k >> 1], sel);
         o[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(a[0], a[1], a[2], a[3]), p, o[k], 0, 0, 0);
       }
-    }
+      load_values(x, values_of(then_h), then, token_bytes, g);
+      at = then;
+      base += kStep;
+    } while (base < now.stop);
 
-    // The four waves' results joined in wave order. o[k][r] is the sum of
-    // query head c at column (4 g + r) D / 16 + k.
-    float *mine = join + static_cast<uint64_t>(wave) * tile_rows * (D + 2);
-    if (c < tile_live) {
-      float *dst = mine + c * (D + 2);
+    // The waves' results joined in wave order. o[k][r] is the sum of query head
+    // c at column (4 g + r) D / 16 + k.
+    float *join = reinterpret_cast<float *>(lds + ((static_cast<uint32_t>(d.max_sequences) * 4 + 4 + 15) & ~15u));
+    constexpr int kRow = D + 4;  // of a row in LDS: D sums, maximum, weight sum
+    if (c < now.live) {
+      float *dst = join + (wave * tile_rows + c) * kRow;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) dst[(4 * g + r) * (D / 16) + k] = o[k][r];
+        for (int k = 0; k < D / 16; k += 4)
+          *reinterpret_cast<f32x4 *>(dst + (4 * g + r) * (D / 16) + k) =
+              f32x4{o[k][r], o[k + 1][r], o[k + 2][r], o[k + 3][r]};
       }
       if (g == 0) {
         dst[D] = top;
@@ -472,100 +724,91 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       }
     }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == span.tiles;
-    float *slot = slot_of<D>(w, part_slot(blockIdx.x, u - t0, share));
-    const float vscale = E4M3 ? scales[Hkv + h] : 1.0f;
-    for (int x = threadIdx.x; x < tile_live * D; x += 256) {
-      const int r = x / D, col = x % D;
-      const float *src = join + r * (D + 2);
+    const Parts parts = parts_of(now.pair, now.tiles, share);
+    const bool whole = parts.first == parts.last;
+    const float vscale = E4M3 ? scales[Hkv + now.h] : 1.0f;
+    const int live = now.live;
+    uint16_t *dst = out + (static_cast<uint64_t>(now.row < 0 ? 0 : now.row) * Hq + now.h * group + now.row0) * D;
+    float *part = w.parts + static_cast<uint64_t>(part_slot(block, now.pair, share)) * w.floats;
+    auto finish = [&](int r, int col, float acc, float sum) {
+      if (now.row >= 0) dst[r * D + col] = static_cast<uint16_t>(f32_to_bf16(sum == 0.0f ? 0.0f : acc / sum * vscale));
+    };
+    for (int x1 = threadIdx.x; x1 < live * D; x1 += 64 * kWaves) {
+      const int r = x1 / D, col = x1 % D;
+      const float *src = join + r * kRow;
       float m = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) m = fmaxf(m, src[k * tile_rows * (D + 2) + D]);
+      for (int k = 0; k < kWaves; ++k) m = fmaxf(m, src[k * tile_rows * kRow + D]);
       const float from = m == -INFINITY ? 0.0f : m;
       float acc = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < kWaves; ++k) {
-        const float *p = src + k * tile_rows * (D + 2);
+        const float *p = src + k * tile_rows * kRow;
         const float f = __builtin_amdgcn_exp2f(p[D] - from);
         acc += f * p[col];
         sum += f * p[D + 1];
       }
       if (whole) {
-        const float y = sum == 0.0f ? 0.0f : acc / sum * vscale;
-        if (row_ok) {
-          out[(static_cast<uint64_t>(row) * Hq + h * group + row0 + r) * D + col] =
-              static_cast<uint16_t>(f32_to_bf16(y));
-        }
+        finish(r, col, acc, sum);
       } else {
-        slot[r * D + col] = acc;
+        store_agent(part + x1, acc);
         if (col == 0) {
-          slot[kHeadTile * D + r] = m;
-          slot[kHeadTile * D + kHeadTile + r] = sum;
+          store_agent(part + tile_rows * D + r, m);
+          store_agent(part + tile_rows * (D + 1) + r, sum);
         }
       }
     }
-    __syncthreads();
-    u += t1 - t0;
+    if (!whole) {
+      const int count = parts.last - parts.first + 1, group_count = (count + kGroup - 1) / kGroup;
+      const int start = parts.first + (block - parts.first) / kGroup * kGroup;
+      const int in_group = parts.last + 1 - start < kGroup ? parts.last + 1 - start : kGroup;
+      // the group's parts, then, if there are several groups, their sums
+      float *sums = w.groups + static_cast<uint64_t>(group_slot(start, parts.first)) * w.floats;
+      const float *from = w.parts;
+      int first = part_slot(start, now.pair, share) * w.floats, rest = 2 * start * w.floats, adds = in_group;
+      bool done = group_count == 1;
+      bool go_on = arrive(w.group_arrivals + part_slot(start, now.pair, share), in_group, &arrived);
+      while (go_on) {
+        add_parts<D>(from, first, rest, 2 * w.floats, adds, live, tile_rows, stats,
+                     [&](int r, int col, float acc, float sum, float m) {
+                       if (done) {
+                         finish(r, col, acc, sum);
+                       } else {
+                         store_agent(sums + r * D + col, acc);
+                         if (col == 0) {
+                           store_agent(sums + tile_rows * D + r, m);
+                           store_agent(sums + tile_rows * (D + 1) + r, sum);
+                         }
+                       }
+                     });
+        go_on = !done && arrive(w.pair_arrivals + part_slot(parts.first, now.pair, share), group_count, &arrived);
+        done = true;
+        adds = group_count;
+        from = w.groups;
+        first = group_slot(parts.first, parts.first) * w.floats;
+        rest = first - w.floats;
+      }
+    }
+    __syncthreads();  // the join area has been read
+    if (!has_next) break;
+    now = next;
+    has_next = take_mine(next);
+    if (!has_next) next = now;
+    after_one_tile();
   }
-  if (bad) flag_error(w.head);
-}
-
-// One wave per (sequence, query head): the partial results of its pair, in
-// block order; pairs that one block finished are left alone.
-template <int D>
-LF_DEVICE void join(const int32_t *counts, const int32_t *row_offsets, const uint8_t *attn, uint16_t *out,
-                    uint8_t *ws) {
-  const Desc &d = desc_of(attn);
-  if (d.magic != kMagic) return;
-  const Ws w = ws_of(d, ws);
-  const int lane = threadIdx.x & 63;
-  const int item = static_cast<int>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-  const int Hq = d.query_heads, Hkv = d.kv_heads, group = Hq / Hkv;
-  const int i = item / Hq, qh = item - i * Hq;
-  const int n = w.head[1], share = w.head[2];
-  if (i >= n || share <= 0) return;
-  const int row = row_offsets[w.head[3] + i];
-  if (row < 0 || row >= live_rows(counts, d.max_tokens)) return;
-  const int group_tiles = (group + kHeadTile - 1) / kHeadTile;
-  const int h = qh / group, in_group = qh - h * group;
-  const int ht = h * group_tiles + in_group / kHeadTile, r = in_group & (kHeadTile - 1);
-  const int tiles = w.prefix[i + 1] - w.prefix[i];
-  const int begin = w.prefix[i] * head_tiles_of(d) + ht * tiles;
-  const Parts parts = parts_of(begin, tiles, share);
-  if (parts.first == parts.last) return;
-  constexpr int kPer = D / 64;
-  float m = -INFINITY;
-  for (int b = parts.first; b <= parts.last; ++b) {
-    const float *slot = slot_of<D>(w, part_slot(b, begin, share));
-    m = fmaxf(m, slot[kHeadTile * D + r]);
-  }
-  const float from = m == -INFINITY ? 0.0f : m;
-  float acc[kPer], sum = 0.0f;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-  for (int b = parts.first; b <= parts.last; ++b) {
-    const float *slot = slot_of<D>(w, part_slot(b, begin, share));
-    const float f = __builtin_amdgcn_exp2f(slot[kHeadTile * D + r] - from);
-    sum += f * slot[kHeadTile * D + kHeadTile + r];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[e] += f * slot[r * D + lane * kPer + e];
-  }
-  const float *scales = reinterpret_cast<const float *>(attn + d.scale_offset);
-  const float vscale = scales[Hkv + h];
-  uint16_t *dst = out + (static_cast<uint64_t>(row) * Hq + qh) * D + lane * kPer;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    dst[e] = static_cast<uint16_t>(f32_to_bf16(sum == 0.0f ? 0.0f : acc[e] / sum * vscale));
-  }
+  if (bad) flag_error(w.error);
 }
 
 }  // namespace attn
 
 #define LF_ATTN_ROPE(TYPE, E4M3)                                                                             \
   extern "C" __global__ __launch_bounds__(256) void lf_attn_qk_norm_rope_##TYPE(                             \
-      const int32_t *counts, const int32_t *positions, const int32_t *row_offsets, const int32_t *lengths,   \
-      const int32_t *page_offsets, const int32_t *page_indices, const uint8_t *desc, const uint16_t *qkv,    \
-      const uint16_t *gq, const uint16_t *gk, uint16_t *q, uint8_t *kc, uint8_t *vc, int *status) {          \
+      const int32_t *__restrict__ counts, const int32_t *__restrict__ positions, \
+      const int32_t *__restrict__ row_offsets, const int32_t *__restrict__ lengths, \
+      const int32_t *__restrict__ page_offsets, const int32_t *__restrict__ page_indices, \
+      const uint8_t *__restrict__ desc, const uint16_t *__restrict__ qkv, \
+      const uint16_t *__restrict__ gq, const uint16_t *__restrict__ gk, uint16_t *__restrict__ q, \
+      uint8_t *__restrict__ kc, uint8_t *__restrict__ vc, int *__restrict__ status) { \
     attn::qk_norm_rope<E4M3>(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv, \
                              gq, gk, q, kc, vc, status);                                                     \
   }
@@ -573,10 +816,12 @@ LF_ATTN_ROPE(bf16, false)
 LF_ATTN_ROPE(e4m3, true)
 
 #define LF_ATTN_DECODE(D, TYPE, E4M3)                                                                          \
-  extern "C" __global__ __launch_bounds__(256) void lf_attn_decode_d##D##_##TYPE(                              \
-      const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths, const int32_t *page_offsets,  \
-      const int32_t *page_indices, const uint8_t *desc, const uint16_t *q, uint16_t *out, const uint8_t *kc,   \
-      const uint8_t *vc, uint8_t *ws) {                                                                        \
+  extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void lf_attn_decode_d##D##_##TYPE(                              \
+      const int32_t *__restrict__ counts, const int32_t *__restrict__ row_offsets, \
+      const int32_t *__restrict__ lengths, const int32_t *__restrict__ page_offsets, \
+      const int32_t *__restrict__ page_indices, const uint8_t *__restrict__ desc, \
+      const uint16_t *__restrict__ q, uint16_t *__restrict__ out, const uint8_t *__restrict__ kc, \
+      const uint8_t *__restrict__ vc, uint8_t *__restrict__ ws) { \
     attn::decode<D, E4M3>(counts, row_offsets, lengths, page_offsets, page_indices, desc, q, out, kc, vc, ws); \
   }
 LF_ATTN_DECODE(64, bf16, false)
@@ -585,12 +830,3 @@ LF_ATTN_DECODE(256, bf16, false)
 LF_ATTN_DECODE(64, e4m3, true)
 LF_ATTN_DECODE(128, e4m3, true)
 LF_ATTN_DECODE(256, e4m3, true)
-
-#define LF_ATTN_JOIN(D)                                                                                     \
-  extern "C" __global__ __launch_bounds__(256) void lf_attn_join_d##D(                                      \
-      const int32_t *counts, const int32_t *row_offsets, const uint8_t *desc, uint16_t *out, uint8_t *ws) { \
-    attn::join<D>(counts, row_offsets, desc, out, ws);                                                      \
-  }
-LF_ATTN_JOIN(64)
-LF_ATTN_JOIN(128)
-LF_ATTN_JOIN(256)

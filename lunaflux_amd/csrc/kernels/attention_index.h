@@ -21,12 +21,11 @@ struct Desc {
 };
 constexpr uint32_t kMagic = 0x4E54414Cu;
 
-// Entries of sequence s in the page table; none where the offsets leave it.
+// A sequence's entries [first, end) of the page table; none where they leave it.
 struct Pages {
   int first, count;
 };
-LF_DEVICE Pages pages_of(const Desc &d, const int32_t *offsets, int s, bool &bad) {
-  const int first = offsets[s], end = offsets[s + 1];
+LF_DEVICE Pages pages_of(const Desc &d, int first, int end, bool &bad) {
   if (first < 0 || end < first || end > d.table_entries) {
     bad = true;
     return {0, 0};
@@ -53,7 +52,7 @@ struct Place {
 LF_DEVICE Place place_of(const Desc &d, const int32_t *row_offsets, const int32_t *lengths,
                          const int32_t *page_offsets, const int32_t *page_indices, int s, int row) {
   bool bad = false;
-  const Pages pages = pages_of(d, page_offsets, s, bad);
+  const Pages pages = pages_of(d, page_offsets[s], page_offsets[s + 1], bad);
   const int64_t token = static_cast<int64_t>(lengths[s]) - row_offsets[s + 1] + row;
   const int shift = __builtin_ctz(static_cast<uint32_t>(d.page_size));
   if (token < 0 || (token >> shift) >= pages.count) return {-1, 0};
@@ -64,7 +63,7 @@ LF_DEVICE Place place_of(const Desc &d, const int32_t *row_offsets, const int32_
 
 // ---- single-token attention -------------------------------------------------------
 
-constexpr int kTileKeys = 128;
+constexpr int kTileKeys = 32;
 constexpr int kHeadTile = 16;
 
 // Keys [lo, len) of a sequence, in `tiles` tiles from the one that holds lo;
@@ -72,9 +71,7 @@ constexpr int kHeadTile = 16;
 struct Span {
   int first_tile, tiles, lo, len;
 };
-LF_DEVICE Span span_of(const Desc &d, const int32_t *lengths, const int32_t *page_offsets, int s, bool &bad) {
-  const Pages p = pages_of(d, page_offsets, s, bad);
-  int len = lengths[s];
+LF_DEVICE Span span_of(const Desc &d, int len, Pages p, bool &bad) {
   const int most = p.count * d.page_size;
   if (len < 0 || len > most) {
     bad = true;
@@ -86,18 +83,14 @@ LF_DEVICE Span span_of(const Desc &d, const int32_t *lengths, const int32_t *pag
   return {first, end > first ? end - first : 1, lo, len};
 }
 
-// Page of key j, or -1: outside the entries [first, end) that hold keys which
-// count (a released page before the window, an unused one behind the length),
-// or outside the cache.
-LF_DEVICE int page_of(const Desc &d, const int32_t *table, int first, int end, int shift, int j, bool &bad) {
+// A key tile is four groups of eight keys, each in one page. The table entry of
+// the group that starts at key j, of a sequence whose keys that count are in the
+// entries [first, end), end > first: groups before and behind those (a released
+// page before the window, an unused one behind the length) take the nearest of
+// them, and their keys are masked.
+LF_DEVICE int entry_of(int first, int end, int shift, int j) {
   const int e = j >> shift;
-  if (e < first || e >= end) return -1;
-  const int page = table[e];
-  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(d.pages)) {
-    bad = true;
-    return -1;
-  }
-  return page;
+  return e < first ? first : e < end ? e : end - 1;
 }
 
 LF_DEVICE int head_tiles_of(const Desc &d) {
@@ -109,19 +102,25 @@ LF_DEVICE int head_tiles_of(const Desc &d) {
 struct Decoded {
   int s0, n;
 };
-LF_DEVICE Decoded decoded_of(const Desc &d, const int32_t *counts) {
-  int total = counts[2], s0 = counts[0], n = counts[1];
+LF_DEVICE Decoded decoded_of(const Desc &d, int s0, int n, int total) {
   total = total < 0 ? 0 : total > d.max_sequences ? d.max_sequences : total;
   s0 = s0 < 0 ? 0 : s0 > total ? total : s0;
   n = n < 0 ? 0 : n > total - s0 ? total - s0 : n;
   return {s0, n};
 }
 
-// The step's items are the tiles of every (sequence, head tile) pair in turn:
-// pair (i, ht) starts at prefix[i] head_tiles + ht tiles(i), where prefix adds
-// up the tiles of the sequences before i. Block b holds the items
-// [b share, (b + 1) share).
-LF_DEVICE int share_of(int items, int blocks) { return (items + blocks - 1) / blocks; }
+// The step's items are the key tiles of every (sequence, head tile) pair in
+// turn: pair (i, ht) starts at prefix[i] head_tiles + ht tiles(i), where prefix
+// adds up the tiles of the sequences before i. Block b holds the items [b share,
+// (b + 1) share): a part of a pair is worth adding up from about kLeastShare
+// tiles on, and pairs shorter than that get a block each while there are enough.
+constexpr int kLeastShare = 8;
+LF_DEVICE int share_of(int items, int pairs, int blocks) {
+  if (pairs < 1) return 1;
+  const int share = (items + blocks - 1) / blocks, whole = (items + pairs - 1) / pairs;
+  const int least = whole < kLeastShare ? whole : kLeastShare;
+  return share > least ? share : least;
+}
 
 // The sequence that item u belongs to (prefix rises by at least 1 a sequence).
 LF_DEVICE int sequence_at(const int *prefix, int n, int head_tiles, int u) {
@@ -139,9 +138,9 @@ LF_DEVICE int sequence_at(const int *prefix, int n, int head_tiles, int u) {
 }
 
 // The blocks first .. last that hold parts of the pair whose items are [begin,
-// begin + tiles), and where block b leaves its part: partial result 2 b if the
-// pair is the first thing in the block's range, 2 b + 1 if it comes after
-// another (only the pair's first block can, so no two parts share a place).
+// begin + tiles), and where block b's part goes: partial result 2 b if the pair
+// is the first thing in the block's range, 2 b + 1 if it comes after another
+// (only the pair's first block can, so no two parts share a place).
 struct Parts {
   int first, last;
 };
@@ -149,5 +148,12 @@ LF_DEVICE Parts parts_of(int begin, int tiles, int share) {
   return {begin / share, (begin + tiles - 1) / share};
 }
 LF_DEVICE int part_slot(int block, int begin, int share) { return 2 * block + (begin > block * share ? 1 : 0); }
+
+// Parts are added up in groups of kGroup neighbours, from the pair's first on,
+// then the groups. The sum of the group that starts at block `start` has a
+// place of its own among the pairs of more than one group: of those, at most
+// one first group and one later group start in a window of kGroup blocks.
+constexpr int kGroup = 32;
+LF_DEVICE int group_slot(int start, int first) { return 2 * (start / kGroup) + (start == first ? 1 : 0); }
 
 }  // namespace attn

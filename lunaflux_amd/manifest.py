@@ -72,9 +72,8 @@ FAMILIES = (
     (11, "lf_fp8_w8a8_gated_mlp_"),
     (23, "lf_attn_qk_norm_rope_"),
     (24, "lf_attn_decode_"),
-    (25, "lf_attn_join_"),
-    (26, "lf_low_rank_shrink_"),
-    (27, "lf_low_rank_expand_"),
+    (25, "lf_low_rank_shrink_"),
+    (26, "lf_low_rank_expand_"),
 )
 
 

@@ -114,15 +114,15 @@ def test_geometry_and_workspace():
     for head_dim in (64, 128, 256):
         for cache in ("bf16", "e4m3"):
             d = make(head_dim=head_dim, cache=cache)
-            names = [attention.launch_geometry(e, d)[1] for e in (_abi.ATTN_QK_NORM_ROPE, _abi.ATTN_DECODE, _abi.ATTN_JOIN)]
-            assert names == [f"lf_attn_qk_norm_rope_{cache}", f"lf_attn_decode_d{head_dim}_{cache}", f"lf_attn_join_d{head_dim}"]
+            names = [attention.launch_geometry(e, d)[1] for e in (_abi.ATTN_QK_NORM_ROPE, _abi.ATTN_DECODE)]
+            assert names == [f"lf_attn_qk_norm_rope_{cache}", f"lf_attn_decode_d{head_dim}_{cache}"]
             for name in names:
                 assert name.encode() + b"\0" in _abi.code_object_bytes()
     # the largest head tile and prefix fit the launch's LDS limit
     d = make(query_heads=64, head_dim=256, max_sequences=2048)
     dims, _ = attention.launch_geometry(_abi.ATTN_DECODE, d)
     assert dims.shared_memory_bytes <= 98304
-    assert attention.workspace_bytes(_abi.ATTN_DECODE, d) == attention.workspace_bytes(_abi.ATTN_JOIN, d) > 0
+    assert attention.workspace_bytes(_abi.ATTN_DECODE, d) > 0
     with pytest.raises(DeviceError):
         attention.launch_geometry(9, d)
     with pytest.raises(DeviceError):
@@ -213,15 +213,29 @@ def test_binding_refusals():
                     (3, region(q - 2)), (4, region(cache - 1)), (5, region(cache - 1)), (5, region(cache, 4))]:
         with pytest.raises(DeviceError):
             bind(rt, layer, step, *ok[:at], bad, *ok[at + 1:])
+    one = FakeAllocation(2 * qkv)
+    whole = KernelArgument.device_region(one, 0, qkv, 16)
+    for at, bad in [(3, KernelArgument.device_region(one, qkv - 16, q, 16)), (4, KernelArgument.device_region(one, 256, cache, 16)),
+                    (3, KernelArgument.device_region(one, 0, q, 16))]:
+        args = [whole, *ok[1:]]
+        args[at] = bad
+        with pytest.raises(DeviceError):  # overlap
+            bind(rt, layer, step, *args)
+    with pytest.raises(DeviceError):
+        bind(rt, layer, step, *ok[:4], ok[4], ok[4])
     rt2, plain, step2 = bound()
     with pytest.raises(DeviceError):      # norm weights for a layer without a norm
         bind(rt2, plain, step2, *ok)
     decode = attention.bind_paged_decode
     ok = [region(q), region(q), region(cache), region(cache)]
-    assert [s.name for s in decode(rt, layer, step, *ok).steps] == ["lf_attn_decode_d128_bf16", "lf_attn_join_d128"]
+    assert [s.name for s in decode(rt, layer, step, *ok).steps] == ["lf_attn_decode_d128_bf16"]
     for at, bad in [(0, region(q - 2)), (1, region(q - 2)), (2, region(cache - 1)), (3, region(cache, 2))]:
         with pytest.raises(DeviceError):
             decode(rt, layer, step, *ok[:at], bad, *ok[at + 1:])
+    for at in (0, 2, 3):                  # out is one of the others
+        with pytest.raises(DeviceError):
+            decode(rt, layer, step, *(ok[1] if i == at else r for i, r in enumerate(ok)))
+    decode(rt, layer, step, *ok[:3], ok[2])   # keys that are their own values are only read
     other = attention.PagedStep(rt, attention.attention_layer(rt, **{**FIELDS, "max_sequences": 5}))
     with pytest.raises(DeviceError):      # a step of another descriptor
         decode(rt, layer, other, *ok)

@@ -60,28 +60,34 @@ static void hostile() {
   // regions of exactly the descriptor's sizes; .at() faults outside them
   auto counts = garbage(5), row_offsets = garbage(d.max_sequences + 1), lengths = garbage(d.max_sequences);
   auto page_offsets = garbage(d.max_sequences + 1), table = garbage(d.table_entries);
-  const Decoded dec = decoded_of(d, counts.data());
+  const Decoded dec = decoded_of(d, counts[0], counts[1], counts[2]);
   CHECK(dec.s0 >= 0 && dec.n >= 0 && dec.s0 + dec.n <= d.max_sequences);
   for (int s = 0; s < d.max_sequences; ++s) {
     bool bad = false;
-    const Pages p = pages_of(d, page_offsets.data(), s, bad);
+    const Pages p = pages_of(d, page_offsets[s], page_offsets[s + 1], bad);
     CHECK(p.first >= 0 && p.count >= 0 && p.first + p.count <= d.table_entries);
-    const Span span = span_of(d, lengths.data(), page_offsets.data(), s, bad);
+    const Span span = span_of(d, lengths[s], p, bad);
     CHECK(span.len >= 0 && span.len <= int64_t(p.count) * d.page_size && span.lo >= 0 && span.lo <= span.len);
     CHECK(span.tiles >= 1);
     const int shift = __builtin_ctz(d.page_size), first = span.lo >> shift, end = (span.len + d.page_size - 1) >> shift;
     CHECK(end <= p.count);
-    for (int t = 0; t < span.tiles; ++t) {
-      for (int j = (span.first_tile + t) * kTileKeys; j < (span.first_tile + t + 1) * kTileKeys; ++j) {
-        const int e = j >> shift;
-        if (e >= first && e < end) CHECK(p.first + e >= 0 && p.first + e < d.table_entries);
-        const int page = page_of(d, table.data() + p.first, first, end, shift, j, bad);
-        CHECK(page >= -1 && page < d.pages);
-        // the kernel reads page 0 where there is none
-        for (int h = 0; h < d.kv_heads; ++h) {
-          const uint64_t at = cache_byte<true>(d, page < 0 ? 0 : page, h, j & (d.page_size - 1));
-          CHECK(at + d.head_dim <= static_cast<uint64_t>(elements(d)));
-          CHECK(cache_byte<false>(d, page < 0 ? 0 : page, h, j & (d.page_size - 1)) == 2 * at);
+    if (span.len > 0) CHECK(end > first);
+    for (int t = 0; t < span.tiles && span.len > 0; ++t) {
+      const int base = (span.first_tile + t) * kTileKeys;
+      CHECK(base < span.len);
+      for (int j = base; j < base + kTileKeys; j += 8) {
+        const int e = entry_of(first, end, shift, j);
+        CHECK(e >= first && e < end && p.first + e < d.table_entries);
+        for (int i = j; i < j + 8; ++i) {
+          if (i >= span.lo && i < span.len) CHECK(e == i >> shift);   // keys that count are in their page
+          // pages outside the cache are read as page 0
+          for (int page = 0; page < d.pages; page += d.pages > 1 ? d.pages - 1 : 1) {
+            for (int h = 0; h < d.kv_heads; ++h) {
+              const uint64_t at = cache_byte<true>(d, page, h, i & (d.page_size - 1));
+              CHECK(at + d.head_dim <= static_cast<uint64_t>(elements(d)));
+              CHECK(cache_byte<false>(d, page, h, i & (d.page_size - 1)) == 2 * at);
+            }
+          }
         }
       }
     }
@@ -92,7 +98,7 @@ static void hostile() {
   }
 }
 
-static void cut(int blocks) {
+static void cut(int workers) {  // ranges
   Desc d = desc();
   const int n = pick(0, d.max_sequences), head_tiles = head_tiles_of(d);
   std::vector<int> prefix(n + 1, 0), tiles(n);
@@ -100,10 +106,11 @@ static void cut(int blocks) {
     tiles[i] = pick(0, 4) ? pick(1, 5) : pick(1, 400);
     prefix[i + 1] = prefix[i] + tiles[i];
   }
-  const int items = prefix[n] * head_tiles, share = share_of(items, blocks);
+  const int items = prefix[n] * head_tiles, share = share_of(items, n * head_tiles, workers);
+  CHECK(share > 0 && int64_t(share) * workers >= items);
   std::vector<int> seen(items, 0);
-  std::set<int> left, read;
-  for (int b = 0; b < blocks; ++b) {
+  std::set<int> left, read, sums;
+  for (int b = 0; b < workers; ++b) {
     const int begin = b * share, end = begin + share < items ? begin + share : items;
     for (int u = begin; u < end;) {
       const int i = sequence_at(prefix.data(), n, head_tiles, u);
@@ -114,7 +121,7 @@ static void cut(int blocks) {
       for (int t = t0; t < t1; ++t) seen[prefix[i] * head_tiles + ht * tiles[i] + t]++;
       if (t0 != 0 || t1 != tiles[i]) {
         const int slot = part_slot(b, u - t0, share);
-        CHECK(slot >= 0 && slot < 2 * blocks && left.insert(slot).second);
+        CHECK(slot >= 0 && slot < 2 * workers && left.insert(slot).second);
       }
       u += t1 - t0;
     }
@@ -125,7 +132,17 @@ static void cut(int blocks) {
       const int begin = prefix[i] * head_tiles + ht * tiles[i];
       const Parts parts = parts_of(begin, tiles[i], share);
       if (parts.first == parts.last) continue;
-      for (int b = parts.first; b <= parts.last; ++b) CHECK(read.insert(part_slot(b, begin, share)).second);
+      for (int b = parts.first; b <= parts.last; ++b) {
+        CHECK(read.insert(part_slot(b, begin, share)).second);
+        if (b > parts.first) CHECK(part_slot(b, begin, share) == 2 * b);   // the kernel steps from part to part
+      }
+      if (parts.last - parts.first < kGroup) continue;
+      for (int start = parts.first; start <= parts.last; start += kGroup) {
+        const int place = group_slot(start, parts.first);
+        CHECK(place >= 0 && place <= 2 * workers / kGroup + 1 && sums.insert(place).second);
+        if (start > parts.first)
+          CHECK(place == group_slot(parts.first, parts.first) - 1 + 2 * ((start - parts.first) / kGroup));
+      }
     }
   }
   CHECK(left == read);
@@ -133,8 +150,8 @@ static void cut(int blocks) {
 
 int main() {
   for (int i = 0; i < 300; ++i) hostile();
-  const int blocks[] = {1, 2, 7, 256, 1024};
-  for (int i = 0; i < 400; ++i) cut(blocks[i % 5]);
+  const int workers[] = {1, 2, 7, 256, 1024, 2048};
+  for (int i = 0; i < 600; ++i) cut(workers[i % 6]);
   std::printf("ok\n");
 }
 """
