@@ -627,9 +627,11 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
  * out = y + scaling[a] (x A[a]^T) B[a]^T for each row, a = ids[row] its
  * request's adapter: what a low-rank adapter adds to the output y of a shared
  * projection of x. One launch pair serves the rows of many adapters.
- *  lf_low_rank_shrink_r{16,64} (counts, ids, desc, x, a, ws)
- *  lf_low_rank_expand_r{16,64} (counts, ids, desc, scaling, b, y, out, ws)
- *                              after the shrink, on its workspace
+ *  lf_low_rank_r16        (counts, ids, desc, scaling, x, a, b, y, out, ws)
+ *                         profiles of up to 512 rows, one launch
+ *  lf_low_rank_shrink_r64 (counts, ids, desc, x, a, ws), then
+ *  lf_low_rank_expand_r64 (counts, ids, desc, scaling, b, y, out, ws)
+ *                         larger ones
  * (_r16, _r64: rows of a block's tile.) ids int32 [max_tokens], -1 (any
  * negative value): the row has no adapter and is copied. x bf16 [M, hidden];
  * y, out bf16 [M, columns], the same region or disjoint ones. The columns are
@@ -639,10 +641,13 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
  * scaling fp32 [adapters]. x A^T is summed in fp32 and enters the second
  * product as two bf16 terms (16 bits of it); the sum with y is rounded once.
  * A row's values depend on its own adapter only, whatever the others hold.
- * An id past the adapters leaves the row without one and sets the int32 error
- * word at the start of ws (until the caller clears it). Sums over hidden are
- * taken in slices whose number follows from the descriptor, in their order.
+ * An id past the adapters leaves the row without one and sets the int32 word at
+ * LF_FP8_LOW_RANK_BAD_ID_OFFSET of ws (until the caller clears it). The one
+ * launch holds counted waits: the error word at the start of ws as for the _AQ
+ * entries (LF_FP8_AQ_ERROR_OFFSET). Sums over hidden are taken in slices whose
+ * number follows from the descriptor, in their order.
  */
+#define LF_FP8_LOW_RANK_BAD_ID_OFFSET 64
 #define LF_FP8_LOW_RANK_MAGIC 0x4B4E524Cu /* bytes "LRNK" */
 #define LF_FP8_LOW_RANK_SLICES 4
 
@@ -654,19 +659,27 @@ typedef struct lf_fp8_low_rank_desc {
   int32_t slices;     /* 1 .. 4 */
   int32_t columns;    /* the sum of the slices' widths */
   int32_t max_tokens;
-  int32_t splits;     /* slices of hidden, written by lunaflux_fp8_low_rank_descriptor */
+  int32_t splits;     /* written by lunaflux_fp8_low_rank_descriptor: slices of hidden */
   int32_t ends[LF_FP8_LOW_RANK_SLICES]; /* column behind each slice */
-  int32_t reserved[4];
+  int32_t slots;         /* blocks that share a tile's adapters, written as splits */
+  int32_t column_blocks; /* blocks a tile's columns are cut into, written as splits */
+  int32_t reserved[2];
 } lf_fp8_low_rank_desc;
 
-enum lf_fp8_low_rank_entry { LF_FP8_LOW_RANK_SHRINK = 1, LF_FP8_LOW_RANK_EXPAND = 2 };
+enum lf_fp8_low_rank_entry {
+  LF_FP8_LOW_RANK_ONE_LAUNCH = 1,
+  LF_FP8_LOW_RANK_SHRINK = 2,
+  LF_FP8_LOW_RANK_EXPAND = 3
+};
 
 /* widths: `slices` output widths, multiples of 64. */
 int32_t lunaflux_fp8_low_rank_descriptor(int32_t adapters, int32_t rank, int64_t hidden, const int64_t *widths,
                                          int32_t slices, int32_t max_tokens, lf_fp8_low_rank_desc *out);
-/* Workspace of both launches: its error word zeroed once when allocated;
- * launches sharing one must not overlap. -1 if invalid. */
+/* Workspace of the operation, zero-filled once when allocated (its counters
+ * return to zero at the end of every launch); launches sharing one must not
+ * overlap. -1 if invalid. */
 int64_t lunaflux_fp8_low_rank_workspace_bytes(const lf_fp8_low_rank_desc *desc);
+/* LF_UNSUPPORTED for an entry that the profile does not launch. */
 int32_t lunaflux_fp8_low_rank_launch_geometry(int32_t entry, const lf_fp8_low_rank_desc *desc, int32_t dims[7],
                                               char symbol[LF_FP8_SYMBOL_BYTES]);
 

@@ -29,7 +29,7 @@ class LowRankDescriptor(ctypes.Structure):
     _fields_ = [("magic", ctypes.c_uint32), ("adapters", ctypes.c_int32), ("rank", ctypes.c_int32),
                 ("hidden", ctypes.c_int32), ("slices", ctypes.c_int32), ("columns", ctypes.c_int32),
                 ("max_tokens", ctypes.c_int32), ("splits", ctypes.c_int32), ("ends", ctypes.c_int32 * 4),
-                ("reserved", ctypes.c_int32 * 4)]
+                ("slots", ctypes.c_int32), ("column_blocks", ctypes.c_int32), ("reserved", ctypes.c_int32 * 2)]
 
 
 def _check(operation, status):
@@ -61,10 +61,13 @@ def workspace_bytes(desc: LowRankDescriptor) -> int:
 
 
 def launch_geometry(entry: int, desc: LowRankDescriptor):
+    """(dims, symbol), or None for an entry that the profile does not launch."""
     dims = (ctypes.c_int32 * 7)()
     symbol = ctypes.create_string_buffer(128)
-    _check("low_rank_launch_geometry", _abi.lib().lunaflux_fp8_low_rank_launch_geometry(
-        entry, ctypes.byref(desc), dims, symbol))
+    status = _abi.lib().lunaflux_fp8_low_rank_launch_geometry(entry, ctypes.byref(desc), dims, symbol)
+    if status == _abi.LF_UNSUPPORTED:
+        return None
+    _check("low_rank_launch_geometry", status)
     return (KernelLaunchDimensions.new(tuple(dims[0:3]), tuple(dims[3:6]), dims[6]),
             symbol.value.decode("ascii"))
 
@@ -107,12 +110,15 @@ class LowRankAdapters:
 
 @dataclass
 class BoundLowRank(BoundOperation):
-    """check(): DeviceError(INVALID_ARGUMENT) if a launch met an adapter id past
-    the adapters (its row was left without one); the error word is cleared."""
+    """check() also raises DeviceError(INVALID_ARGUMENT) if a launch met an
+    adapter id past the adapters (its row was left without one); the word is
+    cleared."""
 
     def check(self):
-        if self.workspace.read(np.int32, (1,))[0] != 0:
-            self.workspace.copy_from_host(np.zeros(1, np.int32))
+        super().check()
+        at = _abi.LF_FP8_LOW_RANK_BAD_ID_OFFSET
+        if self.workspace.read(np.int32, (1,), at)[0] != 0:
+            self.workspace.copy_from_host(np.zeros(1, np.int32), offset=at)
             raise DeviceError("a row names an adapter that does not exist", _abi.LF_INVALID_ARGUMENT)
 
 
@@ -139,18 +145,23 @@ def bind_low_rank(rt: ProjectionRuntime, counts: Allocation, ids: KernelArgument
     if (_overlap(out, y, columns) and out.offset != y.offset) or \
             _overlap(out, x, max(columns, 2 * max_tokens * desc.hidden)):
         raise _invalid("out overlaps y or x")
-    ws = rt.context.allocate(workspace_bytes(desc))
-    ws.copy_from_host(np.zeros(64, np.int32))
+    nbytes = workspace_bytes(desc)
+    ws = rt.context.allocate(nbytes)
+    ws.copy_from_host(np.zeros(nbytes, np.uint8))
     desc_alloc = rt.context.upload(np.frombuffer(bytes(desc), np.uint8).copy())
     c, dr, wsr = _region(counts, COUNTS_BYTES, alignment=4), _region(desc_alloc, alignment=4), _region(ws, alignment=256)
+    a, b, scaling = adapters.a, adapters.b, adapters.scaling
 
     def step(entry, args):
-        dims, symbol = launch_geometry(entry, desc)
-        return LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)
+        geometry = launch_geometry(entry, desc)
+        return None if geometry is None else LaunchStep(rt.function(geometry[1]), geometry[0], KernelArguments(args),
+                                                        geometry[1])
 
-    return BoundLowRank([step(_abi.LOW_RANK_SHRINK, [c, ids, dr, x, adapters.a, wsr]),
-                         step(_abi.LOW_RANK_EXPAND, [c, ids, dr, adapters.scaling, adapters.b, y, out, wsr])],
-                        workspace=ws, keep=[adapters])
+    steps = [step(_abi.LOW_RANK_ONE_LAUNCH, [c, ids, dr, scaling, x, a, b, y, out, wsr]),
+             step(_abi.LOW_RANK_SHRINK, [c, ids, dr, x, a, wsr]),
+             step(_abi.LOW_RANK_EXPAND, [c, ids, dr, scaling, b, y, out, wsr])]
+    return BoundLowRank([s for s in steps if s is not None], workspace=ws, keep=[adapters],
+                        error_offset=_abi.LF_FP8_AQ_ERROR_OFFSET)
 
 
 def low_rank(rt: ProjectionRuntime, x: np.ndarray, y: np.ndarray, ids, adapters: LowRankAdapters,

@@ -74,6 +74,7 @@ FAMILIES = (
     (24, "lf_attn_decode_"),
     (25, "lf_low_rank_shrink_"),
     (26, "lf_low_rank_expand_"),
+    (27, "lf_low_rank_r16"),
 )
 
 

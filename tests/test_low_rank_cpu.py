@@ -13,12 +13,15 @@ def test_descriptor_and_geometry():
     d = low_rank.low_rank_descriptor(16, 16, 4096, [4096, 1024, 1024], 64)
     assert ctypes.sizeof(d) == 64 and bytes(d)[:4] == b"LRNK"
     assert list(d.ends) == [4096, 5120, 6144, 0] and d.columns == 6144 and d.slices == 3 and d.splits >= 1
-    names = [low_rank.launch_geometry(e, d)[1] for e in (_abi.LOW_RANK_SHRINK, _abi.LOW_RANK_EXPAND)]
-    assert names == ["lf_low_rank_shrink_r16", "lf_low_rank_expand_r16"]
+    entries = (_abi.LOW_RANK_ONE_LAUNCH, _abi.LOW_RANK_SHRINK, _abi.LOW_RANK_EXPAND)
+    geometry = [low_rank.launch_geometry(e, d) for e in entries]
+    assert geometry[0][1] == "lf_low_rank_r16" and geometry[1:] == [None, None]
+    # every tile and slot: the blocks of x A^T, then those of the columns
+    assert geometry[0][0].grid == (4 * 16 * (d.splits + 12), 1, 1) and d.slots == 16 and d.column_blocks == 12
     d = low_rank.low_rank_descriptor(4, 128, 512, [512], 4096)
-    names += [low_rank.launch_geometry(e, d)[1] for e in (_abi.LOW_RANK_SHRINK, _abi.LOW_RANK_EXPAND)]
-    assert names[2:] == ["lf_low_rank_shrink_r64", "lf_low_rank_expand_r64"]
-    for name in names:
+    geometry = [low_rank.launch_geometry(e, d) for e in entries]
+    assert geometry[0] is None and [g[1] for g in geometry[1:]] == ["lf_low_rank_shrink_r64", "lf_low_rank_expand_r64"]
+    for name in ("lf_low_rank_r16", "lf_low_rank_shrink_r64", "lf_low_rank_expand_r64"):
         assert name.encode() + b"\0" in _abi.code_object_bytes()
     assert low_rank.workspace_bytes(d) >= 256 + 4096 * 128 * 4
     for bad in (low_rank.LowRankDescriptor(),):
@@ -27,7 +30,7 @@ def test_descriptor_and_geometry():
         with pytest.raises(DeviceError):
             low_rank.launch_geometry(_abi.LOW_RANK_SHRINK, bad)
     with pytest.raises(DeviceError):
-        low_rank.launch_geometry(3, d)
+        low_rank.launch_geometry(4, d)
 
 
 @pytest.mark.parametrize("args", [
@@ -67,7 +70,7 @@ def test_binding_refusals():
     ad, counts = adapters(rt), FakeAllocation(20)
     x, y = region(2 * 8 * 256), region(2 * 8 * 192)
     bind = lambda ids=region(32, 4), x=x, y=y, out=y, m=8: low_rank.bind_low_rank(rt, counts, ids, x, ad, y, out, m)  # noqa: E731
-    assert [s.name for s in bind().steps] == ["lf_low_rank_shrink_r16", "lf_low_rank_expand_r16"]
+    assert [s.name for s in bind().steps] == ["lf_low_rank_r16"]
     wide = FakeAllocation(4 * 8 * 192)
     part = lambda offset: wide_region(wide, offset)  # noqa: E731
     bind(y=part(0), out=part(2 * 8 * 192))
