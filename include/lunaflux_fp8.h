@@ -626,28 +626,26 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
 /*
  * out = y + scaling[a] (x A[a]^T) B[a]^T for each row, a = ids[row] its
  * request's adapter: what a low-rank adapter adds to the output y of a shared
- * projection of x. One launch pair serves the rows of many adapters.
- *  lf_low_rank_r16        (counts, ids, desc, scaling, x, a, b, y, out, ws)
- *                         profiles of up to 512 rows, one launch
- *  lf_low_rank_shrink_r64 (counts, ids, desc, x, a, ws), then
- *  lf_low_rank_expand_r64 (counts, ids, desc, scaling, b, y, out, ws)
- *                         larger ones
- * (_r16, _r64: rows of a block's tile.) ids int32 [max_tokens], -1 (any
- * negative value): the row has no adapter and is copied. x bf16 [M, hidden];
- * y, out bf16 [M, columns], the same region or disjoint ones. The columns are
- * those of up to four projections side by side (Q|K|V), each a slice with an A
- * and B of its own: A bf16 [adapters, slices * rank, hidden], B bf16 [adapters,
- * columns, rank]; an adapter of a lower rank, or without a slice, holds zeros.
+ * projection of x, for the rows of many adapters at once.
+ *  lf_low_rank_n{1,2,4}       (counts, ids, desc, scaling, x, a, b, y, out, ws)
+ *                             one launch: few rows, and an A of few bytes
+ *  lf_low_rank_shrink_64x{32,64} (counts, ids, desc, x, a, ws), then
+ *  lf_low_rank_expand_{16x32,16x64,64x32,64x64,64x128}
+ *                             (counts, ids, desc, scaling, b, y, out, ws)
+ *                             otherwise
+ * (the descriptor says which). ids int32 [max_tokens], -1 (any negative value):
+ * the row has no adapter and is copied. x bf16 [M, hidden]; y, out bf16
+ * [M, columns], the same region or disjoint ones. The columns are those of up to
+ * four projections side by side (Q|K|V), each a slice with an A and B of its own:
+ * A bf16 [adapters, slices * rank, hidden], B bf16 [adapters, columns, rank]; an
+ * adapter of a lower rank, or without a slice, holds zeros.
  * scaling fp32 [adapters]. x A^T is summed in fp32 and enters the second
  * product as two bf16 terms (16 bits of it); the sum with y is rounded once.
  * A row's values depend on its own adapter only, whatever the others hold.
- * An id past the adapters leaves the row without one and sets the int32 word at
- * LF_FP8_LOW_RANK_BAD_ID_OFFSET of ws (until the caller clears it). The one
- * launch holds counted waits: the error word at the start of ws as for the _AQ
- * entries (LF_FP8_AQ_ERROR_OFFSET). Sums over hidden are taken in slices whose
- * number follows from the descriptor, in their order.
+ * An id past the adapters leaves the row without one and sets the int32 error
+ * word at the start of ws (until the caller clears it). Sums over hidden are
+ * taken in slices whose number follows from the descriptor, in their order.
  */
-#define LF_FP8_LOW_RANK_BAD_ID_OFFSET 64
 #define LF_FP8_LOW_RANK_MAGIC 0x4B4E524Cu /* bytes "LRNK" */
 #define LF_FP8_LOW_RANK_SLICES 4
 
@@ -661,9 +659,10 @@ typedef struct lf_fp8_low_rank_desc {
   int32_t max_tokens;
   int32_t splits;     /* written by lunaflux_fp8_low_rank_descriptor: slices of hidden */
   int32_t ends[LF_FP8_LOW_RANK_SLICES]; /* column behind each slice */
-  int32_t slots;         /* blocks that share a tile's adapters, written as splits */
+  int32_t slots;      /* blocks that share a tile's adapters, written as splits */
+  int32_t one_launch; /* 1 or 0, written as splits */
   int32_t column_blocks; /* blocks a tile's columns are cut into, written as splits */
-  int32_t reserved[2];
+  int32_t reserved;
 } lf_fp8_low_rank_desc;
 
 enum lf_fp8_low_rank_entry {
@@ -675,9 +674,8 @@ enum lf_fp8_low_rank_entry {
 /* widths: `slices` output widths, multiples of 64. */
 int32_t lunaflux_fp8_low_rank_descriptor(int32_t adapters, int32_t rank, int64_t hidden, const int64_t *widths,
                                          int32_t slices, int32_t max_tokens, lf_fp8_low_rank_desc *out);
-/* Workspace of the operation, zero-filled once when allocated (its counters
- * return to zero at the end of every launch); launches sharing one must not
- * overlap. -1 if invalid. */
+/* Workspace of the operation, its first 256 bytes zero-filled when allocated;
+ * launches sharing one must not overlap. -1 if invalid. */
 int64_t lunaflux_fp8_low_rank_workspace_bytes(const lf_fp8_low_rank_desc *desc);
 /* LF_UNSUPPORTED for an entry that the profile does not launch. */
 int32_t lunaflux_fp8_low_rank_launch_geometry(int32_t entry, const lf_fp8_low_rank_desc *desc, int32_t dims[7],

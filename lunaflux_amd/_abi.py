@@ -157,7 +157,6 @@ LF_FP8_PAIR_HALF, LF_FP8_PAIR_NEIGHBOUR = 0, 1
 LF_FP8_ATTN_MAX_SEQUENCES = 2048
 ATTN_QK_NORM_ROPE, ATTN_DECODE = 1, 2
 LOW_RANK_ONE_LAUNCH, LOW_RANK_SHRINK, LOW_RANK_EXPAND = 1, 2, 3
-LF_FP8_LOW_RANK_BAD_ID_OFFSET = 64
 
 
 class NativeLibraryMissing(RuntimeError):

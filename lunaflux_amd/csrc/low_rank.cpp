@@ -13,39 +13,58 @@ namespace {
 
 constexpr int64_t kMaxWidth = int64_t(1) << 20;
 // kernels/low_rank.hip
-constexpr int64_t kChunk = 64;         // columns of x A^T per block
-constexpr int64_t kColumnBlock = 512;  // output columns per block
-constexpr int64_t kHeaderBytes = 256, kCounterBytes = 256;
+constexpr int64_t kOneColumns = 1024;           // output columns of a one-launch block
+constexpr int64_t kExpandColumns = 512;         // and of an expand block
+constexpr int64_t kHeaderBytes = 256;
 
-// Rows of a block's tile: batches of few rows hold many adapters, so a tile is
-// one 16-row product and its adapters go to blocks of their own; long runs of
-// one adapter share its weights over 64 rows.
-int64_t tile_rows(const lf_fp8_low_rank_desc *d) { return d->max_tokens <= 512 ? 16 : 64; }
+int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+int64_t cut(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
-int64_t tiles(const lf_fp8_low_rank_desc *d) {
-  const int64_t rows = tile_rows(d);
-  return (d->max_tokens + rows - 1) / rows;
+// The one launch reads a slice's A once per 1024 columns, so A has to be small
+// enough to come from L2 quickly, and gives each adapter of 16 rows a block. Against
+// two launches (columns 4096 + 2 x 1024, an adapter per row or so): 61 rows of rank
+// 16 of 4096 13 us and 25, of rank 64 33 and 35, of rank 128 53 and 45; 128 rows 19
+// and 31, 50 and 47, 84 and 64; 256 rows 31 and 39, 83 and 83, 139 and 88.
+int32_t one_launch_of(const lf_fp8_low_rank_desc *d) {
+  return d->max_tokens <= 128 && int64_t(d->rank) * d->hidden <= 262144 ? 1 : 0;
 }
 
-int64_t chunks(const lf_fp8_low_rank_desc *d) { return (int64_t(d->slices) * d->rank + kChunk - 1) / kChunk; }
-
-// Blocks per tile, each taking every slots-th adapter of the tile's rows.
-int32_t slots_of(const lf_fp8_low_rank_desc *d) {
-  return std::min<int32_t>(d->adapters, d->max_tokens <= 128 ? 16 : d->max_tokens <= 512 ? 4 : 2);
+// A shrink block's rows and columns of x A^T; with 32 columns where there are no
+// more, it does not load A's rows twice (509 rows, rank 32: 18.3 us, with 64 19.5).
+constexpr int64_t kTileRows = 64;
+int64_t chunk_of(const lf_fp8_low_rank_desc *d) { return int64_t(d->slices) * d->rank <= 32 ? 32 : 64; }
+int64_t shrink_blocks(const lf_fp8_low_rank_desc *d) {
+  return cut(d->max_tokens, kTileRows) * cut(int64_t(d->slices) * d->rank, chunk_of(d));
 }
 
-// Slices of hidden: two or more steps of 64 for each of a block's four waves,
-// and no more blocks than the chip holds at once.
+// Slices of hidden: two or more steps of 64 for each of a block's eight waves, and
+// no more blocks than the chip has compute units.
 int32_t splits_of(const lf_fp8_low_rank_desc *d) {
-  const int64_t blocks = tiles(d) * chunks(d);
-  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, d->hidden / 512));
-  return static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(most, 768 / std::min<int64_t>(blocks, 768))));
+  if (one_launch_of(d)) return 1;
+  return static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({16, d->hidden / 1024, 256 / shrink_blocks(d)})));
+}
+
+// Blocks that share a tile's adapters. In the two launches most tiles of long
+// prompts have one, so that the other blocks are idle, but a tile of two must not
+// take twice as long: 4093 rows of 8 adapters 84 us with one slot, 69 with two, 66
+// with four.
+int32_t slots_of(const lf_fp8_low_rank_desc *d) {
+  const int64_t most = one_launch_of(d) ? 16 : std::max<int64_t>(2, std::min<int64_t>(8, 768 / shrink_blocks(d)));
+  return static_cast<int32_t>(std::min<int64_t>(d->adapters, most));
+}
+
+// Rows of an expand block: 16, so that few rows still fill the chip, while that
+// reads B from L2 rarely enough. Both launches with 16 and with 64: 200 rows of rank
+// 16 15 us and 18, of rank 64 18 and 21; 509 rows 19 and 20, 29 and 23; 1600 rows 35
+// and 23, 68 and 38.
+int64_t expand_rows(const lf_fp8_low_rank_desc *d) {
+  return d->max_tokens <= 512 && d->rank <= 64 && int64_t(d->max_tokens) * d->rank <= 16384 ? 16 : 64;
 }
 
 int32_t column_blocks_of(const lf_fp8_low_rank_desc *d) {
   int64_t blocks = 0, begin = 0;
   for (int32_t i = 0; i < d->slices; ++i) {
-    blocks += (d->ends[i] - begin + kColumnBlock - 1) / kColumnBlock;
+    blocks += cut(d->ends[i] - begin, one_launch_of(d) ? kOneColumns : kExpandColumns);
     begin = d->ends[i];
   }
   return static_cast<int32_t>(blocks);
@@ -68,7 +87,7 @@ bool fields_ok(const lf_fp8_low_rank_desc *d) {
 
 bool desc_ok(const lf_fp8_low_rank_desc *d) {
   return d != nullptr && d->magic == LF_FP8_LOW_RANK_MAGIC && fields_ok(d) && d->splits == splits_of(d) &&
-         d->slots == slots_of(d) && d->column_blocks == column_blocks_of(d);
+         d->slots == slots_of(d) && d->one_launch == one_launch_of(d) && d->column_blocks == column_blocks_of(d);
 }
 
 }  // namespace
@@ -99,6 +118,7 @@ int32_t lunaflux_fp8_low_rank_descriptor(int32_t adapters, int32_t rank, int64_t
   if (!fields_ok(&d)) return LF_INVALID_ARGUMENT;
   d.splits = splits_of(&d);
   d.slots = slots_of(&d);
+  d.one_launch = one_launch_of(&d);
   d.column_blocks = column_blocks_of(&d);
   *out = d;
   return LF_OK;
@@ -106,34 +126,37 @@ int32_t lunaflux_fp8_low_rank_descriptor(int32_t adapters, int32_t rank, int64_t
 
 int64_t lunaflux_fp8_low_rank_workspace_bytes(const lf_fp8_low_rank_desc *d) {
   if (!desc_ok(d)) return -1;
-  const int64_t counted = tile_rows(d) == 16 ? tiles(d) * d->slots : 0;
-  return kHeaderBytes + counted * kCounterBytes + int64_t(d->splits) * d->max_tokens * d->slices * d->rank * 4;
+  if (d->one_launch) return kHeaderBytes;
+  return kHeaderBytes + int64_t(d->splits) * d->max_tokens * d->slices * d->rank * 4;
 }
 
 int32_t lunaflux_fp8_low_rank_launch_geometry(int32_t entry, const lf_fp8_low_rank_desc *d, int32_t dims[7],
                                               char symbol[LF_FP8_SYMBOL_BYTES]) {
   if (!desc_ok(d) || dims == nullptr || symbol == nullptr) return LF_INVALID_ARGUMENT;
-  const bool one = tile_rows(d) == 16;
   if (entry < LF_FP8_LOW_RANK_ONE_LAUNCH || entry > LF_FP8_LOW_RANK_EXPAND) return LF_INVALID_ARGUMENT;
-  if (one != (entry == LF_FP8_LOW_RANK_ONE_LAUNCH)) return LF_UNSUPPORTED;
-  const int64_t pairs = tiles(d) * d->slots;
-  int64_t gx = pairs, gy = 1, gz = 1;
-  const char *name = "lf_low_rank_r16";
-  if (one) {
-    gx = pairs * (chunks(d) * d->splits + d->column_blocks);
-  } else if (entry == LF_FP8_LOW_RANK_SHRINK) {
-    name = "lf_low_rank_shrink_r64";
-    gy = chunks(d);
-    gz = d->splits;
-  } else {
-    name = "lf_low_rank_expand_r64";
+  if ((d->one_launch != 0) != (entry == LF_FP8_LOW_RANK_ONE_LAUNCH)) return LF_UNSUPPORTED;
+  int64_t gx = 0, gy = 1, threads = 256;
+  if (entry == LF_FP8_LOW_RANK_ONE_LAUNCH) {
+    std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_low_rank_n%d", d->rank == 16 ? 1 : d->rank == 32 ? 2 : 4);
+    gx = cut(d->max_tokens, 16) * d->slots;
+    threads = 512;
     gy = d->column_blocks;
+  } else if (entry == LF_FP8_LOW_RANK_SHRINK) {
+    std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_low_rank_shrink_%dx%d", static_cast<int>(kTileRows),
+                  static_cast<int>(chunk_of(d)));
+    threads = 512;
+    gx = align_up(shrink_blocks(d) * d->splits, 8);  // XCDs have neighbouring blocks each
+  } else {
+    std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_low_rank_expand_%dx%d", static_cast<int>(expand_rows(d)),
+                  d->rank <= 32 ? 32 : d->rank <= 64 ? 64 : 128);
+    gx = align_up(cut(d->max_tokens, expand_rows(d)) * d->column_blocks, 8);
   }
-  std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "%s", name);
+  if (!d->one_launch) gy = d->slots;
+  if (gx > INT32_MAX) return LF_UNSUPPORTED;
   dims[0] = static_cast<int32_t>(gx);
   dims[1] = static_cast<int32_t>(gy);
-  dims[2] = static_cast<int32_t>(gz);
-  dims[3] = 256;
+  dims[2] = 1;
+  dims[3] = static_cast<int32_t>(threads);
   dims[4] = dims[5] = 1;
   dims[6] = 0;
   return LF_OK;

@@ -29,7 +29,8 @@ class LowRankDescriptor(ctypes.Structure):
     _fields_ = [("magic", ctypes.c_uint32), ("adapters", ctypes.c_int32), ("rank", ctypes.c_int32),
                 ("hidden", ctypes.c_int32), ("slices", ctypes.c_int32), ("columns", ctypes.c_int32),
                 ("max_tokens", ctypes.c_int32), ("splits", ctypes.c_int32), ("ends", ctypes.c_int32 * 4),
-                ("slots", ctypes.c_int32), ("column_blocks", ctypes.c_int32), ("reserved", ctypes.c_int32 * 2)]
+                ("slots", ctypes.c_int32), ("one_launch", ctypes.c_int32),
+                ("column_blocks", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 def _check(operation, status):
@@ -110,15 +111,12 @@ class LowRankAdapters:
 
 @dataclass
 class BoundLowRank(BoundOperation):
-    """check() also raises DeviceError(INVALID_ARGUMENT) if a launch met an
-    adapter id past the adapters (its row was left without one); the word is
-    cleared."""
+    """check(): DeviceError(INVALID_ARGUMENT) if a launch met an adapter id past
+    the adapters (its row was left without one); the error word is cleared."""
 
     def check(self):
-        super().check()
-        at = _abi.LF_FP8_LOW_RANK_BAD_ID_OFFSET
-        if self.workspace.read(np.int32, (1,), at)[0] != 0:
-            self.workspace.copy_from_host(np.zeros(1, np.int32), offset=at)
+        if self.workspace.read(np.int32, (1,))[0] != 0:
+            self.workspace.copy_from_host(np.zeros(1, np.int32))
             raise DeviceError("a row names an adapter that does not exist", _abi.LF_INVALID_ARGUMENT)
 
 
@@ -160,8 +158,7 @@ def bind_low_rank(rt: ProjectionRuntime, counts: Allocation, ids: KernelArgument
     steps = [step(_abi.LOW_RANK_ONE_LAUNCH, [c, ids, dr, scaling, x, a, b, y, out, wsr]),
              step(_abi.LOW_RANK_SHRINK, [c, ids, dr, x, a, wsr]),
              step(_abi.LOW_RANK_EXPAND, [c, ids, dr, scaling, b, y, out, wsr])]
-    return BoundLowRank([s for s in steps if s is not None], workspace=ws, keep=[adapters],
-                        error_offset=_abi.LF_FP8_AQ_ERROR_OFFSET)
+    return BoundLowRank([s for s in steps if s is not None], workspace=ws, keep=[adapters])
 
 
 def low_rank(rt: ProjectionRuntime, x: np.ndarray, y: np.ndarray, ids, adapters: LowRankAdapters,

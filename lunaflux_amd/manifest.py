@@ -72,9 +72,9 @@ FAMILIES = (
     (11, "lf_fp8_w8a8_gated_mlp_"),
     (23, "lf_attn_qk_norm_rope_"),
     (24, "lf_attn_decode_"),
-    (25, "lf_low_rank_shrink_"),
+    (25, "lf_low_rank_shrink"),
     (26, "lf_low_rank_expand_"),
-    (27, "lf_low_rank_r16"),
+    (27, "lf_low_rank_n"),
 )
 
 

@@ -15,14 +15,26 @@ def test_descriptor_and_geometry():
     assert list(d.ends) == [4096, 5120, 6144, 0] and d.columns == 6144 and d.slices == 3 and d.splits >= 1
     entries = (_abi.LOW_RANK_ONE_LAUNCH, _abi.LOW_RANK_SHRINK, _abi.LOW_RANK_EXPAND)
     geometry = [low_rank.launch_geometry(e, d) for e in entries]
-    assert geometry[0][1] == "lf_low_rank_r16" and geometry[1:] == [None, None]
-    # every tile and slot: the blocks of x A^T, then those of the columns
-    assert geometry[0][0].grid == (4 * 16 * (d.splits + 12), 1, 1) and d.slots == 16 and d.column_blocks == 12
+    assert geometry[0][1] == "lf_low_rank_n1" and geometry[1:] == [None, None]
+    assert geometry[0][0].grid == (4 * 16, 6, 1) and d.slots == 16 and d.one_launch == 1
+    assert low_rank.workspace_bytes(d) == 256
+    for rank, hidden, rows, first, last in ((32, 4096, 128, "n2", None), (64, 2048, 128, "n4", None),
+                                            (128, 1024, 1, "n4", None), (64, 4096, 128, "n4", None), (80, 4096, 128, "shrink_64x64", "expand_64x128"),
+                                            (64, 4096, 256, "shrink_64x64", "expand_16x64"),
+                                            (16, 4096, 129, "shrink_64x32", "expand_16x32"),
+                                            (48, 14336, 1, "shrink_64x64", "expand_16x64"),
+                                            (80, 14336, 1, "shrink_64x64", "expand_64x128"),
+                                            (16, 128, 513, "shrink_64x32", "expand_64x32"),
+                                            (64, 128, 513, "shrink_64x64", "expand_64x64")):
+        d = low_rank.low_rank_descriptor(5, rank, hidden, [512, 64], rows)
+        names = [g[1][len("lf_low_rank_"):] for g in (low_rank.launch_geometry(e, d) for e in entries) if g is not None]
+        assert names == [n for n in (first, last) if n], (rank, hidden, rows)
     d = low_rank.low_rank_descriptor(4, 128, 512, [512], 4096)
     geometry = [low_rank.launch_geometry(e, d) for e in entries]
-    assert geometry[0] is None and [g[1] for g in geometry[1:]] == ["lf_low_rank_shrink_r64", "lf_low_rank_expand_r64"]
-    for name in ("lf_low_rank_r16", "lf_low_rank_shrink_r64", "lf_low_rank_expand_r64"):
-        assert name.encode() + b"\0" in _abi.code_object_bytes()
+    assert geometry[0] is None and [g[1] for g in geometry[1:]] == ["lf_low_rank_shrink_64x64", "lf_low_rank_expand_64x128"]
+    for name in ("n1", "n2", "n4", "shrink_64x32", "shrink_64x64", "expand_16x32", "expand_16x64", "expand_64x32",
+                 "expand_64x64", "expand_64x128"):
+        assert b"lf_low_rank_" + name.encode() + b"\0" in _abi.code_object_bytes()
     assert low_rank.workspace_bytes(d) >= 256 + 4096 * 128 * 4
     for bad in (low_rank.LowRankDescriptor(),):
         with pytest.raises(DeviceError):
@@ -70,7 +82,7 @@ def test_binding_refusals():
     ad, counts = adapters(rt), FakeAllocation(20)
     x, y = region(2 * 8 * 256), region(2 * 8 * 192)
     bind = lambda ids=region(32, 4), x=x, y=y, out=y, m=8: low_rank.bind_low_rank(rt, counts, ids, x, ad, y, out, m)  # noqa: E731
-    assert [s.name for s in bind().steps] == ["lf_low_rank_r16"]
+    assert [s.name for s in bind().steps] == ["lf_low_rank_n1"]
     wide = FakeAllocation(4 * 8 * 192)
     part = lambda offset: wide_region(wide, offset)  # noqa: E731
     bind(y=part(0), out=part(2 * 8 * 192))
