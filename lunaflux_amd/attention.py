@@ -203,7 +203,8 @@ class PagedStep:
         positions [rows, axes] (or [rows] for one axis); None leaves what the
         region holds. DeviceError INVALID_ARGUMENT, with nothing written, for a
         step that does not fit or contradicts itself (page indices are the
-        cache owner's, and checked on the device)."""
+        cache owner's, and checked on the device). Launches that read the step
+        before have to be over: the caller synchronizes their streams first."""
         row_offsets, lengths = np.asarray(row_offsets), np.asarray(lengths)
         n = lengths.size
         for a in (row_offsets, lengths):
