@@ -87,7 +87,9 @@ int64_t tile_rows(const lf_fp8_attn_desc *d) {
 }
 
 // kernels/attention.hip, blocks: blocks of the decode grid.
-int64_t decode_blocks(const lf_fp8_attn_desc *d) { return d->head_dim == 64 ? 512 : 256; }
+int64_t decode_blocks(const lf_fp8_attn_desc *d) {
+  return d->head_dim * (d->cache == LF_FP8_CACHE_E4M3 ? 1 : 2) <= 128 ? 512 : 256;
+}
 
 // The decode workspace: a line with the error word, two arrival counters per
 // partial result, two partial results per block (fp32 [rows][D] sums, maxima

@@ -27,7 +27,8 @@ LF_DEVICE float e4m3_range(float x, float inv_scale) {
   const float v = x * inv_scale;
   return v != v ? v : fminf(fmaxf(v, -448.0f), 448.0f);
 }
-LF_DEVICE uint2 e4m3x8_of(const float *v, float inv_scale) {
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+LF_DEVICE u32x2 e4m3x8_of(const float *v, float inv_scale) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -37,7 +38,7 @@ LF_DEVICE uint2 e4m3x8_of(const float *v, float inv_scale) {
                                         true);
     w[i] = static_cast<uint32_t>(p);
   }
-  return make_uint2(w[0], w[1]);
+  return u32x2{w[0], w[1]};
 }
 
 // The sequence of a row: the number of sequences that end at or before it.
@@ -54,7 +55,13 @@ LF_DEVICE int sequence_of(const int32_t *row_offsets, int sequences, int row) {
 // One block per row, D / 16 lanes per head: a lane holds the 16 values
 // [o0, o0 + 8) and [o1, o1 + 8) of its head, which are eight whole rotary
 // pairs, so the rotation needs no exchange and every load and store is 16
-// bytes.
+// bytes. Loads and stores are nontemporal: 8192 rows of 32 + 16 heads of 128 take
+// 37.7 us so (201 MB at 5.3 TB/s, the rate of a copy), 46.5 otherwise; the rows'
+// loads a step ahead of their use cost occupancy (50).
+template <class T, class P>
+LF_DEVICE void put(P *to, T value) {
+  __builtin_nontemporal_store(value, reinterpret_cast<T *>(to));
+}
 template <bool E4M3>
 LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, const int32_t *row_offsets,
                             const int32_t *lengths, const int32_t *page_offsets, const int32_t *page_indices,
@@ -107,8 +114,8 @@ LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, con
     const int h = base + lane / lanes;
     if (h >= heads) continue;
     const uint16_t *src = qkv + (static_cast<uint64_t>(row) * heads + h) * D;
-    const u32x4 w0 = *reinterpret_cast<const u32x4 *>(src + o0);
-    const u32x4 w1 = *reinterpret_cast<const u32x4 *>(src + o1);
+    const u32x4 w0 = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + o0));
+    const u32x4 w1 = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + o1));
     float a[8], b[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -159,19 +166,19 @@ LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, con
     }
     if (h < Hq) {
       uint16_t *dst = q + (static_cast<uint64_t>(row) * Hq + h) * D;
-      *reinterpret_cast<u32x4 *>(dst + o0) = bf16x8_of(a);
-      *reinterpret_cast<u32x4 *>(dst + o1) = bf16x8_of(b);
+      put(dst + o0, bf16x8_of(a));
+      put(dst + o1, bf16x8_of(b));
     } else if (place.page >= 0) {
       const bool value = h >= Hq + Hkv;
       const int kh = h - Hq - (value ? Hkv : 0);
       uint8_t *dst = (value ? vc : kc) + cache_byte<E4M3>(d, place.page, kh, place.slot);
       if constexpr (E4M3) {
         const float inv_scale = 1.0f / scales[(value ? Hkv : 0) + kh];
-        *reinterpret_cast<uint2 *>(dst + o0) = e4m3x8_of(a, inv_scale);
-        *reinterpret_cast<uint2 *>(dst + o1) = e4m3x8_of(b, inv_scale);
+        put(dst + o0, e4m3x8_of(a, inv_scale));
+        put(dst + o1, e4m3x8_of(b, inv_scale));
       } else {
-        *reinterpret_cast<u32x4 *>(dst + 2 * o0) = bf16x8_of(a);
-        *reinterpret_cast<u32x4 *>(dst + 2 * o1) = bf16x8_of(b);
+        put(dst + 2 * o0, bf16x8_of(a));
+        put(dst + 2 * o1, bf16x8_of(b));
       }
     }
   }
@@ -186,14 +193,18 @@ LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, con
 // blocks leave a partial result (fp32 sums, maximum and weight sum of each of
 // the tile's rows) in the workspace; of every kGroup neighbours the last to
 // arrive adds the group's up in order, and the last group to arrive the
-// groups'. Partial results are stored and loaded at agent scope (past the XCD's
+// groups'. HBM bounds it (5.8 TB/s of 131071 keys); a launch with nothing to read
+// takes 5 us, the join 3 to 6, and the XCDs' rates differ by a tenth while their
+// shares are equal. Partial results are stored and loaded at agent scope (past the XCD's
 // L2), and a block counts itself only once its stores have completed.
 constexpr int kWaves = 4;
 
-// Blocks of the grid: one per CU, two with heads of 64 values (half the bytes in
-// flight per wave).
-template <int D>
-LF_DEVICE constexpr int blocks() { return D == 64 ? 512 : 256; }
+// Blocks of the grid: one per CU, two where a key is 128 bytes or less and one
+// would have too few bytes in flight: 96 sequences of up to 5003 keys, heads of 128
+// in e4m3, 126 us with one and 111 with two; in bf16 92 and 102 for 131071 keys, 44
+// and 49 for 32 sequences.
+template <int D, bool E4M3>
+LF_DEVICE constexpr int blocks() { return D * (E4M3 ? 1 : 2) <= 128 ? 512 : 256; }
 
 // Workspace: a line with the error word, arrival counters of groups (at their
 // first part's place) and of pairs (at theirs), the partial results, two per
@@ -203,9 +214,9 @@ struct Ws {
   float *parts, *groups;
   int floats;  // of a partial result: [rows][D] sums, rows maxima, rows weight sums
 };
-template <int D>
+template <int D, bool E4M3>
 LF_DEVICE Ws ws_of(uint8_t *ws, int tile_rows) {
-  constexpr int places = 2 * blocks<D>();
+  constexpr int places = 2 * blocks<D, E4M3>();
   Ws w;
   w.error = reinterpret_cast<int *>(ws);
   w.group_arrivals = reinterpret_cast<int *>(ws + 256);
@@ -329,21 +340,18 @@ struct Tile {
   uint32_t v[8][kWords];
 };
 
+// Values of one row, 16 lanes taking the whole of it: nontemporal, since nothing
+// reads them again (131071 keys 102 us with plain loads and 92 so, 32 sequences 49
+// and 44). Keys, whose lines two loads share, are faster so in bf16 (94, 47) and
+// slower in e4m3 (129, 132), with values so both ways: they are loaded plainly.
 template <int WORDS>
 LF_DEVICE void load_words(uint32_t (&dst)[WORDS], const uint8_t *src) {
-  if constexpr (WORDS == 1) {
-    dst[0] = *reinterpret_cast<const uint32_t *>(src);
-  } else if constexpr (WORDS == 2) {
-    const uint2 w = *reinterpret_cast<const uint2 *>(src);
-    dst[0] = w.x;
-    dst[1] = w.y;
-  } else {
+  typedef uint32_t Words __attribute__((ext_vector_type(WORDS < 4 ? WORDS : 4)));
 #pragma unroll
-    for (int i = 0; i < WORDS; i += 4) {
-      const u32x4 w = *reinterpret_cast<const u32x4 *>(src + 4 * i);
+  for (int i = 0; i < WORDS; i += 4) {
+    const Words w = __builtin_nontemporal_load(reinterpret_cast<const Words *>(src + 4 * i));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dst[i + e] = w[e];
-    }
+    for (int e = 0; e < (WORDS < 4 ? WORDS : 4); ++e) dst[i + e] = w[e];
   }
 }
 
@@ -414,7 +422,8 @@ LF_DEVICE float max_over_groups(float v) {
 }
 
 // A part of a pair: the tiles of keys [base, stop) of a sequence whose keys [lo,
-// len) count, stop at most len, for `live` query heads from head `row0` of key head h's group on.
+// len) count, stop at most len, for `live` query heads from head `row0` of key
+// head h's group on.
 struct Piece {
   const int32_t *table;
   int lo, len, base, stop;
@@ -490,9 +499,9 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   const bool counted = carry * head_tiles <= INT32_MAX;
   if (!counted) bad = true;
   const int items = __builtin_amdgcn_readfirstlane(counted ? static_cast<int>(carry) * head_tiles : 0);
-  const int share = share_of(items, n * head_tiles, blocks<D>());
+  const int share = share_of(items, n * head_tiles, blocks<D, E4M3>());
   const int tile_rows = group < kHeadTile ? group : kHeadTile;
-  const Ws w = ws_of<D>(ws, tile_rows);
+  const Ws w = ws_of<D, E4M3>(ws, tile_rows);
   if (bad) flag_error(w.error);
 
   const int shift = __builtin_ctz(d.page_size);
@@ -801,27 +810,27 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
 
 }  // namespace attn
 
-#define LF_ATTN_ROPE(TYPE, E4M3)                                                                             \
-  extern "C" __global__ __launch_bounds__(256) void lf_attn_qk_norm_rope_##TYPE(                             \
-      const int32_t *__restrict__ counts, const int32_t *__restrict__ positions, \
-      const int32_t *__restrict__ row_offsets, const int32_t *__restrict__ lengths, \
-      const int32_t *__restrict__ page_offsets, const int32_t *__restrict__ page_indices, \
-      const uint8_t *__restrict__ desc, const uint16_t *__restrict__ qkv, \
-      const uint16_t *__restrict__ gq, const uint16_t *__restrict__ gk, uint16_t *__restrict__ q, \
-      uint8_t *__restrict__ kc, uint8_t *__restrict__ vc, int *__restrict__ status) { \
-    attn::qk_norm_rope<E4M3>(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv, \
-                             gq, gk, q, kc, vc, status);                                                     \
+#define LF_ATTN_ROPE(TYPE, E4M3)                                                                               \
+  extern "C" __global__ __launch_bounds__(256) void lf_attn_qk_norm_rope_##TYPE(                               \
+      const int32_t *__restrict__ counts, const int32_t *__restrict__ positions,                               \
+      const int32_t *__restrict__ row_offsets, const int32_t *__restrict__ lengths,                            \
+      const int32_t *__restrict__ page_offsets, const int32_t *__restrict__ page_indices,                      \
+      const uint8_t *__restrict__ desc, const uint16_t *__restrict__ qkv,                                      \
+      const uint16_t *__restrict__ gq, const uint16_t *__restrict__ gk, uint16_t *__restrict__ q,              \
+      uint8_t *__restrict__ kc, uint8_t *__restrict__ vc, int *__restrict__ status) {                          \
+    attn::qk_norm_rope<E4M3>(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv,   \
+                             gq, gk, q, kc, vc, status);                                                       \
   }
 LF_ATTN_ROPE(bf16, false)
 LF_ATTN_ROPE(e4m3, true)
 
 #define LF_ATTN_DECODE(D, TYPE, E4M3)                                                                          \
-  extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void lf_attn_decode_d##D##_##TYPE(                              \
-      const int32_t *__restrict__ counts, const int32_t *__restrict__ row_offsets, \
-      const int32_t *__restrict__ lengths, const int32_t *__restrict__ page_offsets, \
-      const int32_t *__restrict__ page_indices, const uint8_t *__restrict__ desc, \
-      const uint16_t *__restrict__ q, uint16_t *__restrict__ out, const uint8_t *__restrict__ kc, \
-      const uint8_t *__restrict__ vc, uint8_t *__restrict__ ws) { \
+  extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void lf_attn_decode_d##D##_##TYPE(            \
+      const int32_t *__restrict__ counts, const int32_t *__restrict__ row_offsets,                             \
+      const int32_t *__restrict__ lengths, const int32_t *__restrict__ page_offsets,                           \
+      const int32_t *__restrict__ page_indices, const uint8_t *__restrict__ desc,                              \
+      const uint16_t *__restrict__ q, uint16_t *__restrict__ out, const uint8_t *__restrict__ kc,              \
+      const uint8_t *__restrict__ vc, uint8_t *__restrict__ ws) {                                              \
     attn::decode<D, E4M3>(counts, row_offsets, lengths, page_offsets, page_indices, desc, q, out, kc, vc, ws); \
   }
 LF_ATTN_DECODE(64, bf16, false)

@@ -193,7 +193,10 @@ struct ColumnChunk {
   }
 };
 // y of rows `row` + 4 g + i; rows and columns that are not to be written read
-// others
+// others. Stores are nontemporal, and where many rows make a stream of it the
+// loads too: 4093 rows 58.3 us with both, 60.0 with the stores alone, 62.0 with
+// neither; 509 rows 18.7, 17.8 and 17.9.
+template <bool STREAM>
 struct ColumnRows {
   u32x4 y[4];
   LF_DEVICE void load(const Desc &d, uint32_t mine, int row, int any, int n, int end, const uint16_t *yp) {
@@ -202,7 +205,8 @@ struct ColumnRows {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int m = (mine >> (4 * g + i)) & 1 ? row + 4 * g + i : any;
-      y[i] = *reinterpret_cast<const u32x4 *>(yp + static_cast<uint64_t>(m) * d.columns + col);
+      const u32x4 *src = reinterpret_cast<const u32x4 *>(yp + static_cast<uint64_t>(m) * d.columns + col);
+      y[i] = STREAM ? __builtin_nontemporal_load(src) : *src;
     }
   }
   LF_DEVICE void store(const Desc &d, const f32x4 (&acc)[8], float scale, uint32_t mine, int row, int n, int end,
@@ -219,7 +223,8 @@ struct ColumnRows {
                              __builtin_bit_cast(float, y[i][k] & 0xffff0000u) + scale * acc[2 * k + 1][i]};
           o[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(sum, bf16x2));
         }
-        *reinterpret_cast<u32x4 *>(out + static_cast<uint64_t>(row + 4 * g + i) * d.columns + n + 8 * c) = o;
+        uint16_t *to = out + static_cast<uint64_t>(row + 4 * g + i) * d.columns + n + 8 * c;
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x4 *>(to));
       }
     }
   }
@@ -291,7 +296,7 @@ LF_DEVICE void one_launch(const int32_t *counts, const int32_t *ids, const uint8
     const float scale = scaling[adapter];
     const int any = __builtin_ctzll(mine);
     ColumnChunk<kRanks / 4, kRanks> chunk;
-    ColumnRows column;
+    ColumnRows<false> column;
     if (n < cols.end) {
       chunk.load(d, adapter, n, cols.end, 0, lane, b);
       column.load(d, static_cast<uint32_t>(mine), row0, row0 + any, n, cols.end, y);
@@ -506,7 +511,7 @@ LF_DEVICE void expand(const int32_t *counts, const int32_t *ids, const uint8_t *
     const int begin = cols.first + kGroupColumns * side;
     if (begin >= cols.end) return;  // (alike for all waves that share a stage)
     ColumnChunk<RANKS / (RW == 4 ? 16 : 4), RANKS> chunk;
-    ColumnRows column[2];
+    ColumnRows<RW == 4> column[2];
     chunk.load(d, adapter, begin, cols.end, 0, loader, b);
     column[0].load(d, mine, row, any, begin, cols.end, y);
     sync();  // what the stage held has been read
