@@ -20,13 +20,15 @@ constexpr int64_t kHeaderBytes = 256;
 int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t cut(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
-// The one launch reads a slice's A once per 1024 columns, so A has to be small
-// enough to come from L2 quickly, and gives each adapter of 16 rows a block. Against
-// two launches (columns 4096 + 2 x 1024, an adapter per row or so): 61 rows of rank
-// 16 of 4096 13 us and 25, of rank 64 33 and 35, of rank 128 53 and 45; 128 rows 19
-// and 31, 50 and 47, 84 and 64; 256 rows 31 and 39, 83 and 83, 139 and 88.
+// The one launch reads a slice's A once per 1024 columns and 16 rows, so A has to
+// be small enough to come from L2 quickly, and gives each adapter of 16 rows a
+// block. Against two launches (columns 4096 + 2 x 1024, hidden 4096, an adapter per
+// row or so): 16 rows of rank 16, 64 and 128 9 us and 20, 17 and 24, 26 and 37; 61
+// rows 13 and 25, 33 and 35, 53 and 45; 128 rows 19 and 31, 50 and 47, 84 and 64; 256
+// rows 31 and 39, 83 and 83, 139 and 88.
 int32_t one_launch_of(const lf_fp8_low_rank_desc *d) {
-  return d->max_tokens <= 128 && int64_t(d->rank) * d->hidden <= 262144 ? 1 : 0;
+  const int64_t values = int64_t(d->rank) * d->hidden;
+  return d->max_tokens <= 256 && values <= (1 << 19) && d->max_tokens * values <= (1 << 24) ? 1 : 0;
 }
 
 // A shrink block's rows and columns of x A^T; with 32 columns where there are no
@@ -37,11 +39,13 @@ int64_t shrink_blocks(const lf_fp8_low_rank_desc *d) {
   return cut(d->max_tokens, kTileRows) * cut(int64_t(d->slices) * d->rank, chunk_of(d));
 }
 
-// Slices of hidden: two or more steps of 64 for each of a block's eight waves, and
-// no more blocks than the chip has compute units.
+// Slices of hidden: four or more steps of 64 for each of a block's eight waves, and
+// no more blocks than the chip has compute units. Every block of the second launch
+// adds the slices up again: 509 rows of 14336 take 16.9 us in slices of 2048, 17.7 of
+// 1024 and 18.5 of 2560, 800 rows 23, 31 and 24, 1000 rows of 4096 27, 30 and 32.
 int32_t splits_of(const lf_fp8_low_rank_desc *d) {
   if (one_launch_of(d)) return 1;
-  return static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({16, d->hidden / 1024, 256 / shrink_blocks(d)})));
+  return static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({16, d->hidden / 2048, 256 / shrink_blocks(d)})));
 }
 
 // Blocks that share a tile's adapters. In the two launches most tiles of long

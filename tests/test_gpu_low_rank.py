@@ -57,7 +57,7 @@ def check(got, y, want, tol, ids, n):
 
 
 @pytest.mark.parametrize("m,max_tokens", [(1, 1), (1, 16), (15, 16), (17, 64), (128, 128), (61, 61), (129, 129), (64, 256),
-                                          (333, 512)])
+                                          (333, 512), (600, 1000)])
 @pytest.mark.parametrize("hidden,widths,rank,n", [(128, [64], 16, 1), (512, [512, 128, 128], 16, 5), (1408, [64, 192], 48, 20),
                                                   (2048, [320], 128, 3), (4096, [64, 64, 64, 128], 64, 40)])
 def test_low_rank(rt, m, max_tokens, hidden, widths, rank, n):
@@ -71,7 +71,7 @@ def test_low_rank(rt, m, max_tokens, hidden, widths, rank, n):
 
 @pytest.mark.parametrize("ids", [lambda m: np.full(m, -1), lambda m: np.full(m, 3), lambda m: np.arange(m) // 100,
                                  lambda m: np.arange(m) % 7, lambda m: np.where(np.arange(m) % 2, -1, 6)])
-@pytest.mark.parametrize("m", [40, 300])
+@pytest.mark.parametrize("m", [40, 300, 700])
 def test_low_rank_rows_of_adapters(rt, m, ids):
     rng = np.random.default_rng(m)
     x, y, a, b, scaling = arrays(rng, m, 256, [128, 64], 16, 7)
@@ -89,7 +89,7 @@ def test_low_rank_of_ranks_below_a_tile(rt):
     check(low_rank.low_rank(rt, x, y, ids, adapters), y, *expected(x, y, a, b, scaling, ids, [64]), ids, 2)
 
 
-@pytest.mark.parametrize("m", [20, 200])
+@pytest.mark.parametrize("m", [20, 200, 300, 600])
 def test_low_rank_rows_do_not_meet_other_adapters(rt, m):
     """Infinities and NaN in one adapter, or in one row, stay with its rows."""
     rng = np.random.default_rng(2)
@@ -104,7 +104,7 @@ def test_low_rank_rows_do_not_meet_other_adapters(rt, m):
     assert np.isnan(got[ids == 1]).all() and not np.isfinite(got[ids == 2]).any() and not np.isfinite(got[3]).any()
 
 
-@pytest.mark.parametrize("m,cap", [(3, 16), (70, 256), (0, 16)])
+@pytest.mark.parametrize("m,cap", [(3, 16), (70, 256), (0, 16), (130, 300), (0, 300), (333, 700)])
 def test_low_rank_out_of_place_and_rows_behind_the_batch(rt, m, cap):
     rng = np.random.default_rng(3)
     widths, n = [192], 2

@@ -19,9 +19,10 @@ def test_descriptor_and_geometry():
     assert geometry[0][0].grid == (4 * 16, 6, 1) and d.slots == 16 and d.one_launch == 1
     assert low_rank.workspace_bytes(d) == 256
     for rank, hidden, rows, first, last in ((32, 4096, 128, "n2", None), (64, 2048, 128, "n4", None),
-                                            (128, 1024, 1, "n4", None), (64, 4096, 128, "n4", None), (80, 4096, 128, "shrink_64x64", "expand_64x128"),
+                                            (128, 1024, 1, "n4", None), (128, 4096, 32, "n4", None), (80, 4096, 128, "shrink_64x64", "expand_64x128"),
+                                            (16, 4096, 256, "n1", None), (64, 4096, 128, "shrink_64x64", "expand_16x64"),
                                             (64, 4096, 256, "shrink_64x64", "expand_16x64"),
-                                            (16, 4096, 129, "shrink_64x32", "expand_16x32"),
+                                            (16, 4096, 257, "shrink_64x32", "expand_16x32"),
                                             (48, 14336, 1, "shrink_64x64", "expand_16x64"),
                                             (80, 14336, 1, "shrink_64x64", "expand_64x128"),
                                             (16, 128, 513, "shrink_64x32", "expand_64x32"),
