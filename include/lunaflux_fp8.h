@@ -3,7 +3,8 @@
  * catalog: the weight-region format that model/device_materialize writes,
  * the host-side pre-swizzle, the launch geometry a manifest records, and the
  * gfx950 kernel entry points (symbols in lunaflux_fp8.hsaco) with their
- * operand lists.
+ * operand lists; and the operators beside the projections: attention over a
+ * paged cache and low-rank adapters.
  *
  * Operand convention (kernels/launch_contract/paged_admit.mbt:76-107): every
  * kernel parameter is a device region, in canonical order runtime inputs,
@@ -600,7 +601,7 @@ typedef struct lf_fp8_attn_desc {
 /* Checks the fields of *desc, and writes its magic, default strides and the
  * region offsets. LF_INVALID_ARGUMENT for values outside the ranges above,
  * strides that overlap or are not multiples of 16 bytes, or bounds past 32
- * bits (table_entries * page_size, the 128-key tiles of a step times heads). */
+ * bits (table_entries * page_size, the 32-key tiles of a step times heads). */
 int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *desc);
 /* Writes the descriptor region (desc->region_bytes bytes). scales: 2 kv_heads
  * values, finite and above zero (null for a bf16 cache: ones); turns and axis:

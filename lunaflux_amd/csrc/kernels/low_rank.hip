@@ -9,10 +9,10 @@
 //
 // 61 rows of 16 adapters, hidden 4096, rank 16, columns 4096 + 2 x 1024: 13 us in
 // one launch, of which launch and the chain of loads (ids, x and A, B, y) are nearly
-// all; the bytes, at the rate of a copy, would take 2. 4093 rows, rank 64: 27 us for x
-// A^T (8 TB/s from L2) and 34 for the rest (3 TB/s of y and out; 27 without the
-// products), 60 together, the bytes 27. One product of operands loaded from memory
-// straight into the layout of the matrix instructions took 82 + 51.
+// all; the bytes, at the rate of a copy, would take 2. 4093 rows, rank 64: 25 us for x
+// A^T (8 TB/s from L2) and 32 for the rest (3.7 TB/s from and to HBM; 7 less without
+// the products), 56 together, the bytes 28. Operands loaded from memory straight into
+// the layout of the matrix instructions took 82 + 51.
 #include "device_common.h"
 #include "phases.h"
 
@@ -476,7 +476,7 @@ LF_DEVICE void expand(const int32_t *counts, const int32_t *ids, const uint8_t *
     if (k < R) {
       const int at = row0 + m < rows ? row0 + m : rows - 1;
       const float *from = parts + static_cast<uint64_t>(at) * SR + cols.slice * R + k;
-      constexpr int kBatch = 8;
+      constexpr int kBatch = RW == 4 ? 4 : 8;  // (4093 rows, one split: 56 us, with 8 58)
       for (int s0 = 0; s0 < d.splits; s0 += kBatch) {
         f32x4 v[kBatch];
 #pragma unroll
