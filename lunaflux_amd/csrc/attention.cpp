@@ -17,6 +17,7 @@ constexpr int64_t kLimit32 = (int64_t(1) << 31) - 1;
 constexpr int64_t kTileKeys = 32;
 constexpr int64_t kGroup = 32;
 constexpr int64_t kHeadTile = 16;
+constexpr int64_t kMostItems = kLimit32 - (1 << 22);  // attention_index.h
 constexpr int64_t kWaves = 4;
 
 int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
@@ -69,10 +70,11 @@ bool fields_ok(const lf_fp8_attn_desc *d) {
     return false;
   }
   if (d->norm == 1 && !(d->norm_epsilon >= 0.0f && std::isfinite(d->norm_epsilon))) return false;
-  // The kernels count cached tokens, positions and (key tile, head tile) items in 31 bits.
+  // The kernels count cached tokens, positions and (key tile, head tile) items in 31
+  // bits, HIP a grid's threads in 32.
   if (int64_t(d->table_entries) * d->page_size > kLimit32 - 1024 ||
-      int64_t(d->max_tokens) * d->axes > kLimit32 || int64_t(d->max_tokens) > (1 << 24) ||
-      (int64_t(d->table_entries) * d->page_size / kTileKeys + 2 * d->max_sequences) * head_tiles(d) > kLimit32) {
+      int64_t(d->max_tokens) * d->axes > kLimit32 || d->max_tokens >= (1 << 24) ||
+      (int64_t(d->table_entries) * d->page_size / kTileKeys + 2 * d->max_sequences) * head_tiles(d) > kMostItems) {
     return false;
   }
   return true;

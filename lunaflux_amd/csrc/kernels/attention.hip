@@ -496,7 +496,7 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   const int group_tiles = (group + kHeadTile - 1) / kHeadTile;
   const int head_tiles = head_tiles_of(d);
   // (page ranges that overlap may add up to more than the descriptor's bound)
-  const bool counted = carry * head_tiles <= INT32_MAX;
+  const bool counted = carry * head_tiles <= kMostItems;
   if (!counted) bad = true;
   const int items = __builtin_amdgcn_readfirstlane(counted ? static_cast<int>(carry) * head_tiles : 0);
   const int share = share_of(items, n * head_tiles, blocks<D, E4M3>());
@@ -524,8 +524,8 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       const int i = __builtin_amdgcn_readfirstlane(sequence_at(prefix, n, head_tiles, u));
       bool unused = false;
       const Sequence seq = i < 64 * kWaves ? near[i] : load_sequence(s0 + i, unused);
-      const Span span = {__builtin_amdgcn_readfirstlane(seq.span.first_tile), __builtin_amdgcn_readfirstlane(seq.span.tiles),
-                         __builtin_amdgcn_readfirstlane(seq.span.lo), __builtin_amdgcn_readfirstlane(seq.span.len)};
+      auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+      const Span span = {same(seq.span.first_tile), same(seq.span.tiles), same(seq.span.lo), same(seq.span.len)};
       const int within = u - __builtin_amdgcn_readfirstlane(prefix[i]) * head_tiles;
       const int ht = within / span.tiles, t0 = within - ht * span.tiles;
       const int t1 = span.tiles - t0 < end - u ? span.tiles : t0 + (end - u);
@@ -556,7 +556,9 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   auto indices = [&](const int32_t *table, int lo, int len, int base) {
     return table[entry_of(lo >> shift, (len + slot_mask) >> shift, shift, base + 8 * (lane & 3))];
   };
-  auto tile_groups = [&](int page, int base) { return groups_of(page, pages, page_bytes, token_bytes, slot_mask, base); };
+  auto tile_groups = [&](int page, int base) {
+    return groups_of(page, pages, page_bytes, token_bytes, slot_mask, base);
+  };
   // this lane's part of a head's rows: of keys, row c % 8 of a group of eight,
   // chunk g; of values, row 4 g of a half
   const uint32_t key_lane = (c & 7) * token_bytes + 16 * g;

@@ -115,6 +115,7 @@ LF_DEVICE Decoded decoded_of(const Desc &d, int s0, int n, int total) {
 // (b + 1) share): a part of a pair is worth adding up from about kLeastShare
 // tiles on, and pairs shorter than that get a block each while there are enough.
 constexpr int kLeastShare = 8;
+constexpr int kMostItems = INT32_MAX - (1 << 22);  // leaves the sums below room for blocks and pairs
 LF_DEVICE int share_of(int items, int pairs, int blocks) {
   if (pairs < 1) return 1;
   const int share = (items + blocks - 1) / blocks, whole = (items + pairs - 1) / pairs;

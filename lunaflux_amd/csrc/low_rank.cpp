@@ -74,6 +74,12 @@ int32_t column_blocks_of(const lf_fp8_low_rank_desc *d) {
   return static_cast<int32_t>(blocks);
 }
 
+// Multiples of 8: XCDs have neighbouring blocks each.
+int64_t shrink_grid(const lf_fp8_low_rank_desc *d) { return align_up(shrink_blocks(d) * splits_of(d), 8); }
+int64_t expand_grid(const lf_fp8_low_rank_desc *d) {
+  return align_up(cut(d->max_tokens, expand_rows(d)) * column_blocks_of(d), 8);
+}
+
 bool fields_ok(const lf_fp8_low_rank_desc *d) {
   if (d->adapters < 1 || d->adapters > 65536 || d->rank < 16 || d->rank > 128 || d->rank % 16 != 0 ||
       d->hidden < 128 || d->hidden > kMaxWidth || d->hidden % 128 != 0 || d->slices < 1 ||
@@ -86,7 +92,8 @@ bool fields_ok(const lf_fp8_low_rank_desc *d) {
     if (d->ends[i] <= before || d->ends[i] % 64 != 0) return false;
     before = d->ends[i];
   }
-  return before == d->columns;
+  // HIP counts a grid's threads in 32 bits.
+  return before == d->columns && shrink_grid(d) * 512 <= UINT32_MAX && expand_grid(d) * 256 <= UINT32_MAX;
 }
 
 bool desc_ok(const lf_fp8_low_rank_desc *d) {
@@ -149,14 +156,13 @@ int32_t lunaflux_fp8_low_rank_launch_geometry(int32_t entry, const lf_fp8_low_ra
     std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_low_rank_shrink_%dx%d", static_cast<int>(kTileRows),
                   static_cast<int>(chunk_of(d)));
     threads = 512;
-    gx = align_up(shrink_blocks(d) * d->splits, 8);  // XCDs have neighbouring blocks each
+    gx = shrink_grid(d);
   } else {
     std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_low_rank_expand_%dx%d", static_cast<int>(expand_rows(d)),
                   d->rank <= 32 ? 32 : d->rank <= 64 ? 64 : 128);
-    gx = align_up(cut(d->max_tokens, expand_rows(d)) * d->column_blocks, 8);
+    gx = expand_grid(d);
   }
   if (!d->one_launch) gy = d->slots;
-  if (gx > INT32_MAX) return LF_UNSUPPORTED;
   dims[0] = static_cast<int32_t>(gx);
   dims[1] = static_cast<int32_t>(gy);
   dims[2] = 1;

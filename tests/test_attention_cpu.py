@@ -40,7 +40,7 @@ def test_descriptor_defaults_and_layout():
 @pytest.mark.parametrize("changes", [
     dict(query_heads=7), dict(query_heads=0), dict(kv_heads=0), dict(query_heads=2048, kv_heads=2048),
     dict(head_dim=96), dict(head_dim=32), dict(head_dim=512), dict(page_size=4), dict(page_size=24),
-    dict(page_size=2048), dict(pages=0), dict(max_tokens=0), dict(max_tokens=1 << 25), dict(max_sequences=0),
+    dict(page_size=2048), dict(pages=0), dict(max_tokens=0), dict(max_tokens=1 << 25), dict(max_tokens=1 << 24), dict(max_sequences=0),
     dict(max_sequences=2049), dict(table_entries=0), dict(table_entries=1 << 27), dict(table_entries=1 << 40),
     dict(window=-1), dict(norm_epsilon=-1.0), dict(norm_epsilon=math.nan), dict(norm_epsilon=math.inf),
     dict(softmax_scale=math.inf), dict(softmax_scale=math.nan), dict(pages=1 << 33), dict(pages=1.5),

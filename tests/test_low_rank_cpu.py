@@ -51,7 +51,7 @@ def test_descriptor_and_geometry():
     (2, 24, 512, [512], 8), (2, 144, 512, [512], 8), (2, 16, 500, [512], 8), (2, 16, 0, [512], 8),
     (2, 16, 1 << 40, [512], 8), (2, 16, 512, [], 8), (2, 16, 512, [64] * 5, 8), (2, 16, 512, [96], 8),
     (2, 16, 512, [512, 0], 8), (2, 16, 512, [-64, 128], 8), (2, 16, 512, [1 << 40], 8), (2, 16, 512, [512], 0),
-    (2, 16, 512, [512], 1 << 25), (2, 16, 512, [512], 1 << 40), (1 << 40, 16, 512, [512], 8),
+    (2, 16, 512, [1 << 20], 1 << 24), (2, 16, 512, [512], 1 << 25), (2, 16, 512, [512], 1 << 40), (1 << 40, 16, 512, [512], 8),
 ])
 def test_descriptor_refusals(args):
     with pytest.raises(DeviceError):
