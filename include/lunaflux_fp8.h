@@ -663,7 +663,7 @@ typedef struct lf_fp8_low_rank_desc {
   int32_t slots;      /* blocks that share a tile's adapters, written as splits */
   int32_t one_launch; /* 1 or 0, written as splits */
   int32_t column_blocks; /* blocks a tile's columns are cut into, written as splits */
-  int32_t reserved;
+  int32_t block_columns; /* their most columns, written as splits */
 } lf_fp8_low_rank_desc;
 
 enum lf_fp8_low_rank_entry {

@@ -23,7 +23,7 @@ struct Desc {
   uint32_t magic;
   int32_t adapters, rank, hidden, slices, columns, max_tokens, splits;
   int32_t ends[4];
-  int32_t slots, one_launch, column_blocks, reserved;
+  int32_t slots, one_launch, column_blocks, block_columns;
 };
 constexpr uint32_t kMagic = 0x4B4E524Cu;
 LF_DEVICE const Desc &desc_of(const uint8_t *region) { return *reinterpret_cast<const Desc *>(region); }
@@ -140,7 +140,8 @@ LF_DEVICE void split_bf16(float v, __bf16 &top, __bf16 &rest) {
 struct Columns {
   int slice, first, end;
 };
-LF_DEVICE Columns columns_of(const Desc &d, int block, int width) {
+LF_DEVICE Columns columns_of(const Desc &d, int block) {
+  const int width = d.block_columns;
   int begin = 0;
   for (int s = 0; s < d.slices; ++s) {
     const int blocks = (d.ends[s] - begin + width - 1) / width;
@@ -266,7 +267,7 @@ LF_DEVICE void copy_others(const Desc &d, uint32_t none, int row, int n, int end
 // of the slice by itself (the waves take the steps in turn and add up in wave
 // order through LDS): reading A again per 1024 columns, from L2, costs less than
 // passing x A^T from block to block.
-constexpr int kOneWaves = 8, kOneColumns = kOneWaves * kGroupColumns;
+constexpr int kOneWaves = 8;  // of 128 columns each
 template <int NT>
 LF_DEVICE void one_launch(const int32_t *counts, const int32_t *ids, const uint8_t *desc, const float *scaling,
                           const uint16_t *x, const uint16_t *a, const uint16_t *b, const uint16_t *y, uint16_t *out,
@@ -285,7 +286,7 @@ LF_DEVICE void one_launch(const int32_t *counts, const int32_t *ids, const uint8
   const int slot = (blockIdx.x - tile * d.slots + 2 * tile) % d.slots;
   if (row0 >= rows) return;
   const int id = tile_ids<16>(d, ids, row0, rows, reinterpret_cast<int *>(ws));
-  const Columns cols = columns_of(d, blockIdx.y, kOneColumns);
+  const Columns cols = columns_of(d, blockIdx.y);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int r8 = lane >> 3, ch = lane & 7;
@@ -427,14 +428,12 @@ LF_DEVICE void shrink(const int32_t *counts, const int32_t *ids, const uint8_t *
   });
 }
 
-// y + s v B^T, v from the workspace, for 16 RW rows and up to 512 columns of a
-// slice; RANKS = the rank, up to a power of two. RW 4: four waves of 16 rows each
+// y + s v B^T, v from the workspace, for 16 RW rows and a block's columns of a slice; RANKS = the rank, up to a power of two. RW 4: four waves of 16 rows each
 // go through the columns together, with one copy of B in LDS; RW 1: each wave has
 // 128 columns of the same 16 rows. The next columns' B and y are loaded while
 // these are multiplied; B first, so that the wait for it leaves y in flight, and it
 // goes to LDS before the results are stored, so that no wait for a load is one for
 // a store behind it.
-constexpr int kExpandColumns = 512;
 template <int RW, int RANKS>
 LF_DEVICE void expand(const int32_t *counts, const int32_t *ids, const uint8_t *desc, const float *scaling,
                       const uint16_t *b, const uint16_t *y, uint16_t *out, uint8_t *ws) {
@@ -450,7 +449,7 @@ LF_DEVICE void expand(const int32_t *counts, const int32_t *ids, const uint8_t *
   bool some = false;
   for_adapters(id, slot, gridDim.y, [&](int, uint64_t) { some = true; });
   if (!some && slot > 0) return;
-  const Columns cols = columns_of(d, item - tile * d.column_blocks, kExpandColumns);
+  const Columns cols = columns_of(d, item - tile * d.column_blocks);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int side = RW == 4 ? 0 : wave, part = RW == 4 ? wave : 0, row = row0 + 16 * part;

@@ -12,10 +12,7 @@
 namespace {
 
 constexpr int64_t kMaxWidth = int64_t(1) << 20;
-// kernels/low_rank.hip
-constexpr int64_t kOneColumns = 1024;           // output columns of a one-launch block
-constexpr int64_t kExpandColumns = 512;         // and of an expand block
-constexpr int64_t kHeaderBytes = 256;
+constexpr int64_t kHeaderBytes = 256;  // kernels/low_rank.hip, kPartsAt
 
 int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t cut(int64_t v, int64_t by) { return (v + by - 1) / by; }
@@ -65,14 +62,25 @@ int64_t expand_rows(const lf_fp8_low_rank_desc *d) {
   return d->max_tokens <= 512 && d->rank <= 64 && int64_t(d->max_tokens) * d->rank <= 16384 ? 16 : 64;
 }
 
-int32_t column_blocks_of(const lf_fp8_low_rank_desc *d) {
+int64_t blocks_of(const lf_fp8_low_rank_desc *d, int64_t columns) {
   int64_t blocks = 0, begin = 0;
   for (int32_t i = 0; i < d->slices; ++i) {
-    blocks += cut(d->ends[i] - begin, one_launch_of(d) ? kOneColumns : kExpandColumns);
+    blocks += cut(d->ends[i] - begin, columns);
     begin = d->ends[i];
   }
-  return static_cast<int32_t>(blocks);
+  return blocks;
 }
+
+// Columns of a block: 1024 in one launch; 512 for 16 rows, 128 for each of four
+// waves; 512 or 1024 for 64 rows, where each block starts with a chain of loads: 1024
+// if that leaves 384 blocks. Columns 4096 + 2 x 1024, rank 64: 2000 rows 38 us with 512
+// and 40 with 1024, 4093 rows 56 and 52, 8192 rows 100 and 94 (112 with 2048).
+int32_t block_columns_of(const lf_fp8_low_rank_desc *d) {
+  if (one_launch_of(d)) return 1024;
+  return expand_rows(d) == 64 && cut(d->max_tokens, 64) * blocks_of(d, 1024) >= 384 ? 1024 : 512;
+}
+
+int32_t column_blocks_of(const lf_fp8_low_rank_desc *d) { return static_cast<int32_t>(blocks_of(d, block_columns_of(d))); }
 
 // Multiples of 8: XCDs have neighbouring blocks each.
 int64_t shrink_grid(const lf_fp8_low_rank_desc *d) { return align_up(shrink_blocks(d) * splits_of(d), 8); }
@@ -98,7 +106,8 @@ bool fields_ok(const lf_fp8_low_rank_desc *d) {
 
 bool desc_ok(const lf_fp8_low_rank_desc *d) {
   return d != nullptr && d->magic == LF_FP8_LOW_RANK_MAGIC && fields_ok(d) && d->splits == splits_of(d) &&
-         d->slots == slots_of(d) && d->one_launch == one_launch_of(d) && d->column_blocks == column_blocks_of(d);
+         d->slots == slots_of(d) && d->one_launch == one_launch_of(d) && d->column_blocks == column_blocks_of(d) &&
+         d->block_columns == block_columns_of(d);
 }
 
 }  // namespace
@@ -131,6 +140,7 @@ int32_t lunaflux_fp8_low_rank_descriptor(int32_t adapters, int32_t rank, int64_t
   d.slots = slots_of(&d);
   d.one_launch = one_launch_of(&d);
   d.column_blocks = column_blocks_of(&d);
+  d.block_columns = block_columns_of(&d);
   *out = d;
   return LF_OK;
 }

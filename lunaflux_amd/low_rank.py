@@ -30,7 +30,7 @@ class LowRankDescriptor(ctypes.Structure):
                 ("hidden", ctypes.c_int32), ("slices", ctypes.c_int32), ("columns", ctypes.c_int32),
                 ("max_tokens", ctypes.c_int32), ("splits", ctypes.c_int32), ("ends", ctypes.c_int32 * 4),
                 ("slots", ctypes.c_int32), ("one_launch", ctypes.c_int32),
-                ("column_blocks", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+                ("column_blocks", ctypes.c_int32), ("block_columns", ctypes.c_int32)]
 
 
 def _check(operation, status):

@@ -81,6 +81,18 @@ def test_low_rank_rows_of_adapters(rt, m, ids):
     check(got, y, *expected(x, y, a, b, scaling, which, [128, 64]), which, 7)
 
 
+@pytest.mark.parametrize("rank", [16, 48, 112])
+def test_low_rank_of_a_large_profile(rt, rank):
+    """Blocks of up to 1024 columns, the last one of a slice narrower."""
+    rng = np.random.default_rng(rank)
+    widths, n, m, most = [1600, 64], 3, 150, 384 * 64
+    assert low_rank.low_rank_descriptor(n, rank, 128, widths, most).block_columns == 1024
+    x, y, a, b, scaling = arrays(rng, m, 128, widths, rank, n)
+    ids = rng.integers(-1, n, m).astype(np.int32)
+    adapters = low_rank.LowRankAdapters.upload(rt, a, b, scaling, widths)
+    check(low_rank.low_rank(rt, x, y, ids, adapters, most), y, *expected(x, y, a, b, scaling, ids, widths), ids, n)
+
+
 def test_low_rank_of_ranks_below_a_tile(rt):
     rng = np.random.default_rng(1)
     x, y, a, b, scaling = arrays(rng, 9, 256, [64], 5, 2)

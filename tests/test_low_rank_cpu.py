@@ -30,6 +30,10 @@ def test_descriptor_and_geometry():
         d = low_rank.low_rank_descriptor(5, rank, hidden, [512, 64], rows)
         names = [g[1][len("lf_low_rank_"):] for g in (low_rank.launch_geometry(e, d) for e in entries) if g is not None]
         assert names == [n for n in (first, last) if n], (rank, hidden, rows)
+    for rows, widths, block, blocks in ((128, [1600, 64], 1024, 3), (512, [1600, 64], 512, 5), (4096, [4096, 1024, 1024], 1024, 6),
+                                        (2048, [4096, 1024, 1024], 512, 12)):
+        d = low_rank.low_rank_descriptor(4, 16, 4096, widths, rows)
+        assert (d.block_columns, d.column_blocks) == (block, blocks)
     d = low_rank.low_rank_descriptor(4, 128, 512, [512], 4096)
     geometry = [low_rank.launch_geometry(e, d) for e in entries]
     assert geometry[0] is None and [g[1] for g in geometry[1:]] == ["lf_low_rank_shrink_64x64", "lf_low_rank_expand_64x128"]
