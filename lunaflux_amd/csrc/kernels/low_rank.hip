@@ -10,8 +10,8 @@
 // 61 rows of 16 adapters, hidden 4096, rank 16, columns 4096 + 2 x 1024: 13 us in
 // one launch, of which launch and the chain of loads (ids, x and A, B, y) are nearly
 // all; the bytes, at the rate of a copy, would take 2. 4093 rows, rank 64: 25 us for x
-// A^T (8 TB/s from L2) and 32 for the rest (3.7 TB/s from and to HBM; 7 less without
-// the products), 56 together, the bytes 28. Operands loaded from memory straight into
+// A^T (8 TB/s from L2) and 27 for the rest (4 TB/s from and to HBM; 7 less without
+// the products), 52 together, the bytes 28. Operands loaded from memory straight into
 // the layout of the matrix instructions took 82 + 51.
 #include "device_common.h"
 #include "phases.h"
@@ -62,21 +62,23 @@ LF_DEVICE void for_adapters(int id, int slot, int slots, F &&f) {
 // columns = rows of x) want neighbouring lanes on different rows, which the
 // vector memory would serve lane by lane; so rows are loaded in pieces of 128
 // bytes, eight lanes each, and pass through the wave's own LDS (16-byte chunk j
-// of row r at chunk j ^ (r % 8)). AHEAD steps are in flight; LDS serves a wave's
-// accesses in their order, so no wait is needed between them.
+// of row r at chunk j ^ (r % 8)). Two steps are in flight (four cost registers: 61
+// rows of rank 32 21 us and 22.5); LDS serves a wave's accesses in their order, so
+// no wait is needed between them.
+constexpr int kAhead = 2;
 LF_DEVICE void wave_order() {  // of what the wave's lanes pass each other through LDS
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
 template <int MT, int NT>
 constexpr int kStageBytes = (MT + NT) * 2048;
-template <int MT, int NT, int AHEAD>
+template <int MT, int NT>
 LF_DEVICE void shrink_steps(f32x4 (&acc)[NT][MT], const uint8_t *x, const uint32_t (&xo)[2 * MT], const uint8_t *a,
                             int live, uint32_t row_bytes, int first, int steps, int stride, uint8_t *lds) {
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, r8 = lane >> 3, ch = lane & 7;
   struct Step {
     u32x4 x[2 * MT], a[2 * NT];
-  } s[AHEAD];
+  } s[kAhead];
   const uint32_t ao = r8 * row_bytes + 16 * ch;
   if (steps <= 0) return;
   // (the last step again behind it: a load that a branch may skip would make the
@@ -113,17 +115,17 @@ LF_DEVICE void shrink_steps(f32x4 (&acc)[NT][MT], const uint8_t *x, const uint32
     }
     wave_order();
   };
-  static_for<AHEAD>([&](auto j) { load(s[j], j); });
+  static_for<kAhead>([&](auto j) { load(s[j], j); });
   int i = 0;
-  for (; i + AHEAD <= steps; i += AHEAD) {
-    static_for<AHEAD>([&](auto j) {
+  for (; i + kAhead <= steps; i += kAhead) {
+    static_for<kAhead>([&](auto j) {
       multiply(s[j]);
       __builtin_amdgcn_sched_barrier(0);  // the loads stay behind the products
-      load(s[j], i + AHEAD + j);
+      load(s[j], i + kAhead + j);
       __builtin_amdgcn_sched_barrier(0);
     });
   }
-  static_for<AHEAD>([&](auto j) {
+  static_for<kAhead>([&](auto j) {
     if (i + j < steps) multiply(s[j]);
   });
 }
@@ -314,7 +316,7 @@ LF_DEVICE void one_launch(const int32_t *counts, const int32_t *ids, const uint8
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
       __syncthreads();  // what the stages and `low` held has been read
-      shrink_steps<1, NT, NT == 2 ? 4 : 2>(
+      shrink_steps<1, NT>(
           acc, reinterpret_cast<const uint8_t *>(x + static_cast<uint64_t>(row0) * K), xo,
           reinterpret_cast<const uint8_t *>(a + (static_cast<uint64_t>(adapter) * SR + cols.slice * R + r0) * K), live,
           2 * K, wave, steps, kOneWaves, stage[wave]);
@@ -408,7 +410,7 @@ LF_DEVICE void shrink(const int32_t *counts, const int32_t *ids, const uint8_t *
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) acc[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();  // what the stages held has been read
-    shrink_steps<MT, NT, 2>(acc, reinterpret_cast<const uint8_t *>(x + static_cast<uint64_t>(row0) * K), xo,
+    shrink_steps<MT, NT>(acc, reinterpret_cast<const uint8_t *>(x + static_cast<uint64_t>(row0) * K), xo,
                             reinterpret_cast<const uint8_t *>(a + (static_cast<uint64_t>(adapter) * SR + col0) * K),
                             live, 2 * K, first, steps, kShrinkWaves, stage[wave]);
     static_assert(NT * MT * 1024 <= kStageBytes<MT, NT>, "a wave's sums fit its stage");
