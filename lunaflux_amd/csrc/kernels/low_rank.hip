@@ -430,12 +430,13 @@ LF_DEVICE void shrink(const int32_t *counts, const int32_t *ids, const uint8_t *
   });
 }
 
-// y + s v B^T, v from the workspace, for 16 RW rows and a block's columns of a slice; RANKS = the rank, up to a power of two. RW 4: four waves of 16 rows each
-// go through the columns together, with one copy of B in LDS; RW 1: each wave has
-// 128 columns of the same 16 rows. The next columns' B and y are loaded while
-// these are multiplied; B first, so that the wait for it leaves y in flight, and it
-// goes to LDS before the results are stored, so that no wait for a load is one for
-// a store behind it.
+// y + s v B^T, v from the workspace, for 16 RW rows and a block's columns of a
+// slice; RANKS = the rank, up to a power of two. RW 4: four waves of 16 rows each go
+// through the columns together, with one copy of B in LDS; RW 1: each wave has 128
+// columns of the same 16 rows. The next columns' B and y are loaded while these are
+// multiplied; B first, so that the wait for it leaves y in flight, and it goes to
+// LDS before the results are stored, so that no wait for a load is one for a store
+// behind it.
 template <int RW, int RANKS>
 LF_DEVICE void expand(const int32_t *counts, const int32_t *ids, const uint8_t *desc, const float *scaling,
                       const uint16_t *b, const uint16_t *y, uint16_t *out, uint8_t *ws) {

@@ -172,7 +172,11 @@ int32_t lunaflux_fp8_low_rank_launch_geometry(int32_t entry, const lf_fp8_low_ra
                   d->rank <= 32 ? 32 : d->rank <= 64 ? 64 : 128);
     gx = expand_grid(d);
   }
-  if (!d->one_launch) gy = d->slots;
+  // (the second launch's blocks come to a tile's adapters sooner: 400 rows of 16
+  // adapters 55 us with eight slots there, 50 with four or two; 1600 rows of 5 in
+  // runs of 100 44 with five or four, 45 with two, 48 with one)
+  if (entry == LF_FP8_LOW_RANK_SHRINK) gy = d->slots;
+  if (entry == LF_FP8_LOW_RANK_EXPAND) gy = std::min(d->slots, 4);
   dims[0] = static_cast<int32_t>(gx);
   dims[1] = static_cast<int32_t>(gy);
   dims[2] = 1;

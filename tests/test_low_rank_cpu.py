@@ -34,6 +34,10 @@ def test_descriptor_and_geometry():
                                         (2048, [4096, 1024, 1024], 512, 12)):
         d = low_rank.low_rank_descriptor(4, 16, 4096, widths, rows)
         assert (d.block_columns, d.column_blocks) == (block, blocks)
+    d = low_rank.low_rank_descriptor(16, 16, 4096, [512], 300)  # 5 tiles of 64 rows, 19 of 16
+    assert d.slots == 8 and d.splits == 2
+    assert low_rank.launch_geometry(_abi.LOW_RANK_SHRINK, d)[0].grid == (16, 8, 1)
+    assert low_rank.launch_geometry(_abi.LOW_RANK_EXPAND, d)[0].grid == (24, 4, 1)
     d = low_rank.low_rank_descriptor(4, 128, 512, [512], 4096)
     geometry = [low_rank.launch_geometry(e, d) for e in entries]
     assert geometry[0] is None and [g[1] for g in geometry[1:]] == ["lf_low_rank_shrink_64x64", "lf_low_rank_expand_64x128"]
