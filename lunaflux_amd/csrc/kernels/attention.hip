@@ -187,16 +187,16 @@ LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, con
 // ---- attention of one new token per sequence -------------------------------
 
 // The step's work is cut into tiles of 32 keys, (sequence, head tile, key tile)
-// with key tiles innermost, and the tiles into equal ranges, one per block,
-// whose four waves take a pair's tiles in turn and join through LDS. A pair
-// (sequence, head tile) that one block holds whole is finished there. Other
-// blocks leave a partial result (fp32 sums, maximum and weight sum of each of
-// the tile's rows) in the workspace; of every kGroup neighbours the last to
-// arrive adds the group's up in order, and the last group to arrive the
-// groups'. HBM bounds it (5.8 TB/s of 131071 keys); a launch with nothing to read
-// takes 5 us, the join 3 to 6, and the XCDs' rates differ by a tenth while their
-// shares are equal. Partial results are stored and loaded at agent scope (past the XCD's
-// L2), and a block counts itself only once its stores have completed.
+// with key tiles innermost, and the tiles into equal ranges, one per block (by whole
+// pairs (sequence, head tile) if all are short); a block's four waves take a pair's
+// tiles in turn and join through LDS. A pair that one block holds whole is finished
+// there. Other blocks leave a partial result (fp32 sums, maximum and weight sum of
+// each of the tile's rows) in the workspace; of every kGroup neighbours the last to
+// arrive adds the group's up in order, and the last group to arrive the groups'.
+// HBM bounds it (5.8 TB/s of 131071 keys); a launch with nothing to read takes 5 us,
+// the join 3 to 6, and the XCDs' rates differ by a tenth while their shares are
+// equal. Partial results are stored and loaded at agent scope (past the XCD's L2),
+// and a block counts itself only once its stores have completed.
 constexpr int kWaves = 4;
 
 // Blocks of the grid: one per CU, two where a key is 128 bytes or less and one
@@ -442,7 +442,7 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
                       const int32_t *page_offsets, const int32_t *page_indices, const uint8_t *attn,
                       const uint16_t *q, uint16_t *out, const uint8_t *kc, const uint8_t *vc, uint8_t *ws) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ int wave_total[kWaves];
+  __shared__ int wave_total[kWaves], wave_long[kWaves];
   __shared__ int arrived;
   __shared__ float stats[2][kGroup][kHeadTile];
   __shared__ Sequence near[64 * kWaves];
@@ -463,7 +463,8 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   };
 
   int *prefix = reinterpret_cast<int *>(lds);
-  bool bad = false;
+  const int most_tiles = whole_tiles(n * head_tiles_of(d));
+  bool bad = false, longer = false;
   int64_t carry = 0;
   for (int base = 0; base < n; base += 256) {
     const int i = base + static_cast<int>(threadIdx.x);
@@ -473,6 +474,7 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       tiles = q1.span.tiles;
       if (base == 0) near[i] = q1;
     }
+    longer |= tiles > most_tiles;
     int sum = tiles;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -490,6 +492,8 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     __syncthreads();
   }
   if (threadIdx.x == 0) prefix[n] = static_cast<int>(carry);
+  const bool some_longer = __ballot(longer) != 0;
+  if (lane == 0) wave_long[wave] = some_longer ? 1 : 0;
   __syncthreads();
 
   const int Hq = d.query_heads, Hkv = d.kv_heads, group = Hq / Hkv;
@@ -513,10 +517,26 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   const int g = lane >> 4, c = lane & 15;
 
   const int block = blockIdx.x;
-  const int64_t begin64 = static_cast<int64_t>(block) * share;
-  if (begin64 >= items) return;
-  int u = static_cast<int>(begin64);
-  const int end = items - u < share ? items : u + share;
+  const bool by_pair = __builtin_amdgcn_readfirstlane(wave_long[0] | wave_long[1] | wave_long[2] | wave_long[3]) == 0;
+  int u, end;
+  if (by_pair) {
+    int tiles = 0;  // of the pair whose first item it gives
+    auto start = [&](int pair) {
+      const int i = pair / head_tiles, before = prefix[i];
+      tiles = __builtin_amdgcn_readfirstlane(prefix[i + 1] - before);
+      return __builtin_amdgcn_readfirstlane(before) * head_tiles + (pair - i * head_tiles) * tiles;
+    };
+    const PairRange mine = pairs_of(block, n * head_tiles, blocks<D, E4M3>());
+    if (items == 0 || mine.first >= mine.end) return;
+    u = start(mine.first);
+    end = u + tiles;
+    if (mine.end - mine.first > 1) end = start(mine.end - 1) + tiles;
+  } else {
+    const int64_t begin64 = static_cast<int64_t>(block) * share;
+    if (begin64 >= items) return;
+    u = static_cast<int>(begin64);
+    end = items - u < share ? items : u + share;
+  }
 
   // the next part of a pair in the block's range
   auto take = [&](Piece &x) {
@@ -736,7 +756,7 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     }
     __syncthreads();
     const Parts parts = parts_of(now.pair, now.tiles, share);
-    const bool whole = parts.first == parts.last;
+    const bool whole = by_pair || parts.first == parts.last;
     const float vscale = E4M3 ? scales[Hkv + now.h] : 1.0f;
     const int live = now.live;
     uint16_t *dst = out + (static_cast<uint64_t>(now.row < 0 ? 0 : now.row) * Hq + now.h * group + now.row0) * D;

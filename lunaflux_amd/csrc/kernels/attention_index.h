@@ -123,6 +123,21 @@ LF_DEVICE int share_of(int items, int pairs, int blocks) {
   return share > least ? share : least;
 }
 
+// A step whose pairs all are short is dealt out by pairs instead: block b holds the
+// pairs [first, end), and none is cut. Heads of 128, 8 key heads, us by items and by
+// pairs: 15 sequences of up to 179 keys 19.3 and 9.0, 64 of up to 300 27.7 and 19.8,
+// 16 of up to 1000 23.8 and 19.0, 128 of up to 1000 88 and 84; one of 1000 13.0 and
+// 16.9, so few pairs have to be shorter; steps of one tile per pair 0.5 slower.
+LF_DEVICE int whole_tiles(int pairs) { return pairs < 32 ? 16 : 32; }
+struct PairRange {
+  int first, end;
+};
+LF_DEVICE PairRange pairs_of(int block, int pairs, int blocks) {
+  if (pairs <= blocks) return {block, block < pairs ? block + 1 : block};
+  return {static_cast<int>(static_cast<int64_t>(block) * pairs / blocks),
+          static_cast<int>(static_cast<int64_t>(block + 1) * pairs / blocks)};
+}
+
 // The sequence that item u belongs to (prefix rises by at least 1 a sequence).
 LF_DEVICE int sequence_at(const int *prefix, int n, int head_tiles, int u) {
   int i = 0;

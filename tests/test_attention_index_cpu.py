@@ -47,6 +47,20 @@ static int64_t elements(const Desc &d) {
          d.head_dim;
 }
 
+// by pairs: every pair once, in order, in no more blocks than there are
+static void by_pairs() {
+  const int blocks = pick(0, 1) ? 256 : 512, pairs = pick(0, 3) ? pick(0, 3000) : 2048 * 1024 - pick(0, 3);
+  int next = 0;
+  for (int b = 0; b < blocks; ++b) {
+    const PairRange r = pairs_of(b, pairs, blocks);
+    if (r.first >= r.end) continue;
+    CHECK(r.first == next && r.end <= pairs);
+    CHECK(r.end - r.first <= (pairs + blocks - 1) / blocks);
+    next = r.end;
+  }
+  CHECK(next == pairs);
+}
+
 static void hostile() {
   const Desc d = desc();
   auto garbage = [&](size_t n) {
@@ -149,7 +163,8 @@ static void cut(int workers) {  // ranges
 }
 
 int main() {
-  for (int i = 0; i < 300; ++i) hostile();
+  for (int i = 0; i < 300; ++i) by_pairs();
+    hostile();
   const int workers[] = {1, 2, 7, 256, 1024, 2048};
   for (int i = 0; i < 600; ++i) cut(workers[i % 6]);
   std::printf("ok\n");

@@ -188,6 +188,21 @@ def test_decode_strides(rt, strides, cache):
     check_decode(s, read_out(s, run_decode(rt, s, q)[1]), q, lengths)
 
 
+@pytest.mark.parametrize("longest", [20, 512, 513, 1024, 1025])
+@pytest.mark.parametrize("sequences,hq,hkv", [(3, 4, 2), (20, 2, 2), (150, 16, 4)])
+def test_decode_by_pairs_or_by_tiles(rt, longest, sequences, hq, hkv):
+    """One sequence of `longest` keys among short ones, on both sides of the
+    lengths up to which blocks take whole (sequence, head) pairs."""
+    rng = np.random.default_rng(longest + sequences)
+    lengths = [int(x) for x in rng.integers(1, 40, sequences)]
+    lengths[sequences // 2] = longest
+    s = build(rt, rng, lengths=lengths, query_heads=hq, kv_heads=hkv, page=16)
+    q = queries(rng, s)
+    op, oa = run_decode(rt, s, q)
+    check_decode(s, read_out(s, oa), q, lengths)
+    op.check()
+
+
 def test_decode_of_many_sequences(rt):
     """More pairs than blocks: blocks hold whole pairs and ends of others."""
     rng = np.random.default_rng(9)
