@@ -545,7 +545,7 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
  * of [max(0, length - window), length) (window 0: all), p = softmax of
  * softmax_scale q.k_j. Query head h reads key head h / (Hq / Hkv). The scores
  * and the softmax statistics are fp32; the weights p go to the second product
- * as bf16 and are summed as what they were rounded to. A row without keys (or
+ * as two bf16 terms (all but 2^-15 of them). A row without keys (or
  * all of whose scores are -inf) gives zeros; values at keys that do not count
  * are not read into the sum, whatever they hold. Other rows of out stay as
  * they were.
