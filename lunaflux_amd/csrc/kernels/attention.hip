@@ -390,8 +390,7 @@ LF_DEVICE Groups groups_of(int page, int pages, uint32_t page_bytes, uint32_t to
   auto at = [&](int p, int k) {
     const bool ok = static_cast<uint32_t>(p) < static_cast<uint32_t>(pages);
     in |= ok ? 1 << k : 0;
-    return static_cast<uint64_t>(static_cast<uint32_t>(ok ? p : 0)) * page_bytes +
-           static_cast<uint64_t>(static_cast<uint32_t>((base + 8 * k) & slot_mask)) * token_bytes;
+    return row_byte(ok ? p : 0, (base + 8 * k) & slot_mask, page_bytes, token_bytes);
   };
   const uint64_t a = at(__builtin_amdgcn_readlane(page, 0), 0), b = at(__builtin_amdgcn_readlane(page, 1), 1);
   const uint64_t c = at(__builtin_amdgcn_readlane(page, 2), 2), d = at(__builtin_amdgcn_readlane(page, 3), 3);
@@ -587,13 +586,11 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   auto tile_groups = [&](int page, int base) {
     return groups_of(page, pages, page_bytes, token_bytes, slot_mask, base);
   };
-  // this lane's part of a head's rows: of keys, row c % 8 of a group of eight,
-  // chunk g; of values, row 4 g of a half
-  const uint32_t key_lane = (c & 7) * token_bytes + 16 * g;
-  const uint32_t value_lane = (4 * g & 7) * token_bytes + c * (D / 16 * kSize);
+  // this lane's part of a head's rows
+  const uint64_t key_at = key_lane(c, g, token_bytes), value_at = value_lane(c, g, token_bytes, D / 16 * kSize);
   const uint32_t head_bytes = static_cast<uint32_t>(d.head_stride) * kSize;
-  auto keys_of = [&](uint32_t h) { return kc + static_cast<uint64_t>(h) * head_bytes + key_lane; };
-  auto values_of = [&](uint32_t h) { return vc + static_cast<uint64_t>(h) * head_bytes + value_lane; };
+  auto keys_of = [&](uint32_t h) { return kc + static_cast<uint64_t>(h) * head_bytes + key_at; };
+  auto values_of = [&](uint32_t h) { return vc + static_cast<uint64_t>(h) * head_bytes + value_at; };
   // B operand of the first product: query head c, the values of its key chunk
   bf16x8 qv[D / 32];
   auto load_queries = [&](const Piece &x) {

@@ -93,6 +93,21 @@ LF_DEVICE int entry_of(int first, int end, int shift, int j) {
   return e < first ? first : e < end ? e : end - 1;
 }
 
+// Bytes, all in 64 bits (a page's or a token's step may be up to 2^31 - 1 of them):
+// of slot `slot` of a page from the head's first row, and from the first of a group
+// of eight rows of lane 16 g + c's part of them, which is row c % 8, 16-byte chunk g,
+// of keys, and row 4 g % 8, the c-th of 16 pieces of `piece` bytes, of values.
+LF_DEVICE uint64_t row_byte(int page, int slot, uint32_t page_bytes, uint32_t token_bytes) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_bytes +
+         static_cast<uint64_t>(static_cast<uint32_t>(slot)) * token_bytes;
+}
+LF_DEVICE uint64_t key_lane(int c, int g, uint32_t token_bytes) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(c & 7)) * token_bytes + static_cast<uint32_t>(16 * g);
+}
+LF_DEVICE uint64_t value_lane(int c, int g, uint32_t token_bytes, int piece) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(4 * g & 7)) * token_bytes + static_cast<uint32_t>(c * piece);
+}
+
 LF_DEVICE int head_tiles_of(const Desc &d) {
   const int group = d.query_heads / d.kv_heads;
   return d.kv_heads * ((group + kHeadTile - 1) / kHeadTile);
