@@ -506,7 +506,9 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   const int Hq = d.query_heads, Hkv = d.kv_heads, group = Hq / Hkv;
   const int group_tiles = (group + kHeadTile - 1) / kHeadTile;
   const int head_tiles = head_tiles_of(d);
-  // (page ranges that overlap may add up to more than the descriptor's bound)
+  // (page ranges that overlap may add up to more than the descriptor's bound; a wave's
+  // own sums fit 31 bits, since at most every other range of a list of offsets can
+  // rise past another: 32 of 2^26 - 32 tiles and 32 of one)
   const bool counted = carry * head_tiles <= kMostItems;
   if (!counted) bad = true;
   const int items = __builtin_amdgcn_readfirstlane(counted ? static_cast<int>(carry) * head_tiles : 0);

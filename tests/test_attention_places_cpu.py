@@ -66,3 +66,58 @@ int main() {
 
 def test_lanes_of_long_strides(tmp_path):
     run(tmp_path, LANES)
+
+
+OVERLAPS = r"""
+// The tiles of 64 consecutive sequences, whatever the page offsets, stay in the 31 bits
+// that a wave adds them up in: a range that overlaps one before it comes after a range
+// that falls, which has no pages and one tile.
+static void offsets(const Desc &d, const std::vector<int> &ends) {
+  int64_t sum = 0;
+  for (size_t s = 0; s + 1 < ends.size(); ++s) {
+    bool bad = false;
+    const Pages p = pages_of(d, ends[s], ends[s + 1], bad);
+    if (bad) CHECK(p.count == 0);
+    const Span span = span_of(d, INT32_MAX, p, bad);
+    CHECK(span.tiles >= 1 && span.tiles <= (1 << 26) - 32);
+    sum += span.tiles;
+    if ((s + 1) % 64 == 0) {
+      CHECK(sum <= INT32_MAX);
+      sum = 0;
+    }
+  }
+}
+int main() {
+  for (int page : {8, 32, 1024}) {
+    Desc d{};
+    d.page_size = page;
+    d.table_entries = (INT32_MAX - 1024) / page;
+    std::vector<int> ends(2049);
+    for (int phase = 0; phase < 2; ++phase) {
+      for (size_t i = 0; i < ends.size(); ++i) ends[i] = i % 2 == static_cast<size_t>(phase) ? 0 : d.table_entries;
+      offsets(d, ends);
+    }
+    for (int i = 0; i < 500; ++i) {
+      for (auto &e : ends) e = pick(0, 3) ? pick(0, 1) * d.table_entries : pick(-2, d.table_entries);
+      offsets(d, ends);
+    }
+  }
+  std::printf("ok\n");
+}
+"""
+
+
+def test_a_wave_of_overlapping_page_ranges_fits_31_bits(tmp_path):
+    run(tmp_path, OVERLAPS)
+
+
+def test_steps_of_garbage_on_many_descriptors(tmp_path):
+    """hostile() on a descriptor of its own each time, and the cut for both grids of
+    the decode kernels (256 and 512 blocks)."""
+    run(tmp_path, r"""
+int main() {
+  for (int i = 0; i < 400; ++i) hostile();
+  for (int i = 0; i < 400; ++i) cut(i % 2 ? 256 : 512);
+  std::printf("ok\n");
+}
+""")

@@ -1,4 +1,5 @@
-"""Decode attention and the append over caches whose token stride is long."""
+"""Decode attention and the append over caches whose token stride is long, and
+steps whose page ranges overlap."""
 import math
 
 import numpy as np
@@ -6,6 +7,7 @@ import pytest
 
 import attention_oracle as ao
 from lunaflux_amd import attention, fp8, synth
+from lunaflux_amd.device import DeviceError
 from test_gpu_attention import region
 
 pytestmark = pytest.mark.gpu
@@ -64,3 +66,27 @@ def test_tokens_a_gigabyte_apart(rt, cache):
         assert (np.abs(x[length - 1] - np.clip(steps, -448, 448)) <= limit).all()
     decode.launch(rt.stream)
     check()
+
+
+@pytest.mark.parametrize("sequences", [63, 64, 300])
+def test_overlapping_page_ranges_past_the_items_are_reported(rt, sequences):
+    """Every other sequence claims the whole of a table of 2^31 keys, 2^26 tiles each:
+    nothing is written, and the launch says so."""
+    entries, dim = (1 << 21) - 2, 64
+    layer = attention.attention_layer(rt, query_heads=1, kv_heads=1, head_dim=dim, page_size=1024, pages=2,
+                                      max_tokens=sequences, max_sequences=sequences, table_entries=entries)
+    step = attention.PagedStep(rt, layer)
+    step.page_indices.copy_from_host(np.zeros(entries, np.int32))
+    step.stage(np.arange(sequences + 1), [1] * sequences, [[0]] * sequences)
+    caches = [rt.context.upload(np.zeros(layer.cache_bytes, np.uint8)) for _ in range(2)]
+    q = rt.context.upload(np.zeros(sequences * dim, np.uint16))
+    out = rt.context.upload(np.full(sequences * dim, 0x7FA5, np.uint16))
+    op = attention.bind_paged_decode(rt, layer, step, region(q), region(out), *map(region, caches))
+    step.lengths.copy_from_host(np.full(sequences, entries * 1024, np.int32))
+    ends = np.zeros(sequences + 1, np.int32)
+    ends[1::2] = entries
+    step.page_offsets.copy_from_host(ends)
+    with pytest.raises(DeviceError):
+        op.launch(rt.stream)
+    op.check()
+    assert (out.read(np.uint16, (sequences * dim,)) == 0x7FA5).all()
