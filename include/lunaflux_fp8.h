@@ -601,7 +601,9 @@ typedef struct lf_fp8_attn_desc {
 /* Checks the fields of *desc, and writes its magic, default strides and the
  * region offsets. LF_INVALID_ARGUMENT for values outside the ranges above,
  * strides that overlap or are not multiples of 16 bytes, or bounds past 32
- * bits (table_entries * page_size, the 32-key tiles of a step times heads). */
+ * bits (table_entries * page_size, the 32-key tiles of a step times heads).
+ * The functions below take a descriptor as this one left it: one whose region
+ * offsets do not follow from its fields is refused. */
 int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *desc);
 /* Writes the descriptor region (desc->region_bytes bytes). scales: 2 kv_heads
  * values, finite and above zero (null for a bf16 cache: ones); turns and axis:

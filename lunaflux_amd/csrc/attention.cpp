@@ -80,8 +80,23 @@ bool fields_ok(const lf_fp8_attn_desc *d) {
   return true;
 }
 
+// The region's parts behind the descriptor.
+void lay_out(lf_fp8_attn_desc *d) {
+  d->scale_offset = LF_FP8_ATTN_DESC_BYTES;
+  d->turns_offset = d->scale_offset + align_up(int64_t(2) * d->kv_heads * 4, 256);
+  d->axis_offset = d->turns_offset + align_up(int64_t(d->rotary_dim) / 2 * 8, 256);
+  d->region_bytes = d->axis_offset + align_up(int64_t(d->rotary_dim) / 2 * 4, 256);
+}
+
+bool laid_out(const lf_fp8_attn_desc *d) {
+  lf_fp8_attn_desc r = *d;
+  lay_out(&r);
+  return d->scale_offset == r.scale_offset && d->turns_offset == r.turns_offset && d->axis_offset == r.axis_offset &&
+         d->region_bytes == r.region_bytes;
+}
+
 bool desc_ok(const lf_fp8_attn_desc *d) {
-  return d != nullptr && d->magic == LF_FP8_ATTN_MAGIC && fields_ok(d) && strides_ok(d);
+  return d != nullptr && d->magic == LF_FP8_ATTN_MAGIC && fields_ok(d) && strides_ok(d) && laid_out(d);
 }
 
 int64_t tile_rows(const lf_fp8_attn_desc *d) {
@@ -117,10 +132,7 @@ int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *d) {
     r.head_stride = int64_t(r.page_size) * r.head_dim;
     r.page_stride = r.kv_heads * r.head_stride;
   }
-  r.scale_offset = LF_FP8_ATTN_DESC_BYTES;
-  r.turns_offset = r.scale_offset + align_up(int64_t(2) * r.kv_heads * 4, 256);
-  r.axis_offset = r.turns_offset + align_up(int64_t(r.rotary_dim) / 2 * 8, 256);
-  r.region_bytes = r.axis_offset + align_up(int64_t(r.rotary_dim) / 2 * 4, 256);
+  lay_out(&r);
   if (!strides_ok(&r)) return LF_INVALID_ARGUMENT;
   *d = r;
   return LF_OK;
