@@ -66,9 +66,13 @@ class Rotary:
     axes: int = 0  # positions of a row; 0: as many as `axis` names
 
     def __post_init__(self):
-        turns, axis = np.asarray(self.turns, np.float64), np.asarray(self.axis, np.int32)
-        if turns.ndim != 1 or axis.shape != turns.shape or self.pairing not in PAIRINGS:
+        turns, given = np.asarray(self.turns, np.float64), np.asarray(self.axis)
+        if turns.ndim != 1 or given.shape != turns.shape or self.pairing not in PAIRINGS:
             raise _invalid("rotary pairs")
+        if given.dtype.kind not in "iuf" or not (np.abs(given.astype(np.float64)) < 2 ** 31).all() or \
+                (given != given.astype(np.int32)).any():
+            raise _invalid("axes of rotary pairs are whole numbers")
+        axis = given.astype(np.int32)
         object.__setattr__(self, "turns", turns)
         object.__setattr__(self, "axis", axis)
         if self.axes == 0:
@@ -124,10 +128,17 @@ def attention_descriptor(*, query_heads: int, kv_heads: int, head_dim: int, page
                 raise _invalid(name)
         d.rotary_dim = 0 if rotary is None else 2 * len(rotary.turns)
         d.axes = 1 if rotary is None else rotary.axes
+        if rotary is not None and d.axes != rotary.axes:
+            raise _invalid("axes")
         d.pairing = PAIRINGS["half" if rotary is None else rotary.pairing]
         d.norm, d.norm_epsilon = (0, 0.0) if norm_epsilon is None else (1, norm_epsilon)
         d.softmax_scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None and head_dim > 0 else softmax_scale or 0.0
-        d.page_stride, d.head_stride, d.token_stride = (0, 0, 0) if strides is None else strides
+        steps = (0, 0, 0) if strides is None else tuple(strides)
+        if len(steps) != 3:
+            raise _invalid("strides")
+        d.page_stride, d.head_stride, d.token_stride = steps
+        if (d.page_stride, d.head_stride, d.token_stride) != steps:
+            raise _invalid("strides")
     except TypeError as e:
         raise _invalid(str(e)) from None
     _check("attention_descriptor", _abi.lib().lunaflux_fp8_attn_descriptor(ctypes.byref(d)))
