@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from dataclasses import dataclass
 
 import numpy as np
@@ -189,6 +190,33 @@ def launch_geometry(entry: int, desc: AttentionDescriptor):
             symbol.value.decode("ascii"))
 
 
+def _page_table(table) -> np.ndarray:
+    if isinstance(table, list):
+        try:
+            return np.asarray(array("i", table))  # C ints from Python's, the quickest way that changes none
+        except (TypeError, OverflowError):
+            pass
+    return np.asarray(table).reshape(-1)
+
+
+def _page_tables(page_tables) -> tuple:
+    """The number of entries of every sequence's table, and all of them in turn as int32."""
+    tables = [_page_table(t) for t in page_tables]
+    counts = np.array([t.size for t in tables], np.int64)
+    held = [t for t in tables if t.size] or [np.zeros(0, np.int32)]
+    kinds = {t.dtype for t in held}
+    if any(k.kind not in "iu" for k in kinds):
+        raise _invalid("page indices are whole numbers")
+    if len(kinds) > 1:  # types that differ may become a float one, or wrap
+        held = [t.astype(np.int64) if t.dtype != np.uint64 or t.max() < 2 ** 31 else np.array([2 ** 31]) for t in held]
+    indices = np.concatenate(held)
+    if indices.dtype != np.int32:
+        if indices.min() < -2 ** 31 or indices.max() >= 2 ** 31:
+            raise _invalid("page indices are of 32 bits")
+        indices = indices.astype(np.int32)
+    return counts, indices
+
+
 class PagedStep:
     """The runtime inputs of a paged step, in regions sized for the layer's
     descriptor (max_tokens rows, max_sequences, table_entries); every layer of
@@ -231,8 +259,7 @@ class PagedStep:
             raise _invalid("a decoded sequence has one row")
         if (lengths < rows).any():
             raise _invalid("lengths of a step")
-        tables = [np.asarray(t, np.int32).reshape(-1) for t in page_tables]
-        counts = np.array([t.size for t in tables], np.int64)
+        counts, indices = _page_tables(page_tables)
         if (counts * self.page_size < lengths).any() or counts.sum() > self.table_entries:
             raise _invalid("page tables of a step")
         m = int(row_offsets[-1])
@@ -245,13 +272,12 @@ class PagedStep:
                 raise _invalid("positions of a step")
         if lengths.size and lengths.max() >= 2 ** 31:
             raise _invalid("lengths of a step")
-        entries = int(counts.sum())
-        self.counts.copy_from_host(np.array([prefill_rows, n - prefill_rows, n, m, entries], np.int32))
+        self.counts.copy_from_host(np.array([prefill_rows, n - prefill_rows, n, m, indices.size], np.int32))
         self.row_offsets.copy_from_host(row_offsets.astype(np.int32))
         self.lengths.copy_from_host(lengths.astype(np.int32))
         self.page_offsets.copy_from_host(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
-        if entries:
-            self.page_indices.copy_from_host(np.concatenate(tables))
+        if indices.size:
+            self.page_indices.copy_from_host(indices)
         if positions is not None:
             self.positions.copy_from_host(positions.astype(np.int32))
 

@@ -5,7 +5,7 @@ import pytest
 
 from lunaflux_amd import _abi, attention
 from lunaflux_amd.device import DeviceError
-from test_attention_cpu import make
+from test_attention_cpu import bound, make
 
 
 @pytest.mark.parametrize("strides", [
@@ -29,3 +29,28 @@ def test_axes(axes):
 def test_axis_of_a_pair(axis):
     with pytest.raises(DeviceError):
         attention.Rotary(np.ones(8), axis)
+
+
+@pytest.mark.parametrize("table", [
+    [0.5], np.array([1.0]), np.array([(1 << 32) + 3]), np.array([-(1 << 32)]), np.array([1 << 63], np.uint64), [1 << 31],
+    [1 << 80], ["1"], np.array([True]), [None],
+])
+def test_page_tables_of_a_step(table):
+    """Page indices are whole numbers of 32 bits: others would name pages that nobody meant."""
+    _, _, step = bound()
+    before = [a.data.copy() for a in (step.counts, step.lengths, step.page_offsets, step.page_indices)]
+    with pytest.raises(DeviceError) as e:
+        step.stage([0, 1], [1], [table])
+    assert e.value.status == _abi.LF_INVALID_ARGUMENT
+    for a, b in zip((step.counts, step.lengths, step.page_offsets, step.page_indices), before):
+        np.testing.assert_array_equal(a.data, b)
+
+
+def test_page_tables_that_are_taken():
+    """Any integer type, an empty list, and indices outside the cache, which the device reports."""
+    _, _, step = bound()
+    step.stage([0, 1, 2, 2], [1, 17, 0], [np.array([[-1]], np.int64), np.array([2 ** 31 - 1, 3], np.uint64), []], prefill_rows=3)
+    assert step.page_indices.data[:12].view(np.int32).tolist() == [-1, 2 ** 31 - 1, 3]
+    for kind in (np.int32, np.int64, np.uint16):
+        step.stage([0, 1, 2], [3, 18], [np.array([4], kind), np.array([2, 0], kind)])
+        assert step.page_indices.data[:12].view(np.int32).tolist() == [4, 2, 0]
