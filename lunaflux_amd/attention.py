@@ -30,6 +30,7 @@ from .fp8 import COUNTS_BYTES, BoundOperation, LaunchStep, ProjectionRuntime, _r
 CACHES = {"bf16": _abi.LF_FP8_CACHE_BF16, "e4m3": _abi.LF_FP8_CACHE_E4M3}
 PAIRINGS = {"half": _abi.LF_FP8_PAIR_HALF, "neighbour": _abi.LF_FP8_PAIR_NEIGHBOUR}
 MAX_SEQUENCES = _abi.LF_FP8_ATTN_MAX_SEQUENCES
+AS_THEY_ARE = object()  # PagedStep.stage: the positions that the region holds
 
 
 class AttentionDescriptor(ctypes.Structure):
@@ -226,6 +227,7 @@ class PagedStep:
         d = layer.desc
         self.max_tokens, self.max_sequences, self.table_entries = d.max_tokens, d.max_sequences, d.table_entries
         self.axes, self.page_size = d.axes, d.page_size
+        self.positioned = True  # the step's rows have positions
         allocate = rt.context.allocate
         self.counts = allocate(COUNTS_BYTES)
         self.positions = allocate(4 * d.max_tokens * d.axes)
@@ -239,8 +241,10 @@ class PagedStep:
         """Writes a step's inputs. Sequence s has rows row_offsets[s] ..
         row_offsets[s + 1] - 1 and, with them, lengths[s] tokens in the pages
         page_tables[s]; the first prefill_rows sequences are not decoded.
-        positions [rows, axes] (or [rows] for one axis); None leaves what the
-        region holds. DeviceError INVALID_ARGUMENT, with nothing written, for a
+        positions [rows, axes] (or [rows] for one axis); None: the rows have
+        none, and appends of layers that rotate refuse to launch; AS_THEY_ARE:
+        those that the caller wrote to `positions`, or left there by the step
+        before. DeviceError INVALID_ARGUMENT, with nothing written, for a
         step that does not fit or contradicts itself (page indices are the
         cache owner's, and checked on the device). Launches that read the step
         before have to be over: the caller synchronizes their streams first."""
@@ -263,7 +267,8 @@ class PagedStep:
         if (counts * self.page_size < lengths).any() or counts.sum() > self.table_entries:
             raise _invalid("page tables of a step")
         m = int(row_offsets[-1])
-        if positions is not None:
+        written = positions is not None and positions is not AS_THEY_ARE
+        if written:
             positions = np.asarray(positions)
             if positions.dtype.kind not in "iu" or positions.size != m * self.axes or \
                     positions.shape not in ((m,), (m, self.axes)):
@@ -278,15 +283,25 @@ class PagedStep:
         self.page_offsets.copy_from_host(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
         if indices.size:
             self.page_indices.copy_from_host(indices)
-        if positions is not None:
+        if written:
             self.positions.copy_from_host(positions.astype(np.int32))
+        self.positioned = positions is not None or m == 0
 
 
 @dataclass
 class BoundAttention(BoundOperation):
     """check(): DeviceError(INVALID_ARGUMENT) if a launch met offsets, lengths
     or page indices outside the layer's bounds (the rows and keys concerned
-    were left out); the error word is cleared."""
+    were left out); the error word is cleared.
+
+    rotates: the step whose positions the operation turns by, or None."""
+
+    rotates: PagedStep | None = None
+
+    def launch(self, stream, synchronous: bool = True):
+        if self.rotates is not None and not self.rotates.positioned:
+            raise _invalid("rows of the step have no positions to be rotated by")
+        super().launch(stream, synchronous)
 
     def check(self):
         if self.workspace.read(np.int32, (1,))[0] != 0:
@@ -349,7 +364,7 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
             _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4), layer.region, qkv,
             unused if gq is None else gq, unused if gk is None else gk, q, k_cache, v_cache, _region(ws, alignment=256)]
     return BoundAttention([LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)], workspace=ws,
-                          keep=[layer, step])
+                          keep=[layer, step], rotates=step if d.rotary_dim else None)
 
 
 def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedStep, q: KernelArgument,

@@ -1,11 +1,13 @@
 """Arguments of the attention's host side that no 32- or 64-bit field holds as
 they are, page tables among them: refused, not cut."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
 from lunaflux_amd import _abi, attention
 from lunaflux_amd.device import DeviceError
-from test_attention_cpu import bound, make
+from test_attention_cpu import bound, make, region
 
 
 @pytest.mark.parametrize("strides", [
@@ -44,6 +46,47 @@ def test_page_tables_of_a_step(table):
     assert e.value.status == _abi.LF_INVALID_ARGUMENT
     for a, b in zip((step.counts, step.lengths, step.page_offsets, step.page_indices), before):
         np.testing.assert_array_equal(a.data, b)
+
+
+def rotary_append(rotary):
+    rt, layer, step = bound(rotary=rotary)
+    qkv, q, cache = region(2 * 32 * 12 * 128), region(2 * 32 * 8 * 128), layer.cache_bytes
+    op = attention.bind_qk_norm_rope(rt, layer, step, qkv, None, None, q, region(cache), region(cache))
+    launched = []
+    op.steps = [SimpleNamespace(launch=lambda stream, synchronous: launched.append(stream))]
+    return step, op, launched
+
+
+def test_rows_without_positions_are_not_rotated():
+    """A step that was staged without positions does not turn by those of the one before."""
+    step, op, launched = rotary_append(attention.Rotary.of_theta(1e4, 64))
+    launch = lambda: op.launch("a stream", synchronous=False)  # noqa: E731
+    launch()                                        # no rows
+    step.stage([0, 1], [4], [[0]])
+    with pytest.raises(DeviceError) as e:
+        launch()
+    assert e.value.status == _abi.LF_INVALID_ARGUMENT and len(launched) == 1
+    step.stage([0, 1], [4], [[0]], [3])
+    launch()
+    step.stage([0, 2], [6], [[0]], prefill_rows=1)
+    with pytest.raises(DeviceError):
+        launch()
+    step.stage([0, 2], [6], [[0]], attention.AS_THEY_ARE, prefill_rows=1)   # written by the caller
+    launch()
+    assert step.positions.data[:4].view(np.int32).tolist() == [3]
+    with pytest.raises(DeviceError):                # a step that is refused leaves the one before
+        step.stage([0, 2], [1], [[0]], prefill_rows=1)
+    launch()
+    step.stage([0], [], [])
+    launch()
+    assert len(launched) == 5
+
+
+def test_rows_without_positions_without_rotation():
+    step, op, launched = rotary_append(None)
+    step.stage([0, 1], [4], [[0]])
+    op.launch("a stream", synchronous=False)
+    assert len(launched) == 1
 
 
 def test_page_tables_that_are_taken():
