@@ -314,10 +314,10 @@ def _holds(what: str, region: KernelArgument, byte_count: int):
         raise _invalid(f"{what}: {byte_count} bytes aligned to 16 are wanted")
 
 
-def _apart(what: str, *regions: KernelArgument):
-    """Refuses regions of one allocation that overlap."""
-    for i, p in enumerate(regions):
-        for q in regions[:i]:
+def _apart(what: str, written, read):
+    """Refuses regions of one allocation that overlap, one of them written."""
+    for i, p in enumerate(written):
+        for q in (*written[:i], *read):
             if p.allocation is q.allocation and p.offset < q.offset + q.byte_count and q.offset < p.offset + p.byte_count:
                 raise _invalid(f"{what} overlap")
 
@@ -342,10 +342,10 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     """Packed rows qkv [max_tokens, Hq + 2 Hkv, D] (a QKV projection's output)
     to rotated queries q [max_tokens, Hq, D] and, in the cache, keys and values
     of every row of the step. gq, gk: the norm weights [D], given if and only if
-    the layer normalizes its heads. The regions may not overlap."""
+    the layer normalizes its heads. q and the caches may overlap neither each
+    other nor what is read."""
     d = layer.desc
     _step_fits(layer, step)
-    _apart("qkv, q and the caches", qkv, q, k_cache, v_cache)
     heads = d.query_heads + 2 * d.kv_heads
     _holds("qkv", qkv, 2 * d.max_tokens * heads * d.head_dim)
     _holds("q", q, 2 * d.max_tokens * d.query_heads * d.head_dim)
@@ -363,6 +363,7 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
             _region(step.row_offsets, alignment=4), _region(step.lengths, alignment=4),
             _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4), layer.region, qkv,
             unused if gq is None else gq, unused if gk is None else gk, q, k_cache, v_cache, _region(ws, alignment=256)]
+    _apart("q, the caches and what is read", args[10:13], args[:10])
     return BoundAttention([LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)], workspace=ws,
                           keep=[layer, step], rotates=step if d.rotary_dim else None)
 
@@ -375,8 +376,6 @@ def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     may not overlap what is read."""
     d = layer.desc
     _step_fits(layer, step)
-    for region in (q, k_cache, v_cache):
-        _apart("out and what is read", out, region)
     _holds("q", q, 2 * d.max_tokens * d.query_heads * d.head_dim)
     _holds("out", out, 2 * d.max_tokens * d.query_heads * d.head_dim)
     _holds("k_cache", k_cache, layer.cache_bytes)
@@ -386,5 +385,6 @@ def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     args = [_region(step.counts, alignment=4), _region(step.row_offsets, alignment=4), _region(step.lengths, alignment=4),
             _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4), layer.region, q, out,
             k_cache, v_cache, _region(ws, alignment=256)]
+    _apart("out and what is read", [out], [a for i, a in enumerate(args) if i != 7])
     return BoundAttention([LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)], workspace=ws,
                           keep=[layer, step])

@@ -6,8 +6,8 @@ import numpy as np
 import pytest
 
 from lunaflux_amd import _abi, attention
-from lunaflux_amd.device import DeviceError
-from test_attention_cpu import bound, make, region
+from lunaflux_amd.device import DeviceError, KernelArgument
+from test_attention_cpu import FakeAllocation, bound, make, region
 
 
 @pytest.mark.parametrize("strides", [
@@ -97,3 +97,44 @@ def test_page_tables_that_are_taken():
     for kind in (np.int32, np.int64, np.uint16):
         step.stage([0, 1, 2], [3, 18], [np.array([4], kind), np.array([2, 0], kind)])
         assert step.page_indices.data[:12].view(np.int32).tolist() == [4, 2, 0]
+
+
+def within(alloc, offset, n):
+    return KernelArgument.device_region(alloc, offset, n, 16)
+
+
+def test_what_the_append_writes_overlaps_nothing_it_reads():
+    rt, layer, step = bound(norm=1e-6)
+    qkv, q, cache = 2 * 32 * 12 * 128, 2 * 32 * 8 * 128, layer.cache_bytes
+    arena = FakeAllocation(qkv + q + 2 * cache + 512)
+    at = [0, qkv, qkv + 256, qkv + 512, qkv + q + 512, qkv + q + cache + 512]
+    size = [qkv, 256, 256, q, cache, cache]
+    good = [within(arena, a, n) for a, n in zip(at, size)]
+    bind = lambda args: attention.bind_qk_norm_rope(rt, layer, step, *args)  # noqa: E731
+    bind(good)                                     # side by side
+    bind([good[0], good[1], good[1], *good[3:]])   # weights are only read
+    for read in (0, 1, 2):
+        for written in (3, 4, 5):
+            args = list(good)
+            args[read] = within(arena, at[written] + size[written] - 256, size[read]) if read else good[0]
+            if read == 0:
+                args[written] = within(arena, qkv - 256, size[written])
+            with pytest.raises(DeviceError):
+                bind(args)
+    # a step's own regions
+    for alloc in (step.counts, step.positions, step.lengths, step.row_offsets, step.page_offsets, step.page_indices):
+        alloc.byte_count = 1 << 20
+        with pytest.raises(DeviceError):
+            bind([*good[:3], within(alloc, 0, q), *good[4:]])
+
+
+def test_what_decode_writes_overlaps_nothing_it_reads():
+    rt, layer, step = bound()
+    q, cache = 2 * 32 * 8 * 128, layer.cache_bytes
+    arena = FakeAllocation(2 * q + 2 * cache)
+    good = [within(arena, 0, q), within(arena, q, q), within(arena, 2 * q, cache), within(arena, 2 * q + cache, cache)]
+    attention.bind_paged_decode(rt, layer, step, *good)
+    for alloc in (step.counts, step.lengths, step.row_offsets, step.page_offsets, step.page_indices, layer.allocation):
+        alloc.byte_count = 1 << 20
+        with pytest.raises(DeviceError):
+            attention.bind_paged_decode(rt, layer, step, good[0], within(alloc, 0, q), *good[2:])
