@@ -125,30 +125,33 @@ def _holds(what: str, region: KernelArgument, byte_count: int, alignment: int):
         raise _invalid(f"{what}: {byte_count} bytes aligned to {alignment} are wanted")
 
 
-def _overlap(p: KernelArgument, q: KernelArgument, byte_count: int) -> bool:
-    return p.allocation is q.allocation and abs(p.offset - q.offset) < byte_count
+def _overlap(p: KernelArgument, p_bytes: int, q: KernelArgument, q_bytes: int) -> bool:
+    return p.allocation is q.allocation and p.offset < q.offset + q_bytes and q.offset < p.offset + p_bytes
 
 
 def bind_low_rank(rt: ProjectionRuntime, counts: Allocation, ids: KernelArgument, x: KernelArgument,
                   adapters: LowRankAdapters, y: KernelArgument, out: KernelArgument, max_tokens: int) -> BoundLowRank:
     """out = y + the adapters' part of the live rows. x [max_tokens, hidden] is
     the projection's input, y [max_tokens, columns] its output; out may be y (in
-    place) and otherwise overlaps neither y nor x."""
+    place) and otherwise overlaps nothing that is read."""
     desc = low_rank_descriptor(adapters.adapters, adapters.rank, adapters.hidden, adapters.widths, max_tokens)
     columns = 2 * max_tokens * desc.columns
     _holds("ids", ids, 4 * max_tokens, 4)
     _holds("x", x, 2 * max_tokens * desc.hidden, 16)
     _holds("y", y, columns, 16)
     _holds("out", out, columns, 16)
-    if (_overlap(out, y, columns) and out.offset != y.offset) or \
-            _overlap(out, x, max(columns, 2 * max_tokens * desc.hidden)):
-        raise _invalid("out overlaps y or x")
+    c, a, b, scaling = _region(counts, COUNTS_BYTES, alignment=4), adapters.a, adapters.b, adapters.scaling
+    n, r = desc.adapters, desc.rank
+    read = [(c, COUNTS_BYTES), (ids, 4 * max_tokens), (x, 2 * max_tokens * desc.hidden), (scaling, 4 * n),
+            (a, 2 * n * desc.slices * r * desc.hidden), (b, 2 * n * desc.columns * r)]
+    if (_overlap(out, columns, y, columns) and out.offset != y.offset) or \
+            any(_overlap(out, columns, region, size) for region, size in read):
+        raise _invalid("out overlaps what is read")
     nbytes = workspace_bytes(desc)
     ws = rt.context.allocate(nbytes)
     ws.copy_from_host(np.zeros(nbytes, np.uint8))
     desc_alloc = rt.context.upload(np.frombuffer(bytes(desc), np.uint8).copy())
-    c, dr, wsr = _region(counts, COUNTS_BYTES, alignment=4), _region(desc_alloc, alignment=4), _region(ws, alignment=256)
-    a, b, scaling = adapters.a, adapters.b, adapters.scaling
+    dr, wsr = _region(desc_alloc, alignment=4), _region(ws, alignment=256)
 
     def step(entry, args):
         geometry = launch_geometry(entry, desc)
