@@ -14,6 +14,7 @@ none). `low_rank` is the numpy-level call for tests and tools.
 from __future__ import annotations
 
 import ctypes
+import operator
 from dataclasses import dataclass
 
 import numpy as np
@@ -44,8 +45,12 @@ def _invalid(what: str):
 
 def low_rank_descriptor(adapters: int, rank: int, hidden: int, widths, max_tokens: int) -> LowRankDescriptor:
     """widths: the output widths of the projections side by side (one, or Q, K, V)."""
-    widths = [int(w) for w in widths]
-    for value in (adapters, rank, max_tokens):
+    widths = [int(w) if isinstance(w, float) and w.is_integer() else w for w in widths]
+    try:  # (ctypes would cut them to their fields)
+        adapters, rank, hidden, max_tokens, *widths = map(operator.index, (adapters, rank, hidden, max_tokens, *widths))
+    except TypeError:
+        raise _invalid("low-rank shape") from None
+    for value in (adapters, rank, max_tokens, hidden, *widths):
         if not 0 < value < 2 ** 31:
             raise _invalid("low-rank shape")
     d = LowRankDescriptor()
@@ -81,12 +86,13 @@ class LowRankAdapters:
 
     def __init__(self, rt: ProjectionRuntime, *, hidden: int, widths, rank: int, adapters: int, a: KernelArgument,
                  b: KernelArgument, scaling: KernelArgument):
-        self.hidden, self.widths, self.rank, self.adapters = hidden, tuple(int(w) for w in widths), rank, adapters
-        low_rank_descriptor(adapters, rank, hidden, self.widths, 1)
-        slices, columns = len(self.widths), sum(self.widths)
-        _holds("a", a, 2 * adapters * slices * rank * hidden, 16)
-        _holds("b", b, 2 * adapters * columns * rank, 16)
-        _holds("scaling", scaling, 4 * adapters, 4)
+        d = low_rank_descriptor(adapters, rank, hidden, widths, 1)
+        ends = [0, *d.ends[:d.slices]]
+        self.hidden, self.rank, self.adapters = d.hidden, d.rank, d.adapters
+        self.widths = tuple(end - begin for begin, end in zip(ends, ends[1:]))
+        _holds("a", a, 2 * d.adapters * d.slices * d.rank * d.hidden, 16)
+        _holds("b", b, 2 * d.adapters * d.columns * d.rank, 16)
+        _holds("scaling", scaling, 4 * d.adapters, 4)
         self.a, self.b, self.scaling = a, b, scaling
 
     @staticmethod
@@ -96,7 +102,7 @@ class LowRankAdapters:
         filled up with zeros."""
         a, b = np.ascontiguousarray(a, np.uint16), np.ascontiguousarray(b, np.uint16)
         scaling = np.ascontiguousarray(scaling, np.float32)
-        widths = [int(w) for w in widths]
+        widths = list(widths)
         if a.ndim != 4 or b.ndim != 3 or a.shape[0] != b.shape[0] or a.shape[1] != len(widths) or \
                 b.shape[1:] != (sum(widths), a.shape[2]) or scaling.shape != (a.shape[0],):
             raise _invalid("low-rank arrays")
@@ -168,6 +174,9 @@ def low_rank(rt: ProjectionRuntime, x: np.ndarray, y: np.ndarray, ids, adapters:
              max_tokens: int | None = None) -> np.ndarray:
     """x bf16 bits [M, hidden], y bf16 bits [M, columns] -> out bf16 bits, in place on the device."""
     x, y = np.ascontiguousarray(x, np.uint16), np.ascontiguousarray(y, np.uint16)
+    ids = np.asarray(ids)
+    if ids.size and (ids.dtype.kind not in "iu" or ids.min() < -2 ** 31 or ids.max() >= 2 ** 31):
+        raise _invalid("adapter ids are whole numbers of 32 bits")
     ids = np.ascontiguousarray(ids, np.int32)
     m = x.shape[0]
     max_tokens = max(m, 1) if max_tokens is None else max_tokens

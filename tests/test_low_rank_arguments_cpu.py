@@ -55,3 +55,34 @@ def test_out_does_not_overlap_the_counts():
     bind(rt, arena, out=within(arena, 32, Y), **regions)
     with pytest.raises(DeviceError):
         bind(rt, arena, out=within(arena, 16, Y), **regions)
+
+
+@pytest.mark.parametrize("args", [
+    (2, 16, 512, [(1 << 64) + 64], 8), (2, 16, 512, [64.5], 8), (2, 16, (1 << 64) + 512, [64], 8), (2, 16, 512.5, [64], 8),
+    (2, 16.0, 512, [64], 8), (2.5, 16, 512, [64], 8), (2, 16, 512, [64], 8.5), (2, 16, 512, ["64"], 8), (2, 16, 512, [None], 8),
+])
+def test_integers_of_a_descriptor(args):
+    with pytest.raises(DeviceError) as e:
+        low_rank.low_rank_descriptor(*args)
+    assert e.value.status == _abi.LF_INVALID_ARGUMENT
+
+
+def test_integers_of_any_type():
+    d = low_rank.low_rank_descriptor(np.int64(2), np.uint8(16), np.int32(512), np.array([64, 128]), np.int16(8))
+    assert (d.adapters, d.rank, d.hidden, d.columns, d.max_tokens) == (2, 16, 512, 192, 8)
+    held = low_rank.LowRankAdapters(FakeRuntime(), hidden=np.int16(512), widths=[64.0, np.uint8(128)], rank=np.uint8(16),
+                                    adapters=np.uint8(20), a=region(2 * 20 * 32 * 512), b=region(2 * 20 * 192 * 16),
+                                    scaling=region(80, 4))
+    assert held.widths == (64, 128) and held.rank == 16
+
+
+@pytest.mark.parametrize("ids", [np.full(M, 1 << 32), np.full(M, 0.5), np.full(M, -(1 << 32) + 1), np.full(M, (1 << 64) - 1, np.uint64),
+                                 np.ones(M, bool), [1 << 70] * M])
+def test_ids_of_rows(ids):
+    """Ids that a cast would turn into another adapter's."""
+    rt = FakeRuntime()
+    adapters = low_rank.LowRankAdapters(rt, hidden=HIDDEN, widths=WIDTHS, rank=RANK, adapters=N, a=region(A), b=region(B),
+                                        scaling=region(S, 4))
+    with pytest.raises(DeviceError) as e:
+        low_rank.low_rank(rt, np.zeros((M, HIDDEN), np.uint16), np.zeros((M, COLUMNS), np.uint16), ids, adapters)
+    assert e.value.status == _abi.LF_INVALID_ARGUMENT
