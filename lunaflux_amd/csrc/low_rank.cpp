@@ -73,11 +73,13 @@ int64_t blocks_of(const lf_fp8_low_rank_desc *d, int64_t columns) {
 
 // Columns of a block: 1024 in one launch; 512 for 16 rows, 128 for each of four
 // waves; 512 or 1024 for 64 rows, where each block starts with a chain of loads: 1024
-// if that leaves 384 blocks. Columns 4096 + 2 x 1024, rank 64: 2000 rows 38 us with 512
-// and 40 with 1024, 4093 rows 56 and 52, 8192 rows 100 and 94 (112 with 2048).
+// if that leaves most of the compute units a block. Columns 4096 + 2 x 1024, rank 64:
+// 192 blocks of 1024 (2000 rows) take 40.0 us and as many rows with 512 38.5, 228 46.6
+// and 48.4, 264 44.2 and 47.2, 300 46.3 and 49.5, 384 (4093 rows) 52.3 and 56.4, 768 94
+// and 100 (112 with 2048); rank 16, 264 blocks 34.7 and 37.9.
 int32_t block_columns_of(const lf_fp8_low_rank_desc *d) {
   if (one_launch_of(d)) return 1024;
-  return expand_rows(d) == 64 && cut(d->max_tokens, 64) * blocks_of(d, 1024) >= 384 ? 1024 : 512;
+  return expand_rows(d) == 64 && cut(d->max_tokens, 64) * blocks_of(d, 1024) >= 224 ? 1024 : 512;
 }
 
 int32_t column_blocks_of(const lf_fp8_low_rank_desc *d) { return static_cast<int32_t>(blocks_of(d, block_columns_of(d))); }

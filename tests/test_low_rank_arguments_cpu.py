@@ -86,3 +86,12 @@ def test_ids_of_rows(ids):
     with pytest.raises(DeviceError) as e:
         low_rank.low_rank(rt, np.zeros((M, HIDDEN), np.uint16), np.zeros((M, COLUMNS), np.uint16), ids, adapters)
     assert e.value.status == _abi.LF_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("rows,widths,block", [
+    (2368, [4096, 1024, 1024], 512), (2369, [4096, 1024, 1024], 1024), (3600, [4096, 1024, 1024], 1024),
+    (14272, [64], 512), (14273, [64], 1024),
+])
+def test_columns_of_a_block(rows, widths, block):
+    """1024 columns from 224 blocks of 64 rows on."""
+    assert low_rank.low_rank_descriptor(4, 64, 4096, widths, rows).block_columns == block
