@@ -84,6 +84,9 @@ class Rotary:
     def of_theta(theta: float, dim: int, sections=None, pairing: str = "half") -> "Rotary":
         """theta^(-2 i / dim) radians per position for pair i. sections: pairs
         of each axis in turn (time, height, width; they add up to dim / 2)."""
+        if not isinstance(dim, (int, np.integer)) or dim < 0 or dim % 2:
+            raise _invalid("rotary dimensions")
+        dim = int(dim)
         pairs = dim // 2
         sections = [pairs] if sections is None else list(sections)
         if sum(sections) != pairs or min(sections) < 0:

@@ -48,6 +48,14 @@ def test_page_tables_of_a_step(table):
         np.testing.assert_array_equal(a.data, b)
 
 
+@pytest.mark.parametrize("dim", [65, 1, -64, -1, 64.0, 64.5])
+def test_dimensions_of_a_rotation(dim):
+    """Pairs of values: an odd number of them has none of its own frequencies."""
+    assert attention.Rotary.of_theta(1e4, 64).turns.size == 32
+    with pytest.raises(DeviceError):
+        attention.Rotary.of_theta(1e4, dim)
+
+
 def rotary_append(rotary):
     rt, layer, step = bound(rotary=rotary)
     qkv, q, cache = region(2 * 32 * 12 * 128), region(2 * 32 * 8 * 128), layer.cache_bytes
