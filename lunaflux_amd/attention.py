@@ -2,8 +2,10 @@
 paged key / value cache's writer and its single-token reader (the attention
 section of include/lunaflux_fp8.h).
 
-The plan vocabulary has these steps as RotaryEmbedding and CausalAttention
-with the runtime inputs of a paged step (lunaflux_amd/plan.py); here they are
+The plan vocabulary's RotaryEmbedding and CausalAttention (lunaflux_amd/plan.py)
+cut the work elsewhere: there the attention appends to the cache and takes prompt
+rows too, and the catalog has no entry for either. These operations read the same
+runtime inputs of a paged step and are bound beside the plan's projections:
 
   bind_qk_norm_rope   per-head norm of queries and keys, rotary positions of
                       one or several axes, append of the step's keys and values
@@ -248,9 +250,11 @@ class PagedStep:
         none, and appends of layers that rotate refuse to launch; AS_THEY_ARE:
         those that the caller wrote to `positions`, or left there by the step
         before. DeviceError INVALID_ARGUMENT, with nothing written, for a
-        step that does not fit or contradicts itself (page indices are the
-        cache owner's, and checked on the device). Launches that read the step
-        before have to be over: the caller synchronizes their streams first."""
+        step that does not fit or contradicts itself (page indices, of any
+        integer type, are the cache owner's and checked on the device). Launches
+        that read the step before have to be over: the caller synchronizes their
+        streams first. Six copies to the device, one after another: 0.11 ms for
+        a few sequences, 0.12 for 32 of 145 pages, 0.7 for 2048 of 16."""
         row_offsets, lengths = np.asarray(row_offsets), np.asarray(lengths)
         n = lengths.size
         for a in (row_offsets, lengths):
@@ -295,7 +299,8 @@ class PagedStep:
 class BoundAttention(BoundOperation):
     """check(): DeviceError(INVALID_ARGUMENT) if a launch met offsets, lengths
     or page indices outside the layer's bounds (the rows and keys concerned
-    were left out); the error word is cleared.
+    were left out); the error word is cleared. After asynchronous launches the
+    caller synchronizes the stream first.
 
     rotates: the step whose positions the operation turns by, or None."""
 

@@ -141,8 +141,12 @@ LF_DEVICE int share_of(int items, int pairs, int blocks) {
 // A step whose pairs all are short is dealt out by pairs instead: block b holds the
 // pairs [first, end), and none is cut. Heads of 128, 8 key heads, us by items and by
 // pairs: 15 sequences of up to 179 keys 19.3 and 9.0, 64 of up to 300 27.7 and 19.8,
-// 16 of up to 1000 23.8 and 19.0, 128 of up to 1000 88 and 84; one of 1000 13.0 and
-// 16.9, so few pairs have to be shorter; steps of one tile per pair 0.5 slower.
+// 16 of up to 1000 23.8 and 19.0, 128 of up to 1000 88 and 84; one of 1000 13.2 and
+// 15.2, so few pairs have to be shorter; steps of one tile per pair 0.3 slower. One
+// longer sequence among short ones does not mind: 15 of 30 and one of 1000 18.7 and
+// 16.5, 3 of 30 and one of 500 22.5 and 11.6. The rule does not see where pairs of full
+// length leave blocks without one, or give some two: 4 of 1000 (32 pairs) 14.5 and
+// 17.5, 33 of 1000 (264 pairs on 256 blocks) 31.5 and 37.0.
 LF_DEVICE int whole_tiles(int pairs) { return pairs < 32 ? 16 : 32; }
 struct PairRange {
   int first, end;

@@ -9,7 +9,11 @@ adds, scaling (x A^T) B^T, goes to the rows of the batch that are its own:
   added = bind_low_rank(rt, counts, ids, x, adapters, y, y, max_tokens)
 
 with ids int32 [max_tokens], the adapter of each row of the step (negative:
-none). `low_rank` is the numpy-level call for tests and tools.
+none). The kernels and their tiles follow from max_tokens, not from the rows of a
+step, so steps of few rows want a binding of their own to the same regions: 61 rows
+of 16 adapters (columns 4096 + 2 x 1024, hidden 4096) take 13.6 us under up to 256
+tokens, 48 under 2048 and 73 under 8192 at rank 16, 32 (57 under 256), 77 and 196
+at rank 64. `low_rank` is the numpy-level call for tests and tools.
 """
 from __future__ import annotations
 
@@ -118,7 +122,8 @@ class LowRankAdapters:
 @dataclass
 class BoundLowRank(BoundOperation):
     """check(): DeviceError(INVALID_ARGUMENT) if a launch met an adapter id past
-    the adapters (its row was left without one); the error word is cleared."""
+    the adapters (its row was left without one); the error word is cleared.
+    After asynchronous launches the caller synchronizes the stream first."""
 
     def check(self):
         if self.workspace.read(np.int32, (1,))[0] != 0:
