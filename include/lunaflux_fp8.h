@@ -513,12 +513,16 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
 /*
  * The steps from the packed Q|K|V rows of a QKV projection to the rows the
  * output projection reads, over a paged key / value cache:
- *  lf_attn_qk_norm_rope_{bf16,e4m3}
+ *  lf_attn_qk_norm_rope_{bf16,e4m3,e4m3_blocks}
  *      (counts, positions, row_offsets, lengths, page_offsets, page_indices,
  *       attn, qkv, gq, gk, q, k_cache, v_cache, status)
- *  lf_attn_decode_d{64,128,256}_{bf16,e4m3}
+ *  lf_attn_decode_d{64,128,256}_{bf16,bf16_sinks,e4m3,e4m3_sinks,e4m3_blocks}
  *      (counts, row_offsets, lengths, page_offsets, page_indices, attn, q,
  *       out, k_cache, v_cache, ws)
+ *  lf_attn_prefill_d{64,128,256}_{bf16,e4m3,e4m3_blocks}
+ *      (the same), then, where the geometry has blocks for it,
+ *  lf_attn_prefill_join_d{64,128,256}_{bf16,e4m3,e4m3_blocks}
+ *      (counts, row_offsets, lengths, page_offsets, attn, out, ws)
  *
  * Runtime inputs, int32, in the vocabulary of a paged step (model/plan
  * runtime inputs): counts = StepCounts; row_offsets [total_rows + 1], the
@@ -540,15 +544,35 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
  * [M, Hq, D] bf16, keys and values to the row's place in the cache, as bf16 or
  * as e4m3 codes of x * (1 / scale[head]), saturated to +-448 (NaN stays NaN).
  *
+ * An E4M3_BLOCKS cache needs no scales beforehand: each block of block_tokens
+ * tokens of a sequence (16, a whole page of 8) has a power of two per head, in
+ * keys and in values, fp32 [pages][page_size / block_tokens][kv_heads] at
+ * block_scales of the cache region. The append makes it the smallest of 2^-100
+ * .. 2^119 by which the largest finite magnitude of the block's rows is at
+ * most 448 (larger ones saturate). Where a step adds rows to a block that has
+ * some already, the block keeps its scale unless the new rows need a larger one;
+ * then its codes are raised to that, as codes of their values. The first row
+ * of a block starts it anew, whatever the table held. So a step writes to a page
+ * for one sequence only, and a sequence whose rows contradict the step (they
+ * leave the batch or outnumber its tokens) is left out whole.
+ *
  * decode, the sequences prefill_rows .. prefill_rows + decode_rows - 1, one
  * row each (the first of its range): out[row] = sum_j p_j v_j over the keys j
- * of [max(0, length - window), length) (window 0: all), p = softmax of
- * softmax_scale q.k_j. Query head h reads key head h / (Hq / Hkv). The scores
+ * of [max(0, length - window), length) (window 0: all) and, behind a window,
+ * of [0, min(sinks, length)), p = softmax of softmax_scale q.k_j. Query head h reads key head h / (Hq / Hkv). The scores
  * and the softmax statistics are fp32; the weights p go to the second product
  * as two bf16 terms (all but 2^-15 of them). A row without keys (or
  * all of whose scores are -inf) gives zeros; values at keys that do not count
  * are not read into the sum, whatever they hold. Other rows of out stay as
  * they were.
+ *
+ * prefill, the sequences 0 .. prefill_rows - 1, any number of rows each: row i
+ * of a sequence of n is at p = length - n + i and counts the keys j <= p, with a
+ * window those with j > p - window or j < sinks; the rest as for decode, except
+ * that the weights go to the second product as bf16 values (their sum is of the
+ * same values). A sequence whose rows leave the batch or outnumber its tokens,
+ * or whose tokens outnumber its pages' slots, is left out. The join launch
+ * follows the other on the same stream.
  *
  * The cache regions hold, for page p, head h and slot i, D elements at
  * p * page_stride + h * head_stride + i * token_stride (elements; any order of
@@ -563,10 +587,11 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
 #define LF_FP8_ATTN_MAX_SEQUENCES 2048
 #define LF_FP8_ATTN_STATUS_BYTES 256
 
-enum lf_fp8_attn_cache { LF_FP8_CACHE_BF16 = 1, LF_FP8_CACHE_E4M3 = 2 };
+enum lf_fp8_attn_cache { LF_FP8_CACHE_BF16 = 1, LF_FP8_CACHE_E4M3 = 2, LF_FP8_CACHE_E4M3_BLOCKS = 3 };
 enum lf_fp8_attn_pairing { LF_FP8_PAIR_HALF = 0, LF_FP8_PAIR_NEIGHBOUR = 1 };
 
-/* The descriptor region: this structure, then (offsets from its start) the
+/* E4M3_BLOCKS: scales by blocks of tokens, in the cache regions themselves.
+ * The descriptor region: this structure, then (offsets from its start) the
  * cache scales fp32 [2][kv_heads] (keys, values), turns fp64 [rotary_dim / 2]
  * (turns per position) and axis int32 [rotary_dim / 2]. */
 typedef struct lf_fp8_attn_desc {
@@ -595,7 +620,10 @@ typedef struct lf_fp8_attn_desc {
   int64_t turns_offset;
   int64_t axis_offset;
   int64_t region_bytes;
-  uint8_t padding[128];
+  int32_t sinks;         /* first tokens that stay visible behind a window; 0: none */
+  int32_t block_tokens;  /* of an E4M3_BLOCKS cache: 16, or 8 where pages are of 8; else 0 */
+  int64_t block_scales;  /* bytes, its table of scales in a cache region; else 0 */
+  uint8_t padding[112];
 } lf_fp8_attn_desc;
 
 /* Checks the fields of *desc, and writes its magic, default strides and the
@@ -606,7 +634,7 @@ typedef struct lf_fp8_attn_desc {
  * offsets do not follow from its fields is refused. */
 int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *desc);
 /* Writes the descriptor region (desc->region_bytes bytes). scales: 2 kv_heads
- * values, finite and above zero (null for a bf16 cache: ones); turns and axis:
+ * values, finite and above zero (null for a bf16 cache, or E4M3_BLOCKS: ones); turns and axis:
  * rotary_dim / 2 each, turns finite, 0 <= axis < axes (null without rotation). */
 int32_t lunaflux_fp8_attn_region(const lf_fp8_attn_desc *desc, const float *scales,
                                  int64_t scale_count, const double *turns, const int32_t *axis,
@@ -616,12 +644,16 @@ int64_t lunaflux_fp8_attn_cache_bytes(const lf_fp8_attn_desc *desc);
 
 enum lf_fp8_attn_entry {
   LF_FP8_ATTN_QK_NORM_ROPE = 1,
-  LF_FP8_ATTN_DECODE = 2
+  LF_FP8_ATTN_DECODE = 2,
+  LF_FP8_ATTN_PREFILL = 3,
+  LF_FP8_ATTN_PREFILL_JOIN = 4
 };
-/* Workspace of DECODE (ws) or of QK_NORM_ROPE (status): zero-filled once when
+/* Workspace of DECODE or PREFILL (ws; its join's is the same one) or of
+ * QK_NORM_ROPE (status): zero-filled once when
  * allocated (its counters return to zero at the end of every launch; launches
  * sharing one must not overlap). -1 if invalid. */
 int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc *desc);
+/* dims[0] is 0 for a PREFILL_JOIN that the descriptor's sizes never need. */
 int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc *desc,
                                           int32_t dims[7], char symbol[LF_FP8_SYMBOL_BYTES]);
 

@@ -1,6 +1,6 @@
 """Host side of the attention between the QKV and the output projection: the
-paged key / value cache's writer and its single-token reader (the attention
-section of include/lunaflux_fp8.h).
+paged key / value cache's writer and its readers, for single tokens and for
+prompts (the attention section of include/lunaflux_fp8.h).
 
 The plan vocabulary's RotaryEmbedding and CausalAttention (lunaflux_amd/plan.py)
 cut the work elsewhere: there the attention appends to the cache and takes prompt
@@ -11,10 +11,14 @@ runtime inputs of a paged step and are bound beside the plan's projections:
                       one or several axes, append of the step's keys and values
   bind_paged_decode   attention of one new token per sequence, split over the
                       cache's length and joined
+  bind_paged_prefill  attention of the rows of prompts, whole or in parts
 
 over regions that stay where they are from step to step: `AttentionLayer`
 holds the layer's constants, `PagedStep` the step's runtime inputs, which
-`stage` rewrites.
+`stage` rewrites. A cache holds bf16 values, e4m3 codes with a scale per head that
+the layer brings ("e4m3"), or e4m3 codes with a scale per block of 16 tokens and
+head that the append finds ("e4m3_blocks"). Under a window the first `sinks`
+tokens can stay visible.
 """
 from __future__ import annotations
 
@@ -29,7 +33,8 @@ from . import _abi
 from .device import Allocation, DeviceError, KernelArgument, KernelArguments, KernelLaunchDimensions
 from .fp8 import COUNTS_BYTES, BoundOperation, LaunchStep, ProjectionRuntime, _region
 
-CACHES = {"bf16": _abi.LF_FP8_CACHE_BF16, "e4m3": _abi.LF_FP8_CACHE_E4M3}
+CACHES = {"bf16": _abi.LF_FP8_CACHE_BF16, "e4m3": _abi.LF_FP8_CACHE_E4M3,
+          "e4m3_blocks": _abi.LF_FP8_CACHE_E4M3_BLOCKS}
 PAIRINGS = {"half": _abi.LF_FP8_PAIR_HALF, "neighbour": _abi.LF_FP8_PAIR_NEIGHBOUR}
 MAX_SEQUENCES = _abi.LF_FP8_ATTN_MAX_SEQUENCES
 AS_THEY_ARE = object()  # PagedStep.stage: the positions that the region holds
@@ -46,7 +51,8 @@ class AttentionDescriptor(ctypes.Structure):
                 ("norm_epsilon", ctypes.c_float), ("softmax_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
                 ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
                 ("scale_offset", ctypes.c_int64), ("turns_offset", ctypes.c_int64), ("axis_offset", ctypes.c_int64),
-                ("region_bytes", ctypes.c_int64), ("padding", ctypes.c_uint8 * 128)]
+                ("region_bytes", ctypes.c_int64), ("sinks", ctypes.c_int32), ("block_tokens", ctypes.c_int32),
+                ("block_scales", ctypes.c_int64), ("padding", ctypes.c_uint8 * 112)]
 
 
 def _check(operation, status):
@@ -113,24 +119,40 @@ class AttentionLayer:
         """Bytes the key cache spans, and the value cache."""
         return _abi.lib().lunaflux_fp8_attn_cache_bytes(ctypes.byref(self.desc))
 
+    @property
+    def block_scales_offset(self) -> int:
+        """Byte of an e4m3_blocks cache region at which its blocks' scales begin."""
+        return self.desc.block_scales
+
+    @property
+    def block_scales_shape(self) -> tuple:
+        """Those scales, fp32 powers of two: pages, blocks of a page, key heads."""
+        d = self.desc
+        if d.block_tokens == 0:
+            raise _invalid("the cache has no scales by blocks")
+        return d.pages, d.page_size // d.block_tokens, d.kv_heads
+
 
 def attention_descriptor(*, query_heads: int, kv_heads: int, head_dim: int, page_size: int, pages: int,
                          max_tokens: int, max_sequences: int, table_entries: int, cache: str = "bf16",
                          rotary: Rotary | None = None, norm_epsilon: float | None = None,
-                         softmax_scale: float | None = None, window: int = 0, strides=None) -> AttentionDescriptor:
+                         softmax_scale: float | None = None, window: int = 0, strides=None,
+                         sinks: int = 0) -> AttentionDescriptor:
     """lunaflux_fp8_attn_descriptor. norm_epsilon None: heads are not
     normalized; softmax_scale None: 1 / sqrt(head_dim); strides: (page, head,
-    token) strides of the caches in elements, None: [page][head][token]."""
+    token) strides of the caches in elements, None: [page][head][token]; window 0:
+    none; sinks: first tokens that a window leaves visible."""
     if cache not in CACHES:
         raise ValueError(f"unknown cache type {cache!r}; expected one of {tuple(CACHES)}")
     d = AttentionDescriptor()
     try:
         d.query_heads, d.kv_heads, d.head_dim, d.cache = query_heads, kv_heads, head_dim, CACHES[cache]
         d.page_size, d.pages, d.max_tokens, d.max_sequences = page_size, pages, max_tokens, max_sequences
-        d.table_entries, d.window = table_entries, window
+        d.table_entries, d.window, d.sinks = table_entries, window, sinks
         for name, value in (("query_heads", query_heads), ("kv_heads", kv_heads), ("head_dim", head_dim),
                             ("page_size", page_size), ("pages", pages), ("max_tokens", max_tokens),
-                            ("max_sequences", max_sequences), ("table_entries", table_entries), ("window", window)):
+                            ("max_sequences", max_sequences), ("table_entries", table_entries), ("window", window),
+                            ("sinks", sinks)):
             if getattr(d, name) != value:  # ctypes cuts to 32 bits
                 raise _invalid(name)
         d.rotary_dim = 0 if rotary is None else 2 * len(rotary.turns)
@@ -175,7 +197,8 @@ def descriptor_region(desc: AttentionDescriptor, k_scales=None, v_scales=None, r
 def attention_layer(rt: ProjectionRuntime, *, k_scales=None, v_scales=None, rotary: Rotary | None = None,
                     **fields) -> AttentionLayer:
     """Checks a layer's constants (attention_descriptor) and uploads them. An
-    e4m3 cache takes fp32 scales per key head (value = code * scale)."""
+    e4m3 cache takes fp32 scales per key head (value = code * scale); an
+    e4m3_blocks cache takes none: the append writes them."""
     desc = attention_descriptor(rotary=rotary, **fields)
     return AttentionLayer(desc, rt.context.upload(descriptor_region(desc, k_scales, v_scales, rotary)))
 
@@ -188,10 +211,13 @@ def workspace_bytes(entry: int, desc: AttentionDescriptor) -> int:
 
 
 def launch_geometry(entry: int, desc: AttentionDescriptor):
+    """(dimensions, symbol) of an entry; None for a join that the sizes never need."""
     dims = (ctypes.c_int32 * 7)()
     symbol = ctypes.create_string_buffer(128)
     _check("attention_launch_geometry", _abi.lib().lunaflux_fp8_attn_launch_geometry(
         entry, ctypes.byref(desc), dims, symbol))
+    if dims[0] == 0:
+        return None
     return (KernelLaunchDimensions.new(tuple(dims[0:3]), tuple(dims[3:6]), dims[6]),
             symbol.value.decode("ascii"))
 
@@ -233,6 +259,7 @@ class PagedStep:
         self.max_tokens, self.max_sequences, self.table_entries = d.max_tokens, d.max_sequences, d.table_entries
         self.axes, self.page_size = d.axes, d.page_size
         self.positioned = True  # the step's rows have positions
+        self._pages, self._apart = None, True
         allocate = rt.context.allocate
         self.counts = allocate(COUNTS_BYTES)
         self.positions = allocate(4 * d.max_tokens * d.axes)
@@ -293,6 +320,20 @@ class PagedStep:
         if written:
             self.positions.copy_from_host(positions.astype(np.int32))
         self.positioned = positions is not None or m == 0
+        self._pages, self._apart = (rows, lengths, counts, indices), None
+
+    @property
+    def pages_apart(self) -> bool:
+        """Whether no two places of the page tables at which the step's rows
+        are written name one page."""
+        if self._apart is None:
+            rows, lengths, counts, indices = self._pages
+            some = rows > 0
+            first, last = (lengths - rows)[some] // self.page_size, (lengths[some] - 1) // self.page_size
+            n, at = last - first + 1, (np.cumsum(counts) - counts)[some] + first
+            written = indices[np.repeat(at - (np.cumsum(n) - n), n) + np.arange(n.sum())]
+            self._apart = np.unique(written).size == written.size
+        return self._apart
 
 
 @dataclass
@@ -302,13 +343,17 @@ class BoundAttention(BoundOperation):
     were left out); the error word is cleared. After asynchronous launches the
     caller synchronizes the stream first.
 
-    rotates: the step whose positions the operation turns by, or None."""
+    rotates: the step whose positions the operation turns by, or None; scales:
+    the step whose rows it appends to a cache with scales by blocks, or None."""
 
     rotates: PagedStep | None = None
+    scales: PagedStep | None = None
 
     def launch(self, stream, synchronous: bool = True):
         if self.rotates is not None and not self.rotates.positioned:
             raise _invalid("rows of the step have no positions to be rotated by")
+        if self.scales is not None and not self.scales.pages_apart:
+            raise _invalid("rows of the step go to one page by two ways")
         super().launch(stream, synchronous)
 
     def check(self):
@@ -351,7 +396,8 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     to rotated queries q [max_tokens, Hq, D] and, in the cache, keys and values
     of every row of the step. gq, gk: the norm weights [D], given if and only if
     the layer normalizes its heads. q and the caches may overlap neither each
-    other nor what is read."""
+    other nor what is read. Over an e4m3_blocks cache a step that writes to one
+    page for two sequences, or twice for one, refuses to launch."""
     d = layer.desc
     _step_fits(layer, step)
     heads = d.query_heads + 2 * d.kv_heads
@@ -373,7 +419,23 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
             unused if gq is None else gq, unused if gk is None else gk, q, k_cache, v_cache, _region(ws, alignment=256)]
     _apart("q, the caches and what is read", args[10:13], args[:10])
     return BoundAttention([LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)], workspace=ws,
-                          keep=[layer, step], rotates=step if d.rotary_dim else None)
+                          keep=[layer, step], rotates=step if d.rotary_dim else None,
+                          scales=step if d.block_tokens else None)
+
+
+def _attention_args(layer: AttentionLayer, step: PagedStep, q: KernelArgument, out: KernelArgument,
+                    k_cache: KernelArgument, v_cache: KernelArgument, ws: Allocation) -> list:
+    """Checked operands of an attention launch; out is at 7."""
+    d = layer.desc
+    _holds("q", q, 2 * d.max_tokens * d.query_heads * d.head_dim)
+    _holds("out", out, 2 * d.max_tokens * d.query_heads * d.head_dim)
+    _holds("k_cache", k_cache, layer.cache_bytes)
+    _holds("v_cache", v_cache, layer.cache_bytes)
+    args = [_region(step.counts, alignment=4), _region(step.row_offsets, alignment=4), _region(step.lengths, alignment=4),
+            _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4), layer.region, q, out,
+            k_cache, v_cache, _region(ws, alignment=256)]
+    _apart("out and what is read", [out], [a for i, a in enumerate(args) if i != 7])
+    return args
 
 
 def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedStep, q: KernelArgument,
@@ -382,17 +444,29 @@ def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     rotated) against the cached keys of each, out [max_tokens, Hq D] as the
     output projection reads it. Rows of other sequences stay as they were. out
     may not overlap what is read."""
-    d = layer.desc
     _step_fits(layer, step)
-    _holds("q", q, 2 * d.max_tokens * d.query_heads * d.head_dim)
-    _holds("out", out, 2 * d.max_tokens * d.query_heads * d.head_dim)
-    _holds("k_cache", k_cache, layer.cache_bytes)
-    _holds("v_cache", v_cache, layer.cache_bytes)
-    ws = _workspace(rt, _abi.ATTN_DECODE, d)
-    dims, symbol = launch_geometry(_abi.ATTN_DECODE, d)
-    args = [_region(step.counts, alignment=4), _region(step.row_offsets, alignment=4), _region(step.lengths, alignment=4),
-            _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4), layer.region, q, out,
-            k_cache, v_cache, _region(ws, alignment=256)]
-    _apart("out and what is read", [out], [a for i, a in enumerate(args) if i != 7])
+    ws = _workspace(rt, _abi.ATTN_DECODE, layer.desc)
+    args = _attention_args(layer, step, q, out, k_cache, v_cache, ws)
+    dims, symbol = launch_geometry(_abi.ATTN_DECODE, layer.desc)
     return BoundAttention([LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)], workspace=ws,
                           keep=[layer, step])
+
+
+def bind_paged_prefill(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedStep, q: KernelArgument,
+                       out: KernelArgument, k_cache: KernelArgument, v_cache: KernelArgument) -> BoundAttention:
+    """Attention of the rows of the step's first prefill_rows sequences: q
+    [max_tokens, Hq, D] (bf16, rotated) against the cached keys of each up to the
+    row's own, which the append has written, out [max_tokens, Hq D]. Rows of
+    decoded sequences stay as they were. out may not overlap what is read. One
+    launch, or two where the layer's sizes let a row have 1024 keys or more (512
+    for heads of 256): then work is split over the keys, and joined. The
+    workspace is 34 to 68 MB then."""
+    _step_fits(layer, step)
+    ws = _workspace(rt, _abi.ATTN_PREFILL, layer.desc)
+    args = _attention_args(layer, step, q, out, k_cache, v_cache, ws)
+    dims, symbol = launch_geometry(_abi.ATTN_PREFILL, layer.desc)
+    steps = [LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)]
+    join = launch_geometry(_abi.ATTN_PREFILL_JOIN, layer.desc)
+    if join is not None:
+        steps.append(LaunchStep(rt.function(join[1]), join[0], KernelArguments([*args[:4], layer.region, out, args[10]]), join[1]))
+    return BoundAttention(steps, workspace=ws, keep=[layer, step])

@@ -19,6 +19,13 @@ constexpr int64_t kGroup = 32;
 constexpr int64_t kHeadTile = 16;
 constexpr int64_t kMostItems = kLimit32 - (1 << 22);  // attention_index.h
 constexpr int64_t kWaves = 4;
+// kernels/attention_prompt.hip
+constexpr int64_t kPromptBlocks = 256;
+constexpr int64_t kJoinSlices = 4;
+constexpr int64_t kCut = 8;  // attention_index.h
+// Blocks of the append to an E4M3_BLOCKS cache that write keys and values; each goes on
+// in steps of the grid.
+constexpr int64_t kMostAppendBlocks = 1 << 14;
 
 int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
@@ -59,9 +66,9 @@ bool strides_ok(const lf_fp8_attn_desc *d) {
 bool fields_ok(const lf_fp8_attn_desc *d) {
   if (d->query_heads < 1 || d->kv_heads < 1 || d->query_heads > 1024 || d->query_heads % d->kv_heads != 0 ||
       (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256) ||
-      (d->cache != LF_FP8_CACHE_BF16 && d->cache != LF_FP8_CACHE_E4M3) || !power_of_two(d->page_size) ||
+      (d->cache != LF_FP8_CACHE_BF16 && d->cache != LF_FP8_CACHE_E4M3 && d->cache != LF_FP8_CACHE_E4M3_BLOCKS) || !power_of_two(d->page_size) ||
       d->page_size < 8 || d->page_size > 1024 || d->pages < 1 || d->max_tokens < 1 || d->max_sequences < 1 ||
-      d->max_sequences > LF_FP8_ATTN_MAX_SEQUENCES || d->table_entries < 1 || d->window < 0) {
+      d->max_sequences > LF_FP8_ATTN_MAX_SEQUENCES || d->table_entries < 1 || d->window < 0 || d->sinks < 0) {
     return false;
   }
   if (d->rotary_dim < 0 || d->rotary_dim % 16 != 0 || d->rotary_dim > d->head_dim || d->axes < 1 ||
@@ -77,6 +84,7 @@ bool fields_ok(const lf_fp8_attn_desc *d) {
       (int64_t(d->table_entries) * d->page_size / kTileKeys + 2 * d->max_sequences) * head_tiles(d) > kMostItems) {
     return false;
   }
+  if (d->cache == LF_FP8_CACHE_E4M3_BLOCKS && d->max_tokens >= (1 << 24) - kMostAppendBlocks) return false;
   return true;
 }
 
@@ -86,13 +94,16 @@ void lay_out(lf_fp8_attn_desc *d) {
   d->turns_offset = d->scale_offset + align_up(int64_t(2) * d->kv_heads * 4, 256);
   d->axis_offset = d->turns_offset + align_up(int64_t(d->rotary_dim) / 2 * 8, 256);
   d->region_bytes = d->axis_offset + align_up(int64_t(d->rotary_dim) / 2 * 4, 256);
+  const bool blocks = d->cache == LF_FP8_CACHE_E4M3_BLOCKS;
+  d->block_tokens = blocks ? std::min<int32_t>(d->page_size, 16) : 0;
+  d->block_scales = blocks ? align_up(last_element(d), 256) : 0;
 }
 
 bool laid_out(const lf_fp8_attn_desc *d) {
   lf_fp8_attn_desc r = *d;
   lay_out(&r);
   return d->scale_offset == r.scale_offset && d->turns_offset == r.turns_offset && d->axis_offset == r.axis_offset &&
-         d->region_bytes == r.region_bytes;
+         d->region_bytes == r.region_bytes && d->block_tokens == r.block_tokens && d->block_scales == r.block_scales;
 }
 
 bool desc_ok(const lf_fp8_attn_desc *d) {
@@ -105,7 +116,7 @@ int64_t tile_rows(const lf_fp8_attn_desc *d) {
 
 // kernels/attention.hip, blocks: blocks of the decode grid.
 int64_t decode_blocks(const lf_fp8_attn_desc *d) {
-  return d->head_dim * (d->cache == LF_FP8_CACHE_E4M3 ? 1 : 2) <= 128 ? 512 : 256;
+  return d->head_dim * element_bytes(d) <= 128 ? 512 : 256;
 }
 
 // The decode workspace: a line with the error word, two arrival counters per
@@ -115,6 +126,36 @@ int64_t decode_bytes(const lf_fp8_attn_desc *d) {
   const int64_t places = 2 * decode_blocks(d);
   return LF_FP8_ATTN_STATUS_BYTES + 2 * places * 4 +
          (places + places / kGroup + 2) * tile_rows(d) * (d->head_dim + 2) * 4;
+}
+
+// kernels/attention_prompt.hip: query rows and keys of a block's tiles.
+int64_t prompt_rows(const lf_fp8_attn_desc *d) { return d->head_dim == 256 ? 128 : 256; }
+int64_t prompt_keys(const lf_fp8_attn_desc *d) { return d->head_dim == 256 ? 32 : 64; }
+
+// Whether a query tile can be cut: it has to have 2 kCut key tiles (attention_index.h).
+bool prompt_cuts(const lf_fp8_attn_desc *d) {
+  int64_t longest = int64_t(d->table_entries) * d->page_size;
+  const int64_t rows = prompt_rows(d), group = d->query_heads / d->kv_heads;
+  const int64_t tokens = std::max<int64_t>(1, rows / group);
+  if (d->window > 0) longest = std::min(longest, int64_t(d->window) + tokens + d->sinks + 2 * prompt_keys(d));
+  return (longest + prompt_keys(d) - 1) / prompt_keys(d) >= 2 * kCut;
+}
+
+// Its workspace: a line with the error word, and, if tiles can be cut, two partial results per block (fp32 [rows][D]
+// sums, maxima and weight sums).
+int64_t prompt_bytes(const lf_fp8_attn_desc *d) {
+  return LF_FP8_ATTN_STATUS_BYTES +
+         (prompt_cuts(d) ? 2 * kPromptBlocks * prompt_rows(d) * (d->head_dim + 2) * 4 : 0);
+}
+
+// Blocks that write an E4M3_BLOCKS cache: four heads' keys or values of one block of tokens each.
+int64_t append_blocks(const lf_fp8_attn_desc *d) {
+  const int64_t touched = std::min<int64_t>(d->max_tokens, d->max_tokens / d->block_tokens + 2 * int64_t(d->max_sequences));
+  return std::min(kMostAppendBlocks, touched * 2 * ((d->kv_heads + kWaves - 1) / kWaves));
+}
+
+const char *cache_name(const lf_fp8_attn_desc *d) {
+  return d->cache == LF_FP8_CACHE_BF16 ? "bf16" : d->cache == LF_FP8_CACHE_E4M3 ? "e4m3" : "e4m3_blocks";
 }
 
 }  // namespace
@@ -132,8 +173,8 @@ int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *d) {
     r.head_stride = int64_t(r.page_size) * r.head_dim;
     r.page_stride = r.kv_heads * r.head_stride;
   }
-  lay_out(&r);
   if (!strides_ok(&r)) return LF_INVALID_ARGUMENT;
+  lay_out(&r);
   *d = r;
   return LF_OK;
 }
@@ -144,7 +185,8 @@ int32_t lunaflux_fp8_attn_region(const lf_fp8_attn_desc *d, const float *scales,
   if (!desc_ok(d) || region == nullptr || region_bytes != d->region_bytes) return LF_INVALID_ARGUMENT;
   const int64_t pairs = d->rotary_dim / 2;
   if (pair_count != pairs || (pairs > 0 && (turns == nullptr || axis == nullptr))) return LF_INVALID_ARGUMENT;
-  if (scales == nullptr ? (scale_count != 0 || d->cache != LF_FP8_CACHE_BF16) : scale_count != 2 * d->kv_heads) {
+  if (scales == nullptr ? (scale_count != 0 || d->cache == LF_FP8_CACHE_E4M3)
+                        : scale_count != 2 * d->kv_heads || d->cache == LF_FP8_CACHE_E4M3_BLOCKS) {
     return LF_INVALID_ARGUMENT;
   }
   for (int64_t i = 0; i < scale_count; ++i) {
@@ -169,7 +211,9 @@ int32_t lunaflux_fp8_attn_region(const lf_fp8_attn_desc *d, const float *scales,
 }
 
 int64_t lunaflux_fp8_attn_cache_bytes(const lf_fp8_attn_desc *d) {
-  return desc_ok(d) ? last_element(d) * element_bytes(d) : -1;
+  if (!desc_ok(d)) return -1;
+  if (d->cache != LF_FP8_CACHE_E4M3_BLOCKS) return last_element(d) * element_bytes(d);
+  return d->block_scales + int64_t(d->pages) * (d->page_size / d->block_tokens) * d->kv_heads * 4;
 }
 
 int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc *d) {
@@ -177,6 +221,8 @@ int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc 
   switch (entry) {
     case LF_FP8_ATTN_QK_NORM_ROPE: return LF_FP8_ATTN_STATUS_BYTES;
     case LF_FP8_ATTN_DECODE: return decode_bytes(d);
+    case LF_FP8_ATTN_PREFILL:
+    case LF_FP8_ATTN_PREFILL_JOIN: return prompt_bytes(d);
     default: return -1;
   }
 }
@@ -184,17 +230,28 @@ int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc 
 int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc *d, int32_t dims[7],
                                           char symbol[LF_FP8_SYMBOL_BYTES]) {
   if (!desc_ok(d) || dims == nullptr || symbol == nullptr) return LF_INVALID_ARGUMENT;
-  const char *type = d->cache == LF_FP8_CACHE_BF16 ? "bf16" : "e4m3";
+  const char *type = cache_name(d);
   int64_t gx = 0, lds = 0;
   switch (entry) {
     case LF_FP8_ATTN_QK_NORM_ROPE:
-      gx = d->max_tokens;
+      gx = d->max_tokens + (d->cache == LF_FP8_CACHE_E4M3_BLOCKS ? append_blocks(d) : 0);
       std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_qk_norm_rope_%s", type);
       break;
     case LF_FP8_ATTN_DECODE:
       gx = decode_blocks(d);
       lds = align_up((int64_t(d->max_sequences) + 1) * 4, 16) + kWaves * tile_rows(d) * (d->head_dim + 4) * 4;
-      std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_decode_d%d_%s", d->head_dim, type);
+      std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_decode_d%d_%s%s", d->head_dim, type,
+                    d->cache != LF_FP8_CACHE_E4M3_BLOCKS && d->window > 0 && d->sinks > 0 ? "_sinks" : "");
+      break;
+    case LF_FP8_ATTN_PREFILL:
+      gx = kPromptBlocks;
+      lds = (int64_t(d->max_sequences) + 1) / 2 * 16 + 16 + 2 * prompt_keys(d) * d->head_dim * 2 * 2;
+      std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_prefill_d%d_%s", d->head_dim, type);
+      break;
+    case LF_FP8_ATTN_PREFILL_JOIN:
+      gx = prompt_cuts(d) ? kPromptBlocks * kJoinSlices : 0;
+      lds = (int64_t(d->max_sequences) + 1) / 2 * 16 + 16;
+      std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_prefill_join_d%d_%s", d->head_dim, type);
       break;
     default: return LF_INVALID_ARGUMENT;
   }

@@ -62,7 +62,83 @@ template <class T, class P>
 LF_DEVICE void put(P *to, T value) {
   __builtin_nontemporal_store(value, reinterpret_cast<T *>(to));
 }
-template <bool E4M3>
+
+// The 16 values that a lane holds of a head of D, in pairs (a[e], b[e]) of the "half" pairing
+// or as two runs of eight, and where they are in the head.
+struct HeadLane {
+  int o0, o1;
+  bool turned, half;
+};
+LF_DEVICE HeadLane head_lane(const Desc &d, int j) {
+  const int R = d.rotary_dim;
+  HeadLane x;
+  x.turned = 16 * j < R;
+  x.half = d.pairing == 0 && x.turned;
+  x.o0 = x.half ? 8 * j : 16 * j;
+  x.o1 = x.half ? R / 2 + 8 * j : 16 * j + 8;
+  return x;
+}
+LF_DEVICE void load_head(const uint16_t *src, const HeadLane &x, float (&a)[8], float (&b)[8]) {
+  const u32x4 w0 = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + x.o0));
+  const u32x4 w1 = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + x.o1));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[2 * i] = bf16_to_f32(w0[i] & 0xffffu);
+    a[2 * i + 1] = bf16_to_f32(w0[i] >> 16);
+    b[2 * i] = bf16_to_f32(w1[i] & 0xffffu);
+    b[2 * i + 1] = bf16_to_f32(w1[i] >> 16);
+  }
+}
+LF_DEVICE void norm_head(const Desc &d, const uint16_t *g, int lanes, const HeadLane &x, float (&a)[8], float (&b)[8]) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
+  for (int m = 1; m < lanes; m <<= 1) ss += __shfl_xor(ss, m);
+  const float inv = 1.0f / __builtin_sqrtf(ss / static_cast<float>(d.head_dim) + d.norm_epsilon);
+  const u32x4 g0 = *reinterpret_cast<const u32x4 *>(g + x.o0);
+  const u32x4 g1 = *reinterpret_cast<const u32x4 *>(g + x.o1);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[2 * i] *= inv * bf16_to_f32(g0[i] & 0xffffu);
+    a[2 * i + 1] *= inv * bf16_to_f32(g0[i] >> 16);
+    b[2 * i] *= inv * bf16_to_f32(g1[i] & 0xffffu);
+    b[2 * i + 1] *= inv * bf16_to_f32(g1[i] >> 16);
+  }
+}
+LF_DEVICE void turn_head(const HeadLane &w, const float (&c)[8], const float (&sn)[8], float (&a)[8], float (&b)[8]) {
+  if (w.half) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = a[e], y = b[e];
+      a[e] = x * c[e] - y * sn[e];
+      b[e] = y * c[e] + x * sn[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = a[2 * e], y = a[2 * e + 1];
+      a[2 * e] = x * c[e] - y * sn[e];
+      a[2 * e + 1] = y * c[e] + x * sn[e];
+      x = b[2 * e];
+      y = b[2 * e + 1];
+      b[2 * e] = x * c[4 + e] - y * sn[4 + e];
+      b[2 * e + 1] = y * c[4 + e] + x * sn[4 + e];
+    }
+  }
+}
+// Cosine and sine of pair i of the row's rotation.
+LF_DEVICE float2 turn_of(const Desc &d, const uint8_t *attn, const int32_t *positions, int row, int i) {
+  const double *turns = reinterpret_cast<const double *>(attn + d.turns_offset);
+  const int32_t *axis = reinterpret_cast<const int32_t *>(attn + d.axis_offset);
+  const double t = static_cast<double>(positions[static_cast<int64_t>(row) * d.axes + axis[i]]) * turns[i];
+  float sin_t, cos_t;
+  sincospif(static_cast<float>(2.0 * (t - rint(t))), &sin_t, &cos_t);
+  return make_float2(cos_t, sin_t);
+}
+
+// Keys and values of the rows go to the cache too (CACHE kCacheBf16, kCacheE4m3), or are
+// append_blocks' part (kCacheBlocks).
+template <int CACHE>
 LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, const int32_t *row_offsets,
                             const int32_t *lengths, const int32_t *page_offsets, const int32_t *page_indices,
                             const uint8_t *attn, const uint16_t *qkv, const uint16_t *gq, const uint16_t *gk,
@@ -79,109 +155,236 @@ LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, con
   if (s >= sequences || row < row_offsets[0]) return;
 
   const int R = d.rotary_dim;
-  if (static_cast<int>(threadIdx.x) < R / 2) {
-    const int i = threadIdx.x;
-    const double *turns = reinterpret_cast<const double *>(attn + d.turns_offset);
-    const int32_t *axis = reinterpret_cast<const int32_t *>(attn + d.axis_offset);
-    const double t = static_cast<double>(positions[row * d.axes + axis[i]]) * turns[i];
-    float sin_t, cos_t;
-    sincospif(static_cast<float>(2.0 * (t - rint(t))), &sin_t, &cos_t);
-    turn[i] = make_float2(cos_t, sin_t);
-  }
+  if (static_cast<int>(threadIdx.x) < R / 2) turn[threadIdx.x] = turn_of(d, attn, positions, row, threadIdx.x);
   __syncthreads();
 
-  const Place place = place_of(d, row_offsets, lengths, page_offsets, page_indices, s, row);
-  if (place.page < 0 && threadIdx.x == 0) flag_error(status);
+  Place place = {-1, 0};
+  if constexpr (CACHE != kCacheBlocks) {
+    place = place_of(d, row_offsets, lengths, page_offsets, page_indices, s, row);
+    if (place.page < 0 && threadIdx.x == 0) flag_error(status);
+  }
 
   const int D = d.head_dim, lanes = D >> 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int j = lane & (lanes - 1);
-  const bool turned = 16 * j < R;
-  const bool half = d.pairing == 0 && turned;
-  const int o0 = half ? 8 * j : 16 * j;
-  const int o1 = half ? R / 2 + 8 * j : 16 * j + 8;
+  const HeadLane at = head_lane(d, j);
   float c[8], sn[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float2 t = turned ? turn[8 * j + e] : make_float2(1.0f, 0.0f);
+    const float2 t = at.turned ? turn[8 * j + e] : make_float2(1.0f, 0.0f);
     c[e] = t.x;
     sn[e] = t.y;
   }
   const int Hq = d.query_heads, Hkv = d.kv_heads, heads = Hq + 2 * Hkv;
+  const int done = CACHE == kCacheBlocks ? Hq : heads;
   const int per_wave = 64 / lanes;
   const float *scales = reinterpret_cast<const float *>(attn + d.scale_offset);
-  for (int base = wave * per_wave; base < heads; base += 4 * per_wave) {
+  for (int base = wave * per_wave; base < done; base += 4 * per_wave) {
     const int h = base + lane / lanes;
-    if (h >= heads) continue;
-    const uint16_t *src = qkv + (static_cast<uint64_t>(row) * heads + h) * D;
-    const u32x4 w0 = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + o0));
-    const u32x4 w1 = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + o1));
+    if (h >= done) continue;
     float a[8], b[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[2 * i] = bf16_to_f32(w0[i] & 0xffffu);
-      a[2 * i + 1] = bf16_to_f32(w0[i] >> 16);
-      b[2 * i] = bf16_to_f32(w1[i] & 0xffffu);
-      b[2 * i + 1] = bf16_to_f32(w1[i] >> 16);
-    }
+    load_head(qkv + (static_cast<uint64_t>(row) * heads + h) * D, at, a, b);
     if (h < Hq + Hkv) {
-      if (d.norm) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
-        for (int m = 1; m < lanes; m <<= 1) ss += __shfl_xor(ss, m);
-        const float inv = 1.0f / __builtin_sqrtf(ss / static_cast<float>(D) + d.norm_epsilon);
-        const uint16_t *g = h < Hq ? gq : gk;
-        const u32x4 g0 = *reinterpret_cast<const u32x4 *>(g + o0);
-        const u32x4 g1 = *reinterpret_cast<const u32x4 *>(g + o1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[2 * i] *= inv * bf16_to_f32(g0[i] & 0xffffu);
-          a[2 * i + 1] *= inv * bf16_to_f32(g0[i] >> 16);
-          b[2 * i] *= inv * bf16_to_f32(g1[i] & 0xffffu);
-          b[2 * i + 1] *= inv * bf16_to_f32(g1[i] >> 16);
-        }
-      }
-      if (turned) {
-        if (half) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = a[e], y = b[e];
-            a[e] = x * c[e] - y * sn[e];
-            b[e] = y * c[e] + x * sn[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = a[2 * e], y = a[2 * e + 1];
-            a[2 * e] = x * c[e] - y * sn[e];
-            a[2 * e + 1] = y * c[e] + x * sn[e];
-            x = b[2 * e];
-            y = b[2 * e + 1];
-            b[2 * e] = x * c[4 + e] - y * sn[4 + e];
-            b[2 * e + 1] = y * c[4 + e] + x * sn[4 + e];
-          }
-        }
-      }
+      if (d.norm) norm_head(d, h < Hq ? gq : gk, lanes, at, a, b);
+      if (at.turned) turn_head(at, c, sn, a, b);
     }
     if (h < Hq) {
       uint16_t *dst = q + (static_cast<uint64_t>(row) * Hq + h) * D;
-      put(dst + o0, bf16x8_of(a));
-      put(dst + o1, bf16x8_of(b));
+      put(dst + at.o0, bf16x8_of(a));
+      put(dst + at.o1, bf16x8_of(b));
     } else if (place.page >= 0) {
       const bool value = h >= Hq + Hkv;
       const int kh = h - Hq - (value ? Hkv : 0);
-      uint8_t *dst = (value ? vc : kc) + cache_byte<E4M3>(d, place.page, kh, place.slot);
-      if constexpr (E4M3) {
+      uint8_t *dst = (value ? vc : kc) + cache_byte<CACHE == kCacheE4m3>(d, place.page, kh, place.slot);
+      if constexpr (CACHE == kCacheE4m3) {
         const float inv_scale = 1.0f / scales[(value ? Hkv : 0) + kh];
-        put(dst + o0, e4m3x8_of(a, inv_scale));
-        put(dst + o1, e4m3x8_of(b, inv_scale));
+        put(dst + at.o0, e4m3x8_of(a, inv_scale));
+        put(dst + at.o1, e4m3x8_of(b, inv_scale));
       } else {
-        put(dst + 2 * o0, bf16x8_of(a));
-        put(dst + 2 * o1, bf16x8_of(b));
+        put(dst + 2 * at.o0, bf16x8_of(a));
+        put(dst + 2 * at.o1, bf16x8_of(b));
       }
     }
   }
+}
+
+// ---- append with a scale per block of tokens and head --------------------------------
+
+// The scale is the least power of two, of 2^-100 to 2^119, by which the block's largest finite
+// magnitude is at most 448, e4m3's largest. As a power of two it costs no rounding: neither at
+// the append nor where codes become bf16 values, and codes that are raised to a larger
+// scale are rounded again only below 2^-6 of it.
+LF_DEVICE float scale_of(float amax) {
+  const int e = static_cast<int>((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8;  // 448 = 1.75 2^8
+  return __uint_as_float(static_cast<uint32_t>((e < -100 ? -100 : e > 119 ? 119 : e) + 127) << 23);
+}
+
+LF_DEVICE u32x2 raised(u32x2 codes, float ratio) {
+  u32x2 out;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes[i]), false);
+    const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes[i]), true);
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * ratio, lo[1] * ratio, 0, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * ratio, hi[1] * ratio, p, true);
+    out[i] = static_cast<uint32_t>(p);
+  }
+  return out;
+}
+
+// A wave holds the rows of one block of tokens (at most 16) of one head's keys or values in
+// registers: their largest magnitude, the scale, the codes. Blocks of the grid take four heads
+// of one block of tokens, found by the number of blocks that the sequences before have. A block
+// of tokens that holds older ones keeps its scale or raises it, and then their codes.
+template <int D>
+LF_DEVICE void append_rows(const Desc &d, const uint16_t *qkv, const uint16_t *gk, const float2 (*turn)[128],
+                           const Block &x, int page, int unit_head, bool value, uint8_t *cache) {
+  constexpr int kLanes = D / 16, kRows = 64 / kLanes, kPasses = (16 + kRows - 1) / kRows;
+  const int lane = threadIdx.x & 63, j = lane & (kLanes - 1), r = lane / kLanes;
+  const HeadLane at = head_lane(d, j);
+  const int Hq = d.query_heads, Hkv = d.kv_heads, heads = Hq + 2 * Hkv;
+  const int h = Hq + (value ? Hkv : 0) + unit_head;
+  float *scales = reinterpret_cast<float *>(cache + d.block_scales) + scale_index(d, page, x.slot, unit_head);
+  const float old = x.lo > 0 ? *scales : 0.0f;
+  float a[kPasses][8], b[kPasses][8];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int slot = p * kRows + r;
+    const bool mine = slot >= x.lo && slot < x.hi;
+    load_head(qkv + (static_cast<uint64_t>(x.row + (mine ? slot - x.lo : 0)) * heads + h) * D, at, a[p], b[p]);
+  }
+  float amax = 0.0f;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int slot = p * kRows + r;
+    const bool mine = slot >= x.lo && slot < x.hi;
+    if (!value) {
+      if (d.norm) norm_head(d, gk, kLanes, at, a[p], b[p]);
+      if (at.turned) {
+        float c[8], sn[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 t = turn[mine ? slot - x.lo : 0][8 * j + e];
+          c[e] = t.x;
+          sn[e] = t.y;
+        }
+        turn_head(at, c, sn, a[p], b[p]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float u = fabsf(a[p][e]), v = fabsf(b[p][e]);
+      amax = fmaxf(amax, mine && u < INFINITY ? u : 0.0f);
+      amax = fmaxf(amax, mine && v < INFINITY ? v : 0.0f);
+    }
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
+  float scale = scale_of(amax);
+  if (old > scale) scale = old;
+  const bool grows = x.lo > 0 && old != scale;
+  const float inv_scale = 1.0f / scale, ratio = old * inv_scale;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int slot = p * kRows + r;
+    uint8_t *dst = cache + cache_byte<true>(d, page, unit_head, x.slot + slot);
+    if (slot >= x.lo && slot < x.hi) {
+      put(dst + at.o0, e4m3x8_of(a[p], inv_scale));
+      put(dst + at.o1, e4m3x8_of(b[p], inv_scale));
+    } else if (grows && slot < x.lo) {
+      u32x2 *o0 = reinterpret_cast<u32x2 *>(dst + at.o0), *o1 = reinterpret_cast<u32x2 *>(dst + at.o1);
+      const u32x2 w0 = *o0, w1 = *o1;
+      *o0 = raised(w0, ratio);
+      *o1 = raised(w1, ratio);
+    }
+  }
+  if (lane == 0) *scales = scale;
+}
+
+LF_DEVICE void append_blocks(const int32_t *counts, const int32_t *positions, const int32_t *row_offsets,
+                             const int32_t *lengths, const int32_t *page_offsets, const int32_t *page_indices,
+                             const uint8_t *attn, const uint16_t *qkv, const uint16_t *gk, uint8_t *kc, uint8_t *vc,
+                             int *status) {
+  __shared__ int prefix[2048];  // LF_FP8_ATTN_MAX_SEQUENCES
+  __shared__ int wave_total[4];
+  __shared__ float2 turn[16][128];
+  const Desc &d = desc_of(attn);
+  if (d.magic != kMagic) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = live_rows(counts, d.max_tokens);
+  int n = counts[2];
+  n = n < 0 ? 0 : n > d.max_sequences ? d.max_sequences : n;
+  bool bad = false;
+  int64_t carry = 0;
+  for (int base = 0; base < n; base += 256) {
+    const int i = base + static_cast<int>(threadIdx.x);
+    int blocks = 0;
+    if (i < n) blocks = blocks_of(d, prompt_of(d, row_offsets, lengths, page_offsets, i, rows, bad));
+    int sum = blocks;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int up = __shfl_up(sum, m);
+      if (lane >= m) sum += up;
+    }
+    if (lane == 63) wave_total[wave] = sum;
+    __syncthreads();
+    int64_t before = carry;
+    for (int k = 0; k < 4; ++k) {
+      if (k < wave) before += wave_total[k];
+      carry += wave_total[k];
+    }
+    if (i < n) prefix[i] = static_cast<int>(before) + sum - blocks;
+    __syncthreads();
+  }
+  __syncthreads();
+  if (carry > rows) {  // sequences that share rows: a block of tokens has a row at least
+    flag_error(status);
+    return;
+  }
+  const int Hkv = d.kv_heads, groups = (Hkv + 3) / 4;
+  const int64_t items = carry * 2 * groups;
+  for (int64_t u = blockIdx.x - d.max_tokens; u < items; u += gridDim.x - d.max_tokens) {
+    const int b = static_cast<int>(u / (2 * groups)), unit = static_cast<int>(u - static_cast<int64_t>(b) * 2 * groups);
+    const bool value = unit >= groups;
+    int s = 0;  // the last with prefix[s] <= b, so one with blocks
+    for (int hi = n; hi - s > 1;) {
+      const int mid = (s + hi) >> 1;
+      if (prefix[mid] <= b) {
+        s = mid;
+      } else {
+        hi = mid;
+      }
+    }
+    bool unused = false;
+    const Prompt p = prompt_of(d, row_offsets, lengths, page_offsets, s, rows, unused);
+    const Block x = block_of(d, p, b - prefix[s]);
+    const int page = page_indices[x.entry];
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(d.pages)) {
+      bad = true;
+      continue;
+    }
+    if (!value && d.rotary_dim > 0) {
+      const int pairs = d.rotary_dim / 2;
+      __syncthreads();  // the turns of the item before have been read
+      for (int i = threadIdx.x; i < (x.hi - x.lo) * pairs; i += 256) {
+        const int r = i / pairs;
+        turn[r][i - r * pairs] = turn_of(d, attn, positions, x.row + r, i - r * pairs);
+      }
+      __syncthreads();
+    }
+    const int h = (value ? unit - groups : unit) * 4 + wave;
+    if (h >= Hkv) continue;
+    uint8_t *cache = value ? vc : kc;
+    if (d.head_dim == 64) {
+      append_rows<64>(d, qkv, gk, turn, x, page, h, value, cache);
+    } else if (d.head_dim == 128) {
+      append_rows<128>(d, qkv, gk, turn, x, page, h, value, cache);
+    } else {
+      append_rows<256>(d, qkv, gk, turn, x, page, h, value, cache);
+    }
+  }
+  if (bad) flag_error(status);
 }
 
 // ---- attention of one new token per sequence -------------------------------
@@ -436,6 +639,7 @@ struct Piece {
   int lo, len, base, stop;
   int h, row0, live, row;  // row of q and out, or -1
   int pair, tiles;         // its pair's first item and tiles
+  int sink, edge, jump;    // the first keys that count too; from `edge` on, keys are `jump` further
 };
 
 // What a block keeps of each of the first sequences in LDS.
@@ -443,8 +647,16 @@ struct Sequence {
   Span span;
   int entry, row;  // first page table entry, row of q and out
 };
+struct Sinks {
+  int sink, tiles;
+};
 
-template <int D, bool E4M3>
+// BLOCKS: an e4m3 cache with scales by blocks of tokens. A lane's keys of a half of the tile
+// lie in one block, so its key scale multiplies the half's scores and its value scale the
+// weights, which are powers of two and leave the weights' mantissas; the sum of the weights
+// takes its ones divided by them. SINKS: Piece's base, stop and the tiles are counted along the
+// keys that are read, the sinks' tiles and then the window's.
+template <int D, bool E4M3, bool BLOCKS, bool SINKS>
 LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths,
                       const int32_t *page_offsets, const int32_t *page_indices, const uint8_t *attn,
                       const uint16_t *q, uint16_t *out, const uint8_t *kc, const uint8_t *vc, uint8_t *ws) {
@@ -453,6 +665,7 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   __shared__ int arrived;
   __shared__ float stats[2][kGroup][kHeadTile];
   __shared__ Sequence near[64 * kWaves];
+  __shared__ Sinks near_sinks[SINKS ? 64 * kWaves : 1];
   const Desc &d = desc_of(attn);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (the loads before the first wait: each further round trip to memory delays
@@ -463,10 +676,16 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
   if (magic != static_cast<int>(kMagic)) return;
   const Decoded decoded = decoded_of(d, count0, count1, count2);
   const int s0 = decoded.s0, n = decoded.n;
-  auto load_sequence = [&](int s, bool &is_bad) {
+  auto load_sequence = [&](int s, bool &is_bad, Sinks &sinks) {
     const int len = lengths[s], first = page_offsets[s], end = page_offsets[s + 1], row = row_offsets[s];
     const Pages pages = pages_of(d, first, end, is_bad);
-    return Sequence{span_of(d, len, pages, is_bad), pages.first, row};
+    if constexpr (SINKS) {
+      const SinkSpan span = sink_span_of(d, len, pages, is_bad);
+      sinks = {span.sink, span.sink_tiles};
+      return Sequence{span.span, pages.first, row};
+    } else {
+      return Sequence{span_of(d, len, pages, is_bad), pages.first, row};
+    }
   };
 
   int *prefix = reinterpret_cast<int *>(lds);
@@ -477,9 +696,13 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     const int i = base + static_cast<int>(threadIdx.x);
     int tiles = 0;
     if (i < n) {
-      const Sequence q1 = load_sequence(s0 + i, bad);
+      Sinks sinks;
+      const Sequence q1 = load_sequence(s0 + i, bad, sinks);
       tiles = q1.span.tiles;
-      if (base == 0) near[i] = q1;
+      if (base == 0) {
+        near[i] = q1;
+        if constexpr (SINKS) near_sinks[i] = sinks;
+      }
     }
     longer |= tiles > most_tiles;
     int sum = tiles;
@@ -552,7 +775,8 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     while (u < end) {
       const int i = __builtin_amdgcn_readfirstlane(sequence_at(prefix, n, head_tiles, u));
       bool unused = false;
-      const Sequence seq = i < 64 * kWaves ? near[i] : load_sequence(s0 + i, unused);
+      Sinks sinks = SINKS && i < 64 * kWaves ? near_sinks[i] : Sinks{0, 0};
+      const Sequence seq = i < 64 * kWaves ? near[i] : load_sequence(s0 + i, unused, sinks);
       auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
       const Span span = {same(seq.span.first_tile), same(seq.span.tiles), same(seq.span.lo), same(seq.span.len)};
       const int within = u - __builtin_amdgcn_readfirstlane(prefix[i]) * head_tiles;
@@ -571,8 +795,17 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       x.table = page_indices + __builtin_amdgcn_readfirstlane(seq.entry);
       x.lo = span.lo;
       x.len = span.len;
-      x.base = (span.first_tile + t0) * kTileKeys;
-      x.stop = (span.first_tile + t1) * kTileKeys < span.len ? (span.first_tile + t1) * kTileKeys : span.len;
+      if constexpr (SINKS) {
+        const int sink_tiles = same(sinks.tiles);
+        x.sink = same(sinks.sink);
+        x.edge = sink_tiles * kTileKeys;
+        x.jump = (span.first_tile - sink_tiles) * kTileKeys;
+        x.base = t0 * kTileKeys;
+        x.stop = t1 * kTileKeys < span.len - x.jump ? t1 * kTileKeys : span.len - x.jump;
+      } else {
+        x.base = (span.first_tile + t0) * kTileKeys;
+        x.stop = (span.first_tile + t1) * kTileKeys < span.len ? (span.first_tile + t1) * kTileKeys : span.len;
+      }
       u += t1 - t0;
       if (span.len > 0) return true;
       if (x.row >= 0) {  // no keys
@@ -582,8 +815,12 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     }
     return false;
   };
-  auto indices = [&](const int32_t *table, int lo, int len, int base) {
-    return table[entry_of(lo >> shift, (len + slot_mask) >> shift, shift, base + 8 * (lane & 3))];
+  // the key that a tile counted along the piece begins with
+  auto key_of = [&](const Piece &x, int base) { return SINKS ? base + (base >= x.edge ? x.jump : 0) : base; };
+  auto indices = [&](const Piece &x, int base) {
+    const int j = key_of(x, base) + 8 * (lane & 3), first = x.lo >> shift, end = (x.len + slot_mask) >> shift;
+    if constexpr (SINKS) return x.table[sink_entry_of((x.sink + slot_mask) >> shift, first, end, shift, j)];
+    return x.table[entry_of(first, end, shift, j)];
   };
   auto tile_groups = [&](int page, int base) {
     return groups_of(page, pages, page_bytes, token_bytes, slot_mask, base);
@@ -622,24 +859,39 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     return;
   }
   Tile<D, E4M3> x;
-  Groups at = tile_groups(indices(now.table, now.lo, now.len, now.base), now.base);
+  // BLOCKS: lanes 0 .. 3 (of every eight) hold the key scales of a tile's groups, 4 .. 7 the value
+  // scales (a finite one also where no key counts).
+  float steps = 1.0f;
+  auto load_steps = [&](int page, int h, int base) {
+    if constexpr (BLOCKS) {
+      const uint8_t *side = (lane & 4) != 0 ? vc : kc;
+      const int p = static_cast<uint32_t>(page) < static_cast<uint32_t>(pages) ? page : 0;
+      const float v = reinterpret_cast<const float *>(side + d.block_scales)[scale_index(d, p, (base + 8 * (lane & 3)) & slot_mask, h)];
+      return fminf(fmaxf(v, 0x1p-100f), 0x1p119f);
+    } else {
+      return 1.0f;
+    }
+  };
+  const int first_page = indices(now, now.base);
+  Groups at = tile_groups(first_page, key_of(now, now.base));
   load_keys(x, keys_of(now.h), at, c);
+  steps = load_steps(first_page, now.h, key_of(now, now.base));
   load_queries(now);
-  int ahead = indices(now.table, now.lo, now.len, now.base + kStep);
+  int ahead = indices(now, now.base + kStep);
   asm volatile("" ::: "memory");  // values last, as in the loop
   load_values(x, values_of(now.h), at, token_bytes, g);
   bool has_next = take_mine(next);
   if (!has_next) next = now;  // what is loaded behind the last tile
   auto after_one_tile = [&]() {  // a piece of one tile: the tile ahead is the next piece's
     if (now.base + kStep >= now.stop) {
-      ahead = indices(next.table, next.lo, next.len, next.base);
+      ahead = indices(next, next.base);
       asm volatile("" : "+v"(ahead));  // waited for here, not where every tile's is
     }
   };
   after_one_tile();
 
   for (;;) {
-    const float factor = d.softmax_scale * 1.44269504088896341f * (E4M3 ? scales[now.h] : 1.0f);
+    const float factor = d.softmax_scale * 1.44269504088896341f * (E4M3 && !BLOCKS ? scales[now.h] : 1.0f);
     f32x4 o[D / 16];
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -672,24 +924,37 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       // (All loads are issued on every path: a load that a branch may skip makes
       // the wait for an older one a wait for all.)
       const bool more = base + kStep < now.stop;
-      const Groups then = tile_groups(ahead, more ? base + kStep : next.base);
+      const int then_base = more ? key_of(now, base + kStep) : key_of(next, next.base);
+      const Groups then = tile_groups(ahead, then_base);
       const uint32_t then_h = more ? now.h : next.h;
       load_keys(x, keys_of(then_h), then, c);
+      float step[2][2] = {{1.0f, 1.0f}, {1.0f, 1.0f}};  // [key, value][half]
+      if constexpr (BLOCKS) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) step[i >> 1][i & 1] = __shfl(steps, 4 * (i >> 1) + 2 * (i & 1) + (g >> 1));
+        steps = load_steps(ahead, then_h, then_base);
+      }
       if (!more) load_queries(next);
       {
         const bool same = base + 2 * kStep < now.stop;
-        ahead = indices(same ? now.table : next.table, same ? now.lo : next.lo, same ? now.len : next.len,
-                        same ? base + 2 * kStep : more ? next.base : next.base + kStep);
+        if constexpr (SINKS) {
+          ahead = indices(same ? now : next, same ? base + 2 * kStep : more ? next.base : next.base + kStep);
+        } else {
+          Piece of = same ? now : next;
+          ahead = indices(of, same ? base + 2 * kStep : more ? next.base : next.base + kStep);
+        }
       }
       float z[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = sc[e >> 2][e & 3] * factor;
+      for (int e = 0; e < 8; ++e) z[e] = sc[e >> 2][e & 3] * (BLOCKS ? factor * step[0][e >> 2] : factor);
       if (at.in != 15 && base < now.stop) bad = true;
-      if (base < now.lo || base + kTileKeys > now.stop || at.in != 15) {
+      const int key = key_of(now, base);
+      if ((key < now.lo && (!SINKS || key + kTileKeys > now.sink)) || base + kTileKeys > now.stop || at.in != 15) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int j = base + 16 * (e >> 2) + 4 * g + (e & 3);
-          const bool live = j >= now.lo && j < now.stop && ((at.in >> (2 * (e >> 2) + (g >> 1))) & 1) != 0;
+          const int within = 16 * (e >> 2) + 4 * g + (e & 3), j = key + within;
+          const bool live = (j >= now.lo || (SINKS && j < now.sink)) && base + within < now.stop &&
+                            ((at.in >> (2 * (e >> 2) + (g >> 1))) & 1) != 0;
           z[e] = live ? z[e] : -INFINITY;
           // a weight of zero times what the place holds would let an infinity or NaN through
 #pragma unroll
@@ -715,13 +980,22 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       uint32_t pw[4], rw[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p0 = __builtin_amdgcn_exp2f(z[2 * e] - from), p1 = __builtin_amdgcn_exp2f(z[2 * e + 1] - from);
+        float p0 = __builtin_amdgcn_exp2f(z[2 * e] - from), p1 = __builtin_amdgcn_exp2f(z[2 * e + 1] - from);
+        if constexpr (BLOCKS) {
+          p0 *= step[1][e >> 1];
+          p1 *= step[1][e >> 1];
+        }
         pw[e] = upper_halves(p0, p1);
         rw[e] = f32_to_bf16(rest_of(p0)) | (f32_to_bf16(rest_of(p1)) << 16);
       }
       const bf16x8 p = operand(pw[0], pw[1], pw[2], pw[3]), rest = operand(rw[0], rw[1], rw[2], rw[3]);
       constexpr uint32_t kOne2 = 0x3f803f80u;
-      const bf16x8 ones = operand(kOne2, kOne2, kOne2, kOne2);
+      uint32_t one[2] = {kOne2, kOne2};
+      if constexpr (BLOCKS) {  // 2^-e of the halves' value scales 2^e, in bf16
+#pragma unroll
+        for (int half = 0; half < 2; ++half) one[half] = (0x7f00u - (__float_as_uint(step[1][half]) >> 16)) * 0x10001u;
+      }
+      const bf16x8 ones = operand(one[0], one[0], one[1], one[1]);
       sum4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p, sum4, 0, 0, 0);
       sum4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, rest, sum4, 0, 0, 0);
       // values as pairs of neighbouring columns, bf16
@@ -774,7 +1048,7 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     __syncthreads();
     const Parts parts = parts_of(now.pair, now.tiles, share);
     const bool whole = by_pair || parts.first == parts.last;
-    const float vscale = E4M3 ? scales[Hkv + now.h] : 1.0f;
+    const float vscale = E4M3 && !BLOCKS ? scales[Hkv + now.h] : 1.0f;
     const int live = now.live;
     uint16_t *dst = out + (static_cast<uint64_t>(now.row < 0 ? 0 : now.row) * Hq + now.h * group + now.row0) * D;
     float *part = w.parts + static_cast<uint64_t>(part_slot(block, now.pair, share)) * w.floats;
@@ -849,32 +1123,50 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
 
 }  // namespace attn
 
-#define LF_ATTN_ROPE(TYPE, E4M3)                                                                               \
-  extern "C" __global__ __launch_bounds__(256) void lf_attn_qk_norm_rope_##TYPE(                               \
+#define LF_ATTN_ROPE(TYPE, CACHE)                                                                              \
+  extern "C" __global__ __launch_bounds__(256, CACHE == attn::kCacheBf16 ? 8 : CACHE == attn::kCacheE4m3 ? 7 : 3) void lf_attn_qk_norm_rope_##TYPE( \
       const int32_t *__restrict__ counts, const int32_t *__restrict__ positions,                               \
       const int32_t *__restrict__ row_offsets, const int32_t *__restrict__ lengths,                            \
       const int32_t *__restrict__ page_offsets, const int32_t *__restrict__ page_indices,                      \
       const uint8_t *__restrict__ desc, const uint16_t *__restrict__ qkv,                                      \
       const uint16_t *__restrict__ gq, const uint16_t *__restrict__ gk, uint16_t *__restrict__ q,              \
       uint8_t *__restrict__ kc, uint8_t *__restrict__ vc, int *__restrict__ status) {                          \
-    attn::qk_norm_rope<E4M3>(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv,   \
-                             gq, gk, q, kc, vc, status);                                                       \
+    if constexpr (CACHE == attn::kCacheBlocks) {                                                               \
+      if (static_cast<int>(blockIdx.x) >= attn::desc_of(desc).max_tokens) {                                    \
+        attn::append_blocks(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv,    \
+                            gk, kc, vc, status);                                                               \
+        return;                                                                                                \
+      }                                                                                                        \
+    }                                                                                                          \
+    attn::qk_norm_rope<CACHE>(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv,  \
+                              gq, gk, q, kc, vc, status);                                                      \
   }
-LF_ATTN_ROPE(bf16, false)
-LF_ATTN_ROPE(e4m3, true)
+LF_ATTN_ROPE(bf16, attn::kCacheBf16)
+LF_ATTN_ROPE(e4m3, attn::kCacheE4m3)
+LF_ATTN_ROPE(e4m3_blocks, attn::kCacheBlocks)
 
-#define LF_ATTN_DECODE(D, TYPE, E4M3)                                                                          \
+#define LF_ATTN_DECODE(D, TYPE, ...)                                                                           \
   extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void lf_attn_decode_d##D##_##TYPE(            \
       const int32_t *__restrict__ counts, const int32_t *__restrict__ row_offsets,                             \
       const int32_t *__restrict__ lengths, const int32_t *__restrict__ page_offsets,                           \
       const int32_t *__restrict__ page_indices, const uint8_t *__restrict__ desc,                              \
       const uint16_t *__restrict__ q, uint16_t *__restrict__ out, const uint8_t *__restrict__ kc,              \
       const uint8_t *__restrict__ vc, uint8_t *__restrict__ ws) {                                              \
-    attn::decode<D, E4M3>(counts, row_offsets, lengths, page_offsets, page_indices, desc, q, out, kc, vc, ws); \
+    attn::decode<D, __VA_ARGS__>(counts, row_offsets, lengths, page_offsets, page_indices, desc, q, out, kc,   \
+                                 vc, ws);                                                                      \
   }
-LF_ATTN_DECODE(64, bf16, false)
-LF_ATTN_DECODE(128, bf16, false)
-LF_ATTN_DECODE(256, bf16, false)
-LF_ATTN_DECODE(64, e4m3, true)
-LF_ATTN_DECODE(128, e4m3, true)
-LF_ATTN_DECODE(256, e4m3, true)
+LF_ATTN_DECODE(64, bf16, false, false, false)
+LF_ATTN_DECODE(128, bf16, false, false, false)
+LF_ATTN_DECODE(256, bf16, false, false, false)
+LF_ATTN_DECODE(64, e4m3, true, false, false)
+LF_ATTN_DECODE(128, e4m3, true, false, false)
+LF_ATTN_DECODE(256, e4m3, true, false, false)
+LF_ATTN_DECODE(64, bf16_sinks, false, false, true)
+LF_ATTN_DECODE(128, bf16_sinks, false, false, true)
+LF_ATTN_DECODE(256, bf16_sinks, false, false, true)
+LF_ATTN_DECODE(64, e4m3_sinks, true, false, true)
+LF_ATTN_DECODE(128, e4m3_sinks, true, false, true)
+LF_ATTN_DECODE(256, e4m3_sinks, true, false, true)
+LF_ATTN_DECODE(64, e4m3_blocks, true, true, true)
+LF_ATTN_DECODE(128, e4m3_blocks, true, true, true)
+LF_ATTN_DECODE(256, e4m3_blocks, true, true, true)

@@ -18,8 +18,22 @@ struct Desc {
   int32_t reserved;
   int64_t page_stride, head_stride, token_stride;
   int64_t scale_offset, turns_offset, axis_offset, region_bytes;
+  int32_t sinks, block_tokens;
+  int64_t block_scales;
 };
 constexpr uint32_t kMagic = 0x4E54414Cu;
+constexpr int kCacheBf16 = 1, kCacheE4m3 = 2, kCacheBlocks = 3;
+
+// A block of a cache with a scale per block and head: 8 or 16 tokens of one page.
+// Index of its scale in the table behind a cache's codes.
+LF_DEVICE int block_shift(const Desc &d) { return d.block_tokens == 8 ? 3 : 4; }
+LF_DEVICE uint64_t scale_index(const Desc &d, int page, int slot, int head) {
+  const int shift = block_shift(d);
+  return (static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(d.page_size >> shift) +
+          static_cast<uint32_t>(slot >> shift)) *
+             static_cast<uint32_t>(d.kv_heads) +
+         static_cast<uint32_t>(head);
+}
 
 // A sequence's entries [first, end) of the page table; none where they leave it.
 struct Pages {
@@ -61,6 +75,41 @@ LF_DEVICE Place place_of(const Desc &d, const int32_t *row_offsets, const int32_
   return {page, static_cast<int>(token & (d.page_size - 1))};
 }
 
+// Rows of a step that one sequence has, with what is cached before them; none where the
+// step contradicts itself or leaves its bounds (rows: the step's live rows).
+struct Prompt {
+  int row, rows, before, entry;  // first row, their number, tokens before, first page table entry
+};
+LF_DEVICE Prompt prompt_of(const Desc &d, const int32_t *row_offsets, const int32_t *lengths,
+                           const int32_t *page_offsets, int s, int rows, bool &bad) {
+  const int r0 = row_offsets[s], r1 = row_offsets[s + 1], len = lengths[s];
+  const Pages pages = pages_of(d, page_offsets[s], page_offsets[s + 1], bad);
+  if (r0 < 0 || r1 < r0 || r1 > rows || len < r1 - r0 || len > pages.count * d.page_size) {
+    bad = true;
+    return {0, 0, 0, 0};
+  }
+  return {r0, r1 - r0, len - (r1 - r0), pages.first};
+}
+
+// Blocks of tokens with a scale of their own that the rows fall into.
+LF_DEVICE int blocks_of(const Desc &d, const Prompt &p) {
+  const int shift = block_shift(d);
+  return p.rows < 1 ? 0 : ((p.before + p.rows - 1) >> shift) - (p.before >> shift) + 1;
+}
+
+// The b-th of them: its first slot in its page, the slots [lo, hi) that rows are written
+// to, the row of the first, and the page table entry.
+struct Block {
+  int entry, slot, lo, hi, row;
+};
+LF_DEVICE Block block_of(const Desc &d, const Prompt &p, int b) {
+  const int shift = block_shift(d), first = ((p.before >> shift) + b) << shift;  // token
+  const int lo = first < p.before ? p.before - first : 0;
+  const int end = p.before + p.rows - first, hi = end < d.block_tokens ? end : d.block_tokens;
+  return {p.entry + (first >> __builtin_ctz(static_cast<uint32_t>(d.page_size))), first & (d.page_size - 1), lo, hi,
+          p.row + first + lo - p.before};
+}
+
 // ---- single-token attention -------------------------------------------------------
 
 constexpr int kTileKeys = 32;
@@ -83,6 +132,25 @@ LF_DEVICE Span span_of(const Desc &d, int len, Pages p, bool &bad) {
   return {first, end > first ? end - first : 1, lo, len};
 }
 
+// With sinks: the first `sink` keys count too. The tiles are those of the sinks, then
+// those of the window, without the ones between: tile t holds the keys from
+// kTileKeys (t, or t + first_tile - sink_tiles from sink_tiles on).
+struct SinkSpan {
+  Span span;
+  int sink, sink_tiles;
+};
+LF_DEVICE int sink_tiles_of(int sink, int first_tile, int tile_keys) {
+  const int t = (sink + tile_keys - 1) / tile_keys;
+  return t < first_tile ? t : first_tile;
+}
+LF_DEVICE SinkSpan sink_span_of(const Desc &d, int len, Pages p, bool &bad) {
+  SinkSpan s = {span_of(d, len, p, bad), 0, 0};
+  s.sink = d.sinks < s.span.lo ? d.sinks : s.span.lo;
+  s.sink_tiles = sink_tiles_of(s.sink, s.span.first_tile, kTileKeys);
+  s.span.tiles += s.sink_tiles;
+  return s;
+}
+
 // A key tile is four groups of eight keys, each in one page. The table entry of
 // the group that starts at key j, of a sequence whose keys that count are in the
 // entries [first, end), end > first: groups before and behind those (a released
@@ -91,6 +159,14 @@ LF_DEVICE Span span_of(const Desc &d, int len, Pages p, bool &bad) {
 LF_DEVICE int entry_of(int first, int end, int shift, int j) {
   const int e = j >> shift;
   return e < first ? first : e < end ? e : end - 1;
+}
+
+// With sinks, where the keys that count are in the entries [0, sink_end) and [first, end):
+// a group between takes the last of the sinks' (of the window's first, without sinks).
+LF_DEVICE int sink_entry_of(int sink_end, int first, int end, int shift, int j) {
+  const int e = j >> shift;
+  if (e >= first) return e < end ? e : end - 1;
+  return e < sink_end ? e : sink_end > 0 ? sink_end - 1 : first;
 }
 
 // Bytes, all in 64 bits (a page's or a token's step may be up to 2^31 - 1 of them):
@@ -190,5 +266,112 @@ LF_DEVICE int part_slot(int block, int begin, int share) { return 2 * block + (b
 // one first group and one later group start in a window of kGroup blocks.
 constexpr int kGroup = 32;
 LF_DEVICE int group_slot(int start, int first) { return 2 * (start / kGroup) + (start == first ? 1 : 0); }
+
+// ---- attention of prompts -------------------------------------------------------------
+
+// A block's query tile: `tokens` consecutive rows of a sequence with all `heads` query heads
+// of a key head, row-major (token, head) in the tile; where a group has more heads than the
+// tile has rows, one token with `heads` of them at a time, `subs` times.
+struct QueryTile {
+  int tokens, heads, subs;
+};
+LF_DEVICE QueryTile query_tile_of(const Desc &d, int tile_rows) {
+  const int group = d.query_heads / d.kv_heads;
+  if (group > tile_rows) return {1, tile_rows, (group + tile_rows - 1) / tile_rows};
+  return {tile_rows / group, group, 1};
+}
+
+// The step's pairs are (sequence, key head and part of its group, query tile), tiles
+// innermost. A pair weighs the keys that its tile sees, without their rounding to key tiles,
+// and kPairKeys for what it takes whatever its keys are: min(a + step x, cap) for tile x of a
+// sequence, so that sums over x have a closed form. The blocks take equal ranges of weight.
+constexpr int kPairKeys = 128;
+struct Weights {
+  int64_t a, step, cap;
+  int tiles;
+};
+LF_DEVICE Weights weights_of(const Desc &d, const QueryTile &q, const Prompt &p) {
+  Weights w;
+  w.tiles = (p.rows + q.tokens - 1) / q.tokens;
+  w.step = q.tokens;
+  w.a = static_cast<int64_t>(p.before) + q.tokens + kPairKeys;
+  w.cap = d.window > 0 ? static_cast<int64_t>(d.window) + d.sinks + q.tokens + kPairKeys : int64_t(1) << 40;
+  return w;
+}
+LF_DEVICE int64_t weight_of(const Weights &w, int x) {
+  const int64_t v = w.a + w.step * x;
+  return v < w.cap ? v : w.cap;
+}
+// Weight of the tiles before x.
+LF_DEVICE int64_t weight_before(const Weights &w, int x) {
+  int64_t rising = w.a < w.cap ? (w.cap - w.a + w.step - 1) / w.step : 0;
+  if (rising > x) rising = x;
+  return w.a * rising + w.step * (rising * (rising - 1) / 2) + w.cap * (x - rising);
+}
+// The tile in which weight r < weight_before(tiles) lies.
+LF_DEVICE int tile_at(const Weights &w, int64_t r) {
+  int lo = 0;
+  for (int hi = w.tiles; hi - lo > 1;) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (weight_before(w, mid) <= r) {
+      lo = mid;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
+}
+
+// The sequence that weight u of the step belongs to: prefix[i] (of n + 1) adds up the
+// weights of one head's tiles in the sequences before i, and each has `heads` of them.
+LF_DEVICE int prompt_at(const int64_t *prefix, int n, int64_t heads, int64_t u) {
+  int lo = 0;  // the last i with prefix[i] heads <= u, so one with tiles
+  for (int hi = n; hi - lo > 1;) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] * heads <= u) {
+      lo = mid;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
+}
+
+// Keys of query tile x: those of [lo, last] and the first `sink`; key tiles as those of a
+// SinkSpan, tile t from key tile_keys (t, or t + first - sink_tiles from sink_tiles on).
+struct PromptKeys {
+  int first_position, last;  // of the tile's rows
+  int lo, sink, sink_tiles, first, tiles;
+};
+LF_DEVICE PromptKeys keys_of(const Desc &d, const QueryTile &q, const Prompt &p, int x, int tile_keys) {
+  PromptKeys k;
+  const int from = x * q.tokens, rest = p.rows - from;
+  k.first_position = p.before + from;
+  k.last = k.first_position + (rest < q.tokens ? rest : q.tokens) - 1;
+  k.lo = d.window > 0 && k.first_position >= d.window ? k.first_position + 1 - d.window : 0;
+  k.sink = d.sinks < k.lo ? d.sinks : k.lo;
+  k.first = k.lo / tile_keys;
+  k.sink_tiles = sink_tiles_of(k.sink, k.first, tile_keys);
+  k.tiles = k.sink_tiles + k.last / tile_keys + 1 - k.first;
+  return k;
+}
+
+// Where weight u cuts a pair of [begin, begin + weight) with `tiles` key tiles: at a multiple
+// of kCut of them, so that no part is shorter (but a pair itself may be). Does not fall as u rises.
+constexpr int kCut = 8;
+LF_DEVICE int cut_of(int64_t u, int64_t begin, int64_t weight, int tiles) {
+  if (u <= begin) return 0;
+  if (u >= begin + weight) return tiles;
+  const int64_t k = ((u - begin) * tiles + weight / 2) / weight;
+  const int c = static_cast<int>((k + kCut / 2) / kCut * kCut);
+  return tiles - c < kCut ? tiles : c;
+}
+
+// Block b of the grid (as many blocks as CUs) takes the b-th range of weight of those with
+// the XCD in the upper bits: neighbours in weight, which share keys, share an XCD's L2.
+LF_DEVICE int range_of_block(int b, int blocks) { return (b & 7) * (blocks >> 3) + (b >> 3); }
+
+// Partial result of range b: of a pair cut before it, or of one that it begins and does not end.
+LF_DEVICE int prompt_slot(int b, bool begun_before) { return 2 * b + (begun_before ? 0 : 1); }
 
 }  // namespace attn

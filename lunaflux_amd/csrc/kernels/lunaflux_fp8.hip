@@ -5,5 +5,6 @@
 #include "w8a16_gemm.hip"
 #include "moe.hip"
 #include "attention.hip"
+#include "attention_prompt.hip"
 #include "low_rank.hip"
 #include "calibrate.hip"
