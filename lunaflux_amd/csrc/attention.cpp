@@ -129,14 +129,13 @@ int64_t decode_bytes(const lf_fp8_attn_desc *d) {
 }
 
 // kernels/attention_prompt.hip: query rows and keys of a block's tiles.
-int64_t prompt_rows(const lf_fp8_attn_desc *d) { return d->head_dim == 256 ? 128 : 256; }
+constexpr int64_t kPromptRows = 256;
 int64_t prompt_keys(const lf_fp8_attn_desc *d) { return d->head_dim == 256 ? 32 : 64; }
 
 // Whether a query tile can be cut: it has to have 2 kCut key tiles (attention_index.h).
 bool prompt_cuts(const lf_fp8_attn_desc *d) {
   int64_t longest = int64_t(d->table_entries) * d->page_size;
-  const int64_t rows = prompt_rows(d), group = d->query_heads / d->kv_heads;
-  const int64_t tokens = std::max<int64_t>(1, rows / group);
+  const int64_t tokens = std::max<int64_t>(1, kPromptRows / (d->query_heads / d->kv_heads));
   if (d->window > 0) longest = std::min(longest, int64_t(d->window) + tokens + d->sinks + 2 * prompt_keys(d));
   return (longest + prompt_keys(d) - 1) / prompt_keys(d) >= 2 * kCut;
 }
@@ -145,7 +144,7 @@ bool prompt_cuts(const lf_fp8_attn_desc *d) {
 // sums, maxima and weight sums).
 int64_t prompt_bytes(const lf_fp8_attn_desc *d) {
   return LF_FP8_ATTN_STATUS_BYTES +
-         (prompt_cuts(d) ? 2 * kPromptBlocks * prompt_rows(d) * (d->head_dim + 2) * 4 : 0);
+         (prompt_cuts(d) ? 2 * kPromptBlocks * kPromptRows * (d->head_dim + 2) * 4 : 0);
 }
 
 // Blocks that write an E4M3_BLOCKS cache: four heads' keys or values of one block of tokens each.
@@ -257,7 +256,7 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
   }
   dims[0] = static_cast<int32_t>(gx);
   dims[1] = dims[2] = dims[4] = dims[5] = 1;
-  dims[3] = static_cast<int32_t>(64 * kWaves);
+  dims[3] = static_cast<int32_t>(64 * (entry == LF_FP8_ATTN_PREFILL ? 2 * kWaves : kWaves));
   dims[6] = static_cast<int32_t>(lds);
   return LF_OK;
 }

@@ -10,18 +10,18 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // One pass over the keys with the running maximum and sum of each row's softmax. A block holds a
-// query tile (attention_index.h, QueryTile) of which each wave has kRowTiles tiles of 32 rows in
-// registers, as the B operand of S^T = K Q^T; that leaves a lane the scores of one row, so
-// its statistics are lane values, and 16 weights per 32 keys in the order of the B operand of
-// O^T = V^T P^T. Key and value tiles go through LDS, shared by the waves; values are read from it
-// transposed.
+// query tile (attention_index.h, QueryTile) of which each wave has 32 rows in registers, as the
+// B operand of S^T = K Q^T; that leaves a lane the scores of one row, so its statistics are
+// lane values, and 16 weights per 32 keys in the order of the B operand of O^T = V^T P^T. Key and
+// value tiles go through LDS, shared by the waves; values are read from it transposed.
+// The waves are two groups, one wave of each on every SIMD, half a tile apart: between two
+// barriers one group's waves have the products of a tile and the other's its softmax.
 // Blocks are dealt equal ranges of the step's weight (attention_index.h); a query tile cut
 // between ranges leaves fp32 partial results, which a second launch adds up in their order.
 template <int D>
 struct Prompts {
-  static constexpr int kWaves = 4, kBlocks = 256;
-  static constexpr int kRowTiles = D == 256 ? 1 : 2;
-  static constexpr int kRows = 32 * kRowTiles * kWaves;
+  static constexpr int kWaves = 8, kThreads = 64 * kWaves, kBlocks = 256;
+  static constexpr int kRows = 32 * kWaves;
   static constexpr int kKeys = D == 256 ? 32 : 64;
   static constexpr int kKeyTiles = kKeys / 32;
   static constexpr int kTileBytes = kKeys * D * 2;
@@ -36,10 +36,10 @@ struct PromptPlan {
   int64_t heads, total, share;  // heads: pairs of key head and part of its group
 };
 
-template <int D>
+template <int D, int THREADS>
 LF_DEVICE PromptPlan plan_of(const Desc &d, const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths,
                              const int32_t *page_offsets, int64_t *prefix, bool &bad) {
-  __shared__ int64_t wave_total[4], wave_rows[4];
+  __shared__ int64_t wave_total[THREADS / 64], wave_rows[THREADS / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   PromptPlan plan;
   plan.rows = live_rows(counts, d.max_tokens);
@@ -47,7 +47,7 @@ LF_DEVICE PromptPlan plan_of(const Desc &d, const int32_t *counts, const int32_t
   plan.tile = query_tile_of(d, Prompts<D>::kRows);
   plan.heads = static_cast<int64_t>(d.kv_heads) * plan.tile.subs;
   int64_t carry = 0, rows = 0;
-  for (int base = 0; base < plan.n; base += 256) {
+  for (int base = 0; base < plan.n; base += THREADS) {
     const int i = base + static_cast<int>(threadIdx.x);
     int64_t weight = 0;
     int mine = 0;
@@ -66,7 +66,7 @@ LF_DEVICE PromptPlan plan_of(const Desc &d, const int32_t *counts, const int32_t
     if (lane == 63) wave_total[wave] = sum, wave_rows[wave] = some;
     __syncthreads();
     int64_t before = carry;
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < THREADS / 64; ++k) {
       if (k < wave) before += wave_total[k];
       carry += wave_total[k];
       rows += wave_rows[k];
@@ -112,7 +112,11 @@ LF_DEVICE PromptPair pair_at(const Desc &d, const PromptPlan &plan, const int32_
   return pair;
 }
 
-LF_DEVICE uint32_t pack_bf16(float a, float b) { return f32_to_bf16(a) | (f32_to_bf16(b) << 16); }
+// One v_cvt_pk_bf16_f32, rounded to nearest even.
+LF_DEVICE uint32_t pack_bf16(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
 
 // Byte of 16-byte chunk `chunk` of a key's row in an LDS tile of rows of D bf16 values.
 template <int D>
@@ -120,27 +124,96 @@ LF_DEVICE uint32_t tile_byte(int key, int chunk) {
   return static_cast<uint32_t>(key * D * 2 + ((chunk ^ (chunk_swizzle(key & 15) & (D / 8 - 1))) << 4));
 }
 
-// A bf16 pair with an infinity or NaN among the two, and its values: finite ones kept and
-// others zero, or +infinity, -infinity, NaN as 1, 256, 65536 and finite ones zero.
-LF_DEVICE bool odd_half(uint32_t h) { return (h & 0x7f80u) == 0x7f80u; }
-LF_DEVICE uint32_t finite_pair(uint32_t w) {
-  return (odd_half(w) ? 0u : w & 0xffffu) | (odd_half(w >> 16) ? 0u : w & 0xffff0000u);
-}
-LF_DEVICE uint32_t odd_code(uint32_t h) {
-  return !odd_half(h) ? 0u : (h & 0x7fu) != 0 ? 0x4780u : (h & 0x8000u) != 0 ? 0x4380u : 0x3f80u;
-}
-LF_DEVICE uint32_t odd_pair(uint32_t w) { return odd_code(w & 0xffffu) | (odd_code(w >> 16) << 16); }
-LF_DEVICE bool odd_word(uint32_t w) { return odd_half(w) || odd_half(w >> 16); }
-
-LF_DEVICE u32x4 finite4(u32x4 w) {
-  return u32x4{finite_pair(w[0]), finite_pair(w[1]), finite_pair(w[2]), finite_pair(w[3])};
-}
-LF_DEVICE u32x4 odd4(u32x4 w) { return u32x4{odd_pair(w[0]), odd_pair(w[1]), odd_pair(w[2]), odd_pair(w[3])}; }
-
 // Partial results, their maxima and their weight sums in the workspace.
 template <int D>
 LF_DEVICE float *partial_of(uint8_t *ws, int slot) {
   return reinterpret_cast<float *>(ws + 256) + static_cast<uint64_t>(slot) * Prompts<D>::kFloats;
+}
+
+// One global_load_lds_dwordx4: every lane's 16 bytes from its address go to LDS at lds + 16 lane
+// (wave-uniform; M0). As assembly, so that the compiler does not make every LDS read wait for it:
+// the kernel orders it by itself, with vmcnt and barriers.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // M0 is listed as clobbered on purpose
+LF_DEVICE void load_to_lds(const uint8_t *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+LF_DEVICE uint32_t lds_at(const uint8_t *p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t *)p));
+}
+template <class T>
+LF_DEVICE T lds_read(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T *)at;
+}
+template <class T>
+LF_DEVICE void lds_write(uint32_t at, T v) {
+  *(__attribute__((address_space(3))) T *)at = v;
+}
+
+// The block's barrier between intervals: this wave's LDS accesses are over, and no instruction
+// moves past it. LOADS: its loads to LDS have arrived too.
+template <bool LOADS>
+LF_DEVICE void interval_end() {
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (LOADS) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  } else {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The rows of a query tile that one wave has, without the matrix units: for rows that some infinity or NaN
+// reached, since in products of tiles zero times such a value of a key that a row does not count is NaN
+// too. Here only the keys that it counts enter. Lanes c and c + 32 hold the halves of row c. Slow, and
+// apart from the kernel's registers.
+struct CarefulRow {
+  const uint16_t *q;
+  const uint8_t *kc, *vc;
+  const int32_t *table;
+  PromptKeys keys;
+  int k0, k1, h, position;
+  float factor;
+};
+template <int D, int CACHE>
+__device__ __attribute__((noinline)) void careful_row(const Desc &d, const CarefulRow &r, bool flip, float (&acc)[D / 2], float &top, float &sum) {
+  constexpr int kKeys = Prompts<D>::kKeys;
+  constexpr bool E4M3 = CACHE != kCacheBf16;
+  const int half = (threadIdx.x >> 5) & 1;
+  const int shift = __builtin_ctz(d.page_size), slot_mask = d.page_size - 1;
+  auto value = [&](const uint8_t *cache, int page, int slot, int e) {
+    const uint64_t at = cache_byte<E4M3>(d, page, r.h, slot);
+    if constexpr (E4M3) {
+      const float v = __builtin_amdgcn_cvt_f32_fp8(cache[at + e], 0);
+      return CACHE == kCacheBlocks ? v * reinterpret_cast<const float *>(cache + d.block_scales)[scale_index(d, page, slot, r.h)] : v;
+    } else {
+      return bf16_to_f32(*reinterpret_cast<const uint16_t *>(cache + at + 2 * e));
+    }
+  };
+  top = -INFINITY;
+  sum = 0.0f;
+  for (int e = 0; e < D / 2; ++e) acc[e] = 0.0f;
+  for (int t = r.k0; t < r.k1; ++t) {
+    const int base = kKeys * (t < r.keys.sink_tiles ? t : t + r.keys.first - r.keys.sink_tiles);
+    for (int j = base; j < base + kKeys && j <= r.keys.last; ++j) {
+      if (j >= r.keys.sink && j < r.keys.lo) continue;
+      const int page = r.table[j >> shift], slot = j & slot_mask;
+      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(d.pages)) continue;
+      float score = 0.0f;
+      for (int e = 0; e < D / 2; ++e) score += bf16_to_f32(r.q[half * (D / 2) + e]) * value(r.kc, page, slot, half * (D / 2) + e);
+      score += __shfl_xor(score, 32);
+      if (j > r.position || !(d.window == 0 || j > r.position - d.window || j < d.sinks)) continue;
+      const float z = (flip ? -score : score) * r.factor, next = fmaxf(top, z), from = next == -INFINITY ? 0.0f : next;
+      const float keep = __builtin_amdgcn_exp2f(top - from), p = __builtin_amdgcn_exp2f(z - from);
+      top = next;
+      sum = sum * keep + p;
+      for (int e = 0; e < D / 2; ++e) acc[e] = acc[e] * keep + fmaxf(p, 0x1p-126f) * value(r.vc, page, slot, half * (D / 2) + e);
+    }
+  }
 }
 
 template <int D, int CACHE>
@@ -148,28 +221,36 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
                        const int32_t *page_offsets, const int32_t *page_indices, const uint8_t *attn,
                        const uint16_t *q, uint16_t *out, const uint8_t *kc, const uint8_t *vc, uint8_t *ws) {
   using P = Prompts<D>;
-  constexpr int RT = P::kRowTiles, KT = P::kKeyTiles, kKeys = P::kKeys, kSteps = D / 16, kBands = D / 32;
+  constexpr int KT = P::kKeyTiles, kKeys = P::kKeys, kSteps = D / 16, kBands = D / 32;
   constexpr bool E4M3 = CACHE != kCacheBf16;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t stages[];
   const Desc &d = desc_of(attn);
   if (d.magic != kMagic) return;
   int *error = reinterpret_cast<int *>(ws);
-  int64_t *prefix = reinterpret_cast<int64_t *>(lds);
-  uint8_t *keys = lds + ((static_cast<uint32_t>(d.max_sequences) + 1) / 2 * 16 + 16), *values = keys + P::kTileBytes;
+  // stage i & 1: the keys of tile i and the values of tile i - 1; behind the stages the prefix of weights
+  int64_t *prefix = reinterpret_cast<int64_t *>(stages + 4 * P::kTileBytes);
+  const uint32_t stages_at = lds_at(stages);
+  auto keys_at = [&](int i) { return stages_at + (i & 1) * 2 * P::kTileBytes; };
+  auto values_at = [&](int i) { return stages_at + ((i + 1) & 1) * 2 * P::kTileBytes + P::kTileBytes; };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ int once_more;
+  const bool late = wave >= P::kWaves / 2;  // the group that is half a tile behind
   const int c = lane & 31, half = lane >> 5;
   bool bad = false;
-  const PromptPlan plan = plan_of<D>(d, counts, row_offsets, lengths, page_offsets, prefix, bad);
+  const PromptPlan plan = plan_of<D, P::kThreads>(d, counts, row_offsets, lengths, page_offsets, prefix, bad);
   const int range = range_of_block(blockIdx.x, P::kBlocks);
   const int64_t u0 = range * plan.share, u1 = u0 + plan.share < plan.total ? u0 + plan.share : plan.total;
   if (bad) flag_error(error);
   if (u0 >= u1) return;
 
   const int Hq = d.query_heads, Hkv = d.kv_heads, group = Hq / Hkv;
-  const int shift = __builtin_ctz(d.page_size), slot_mask = d.page_size - 1;
+  const int shift = __builtin_ctz(d.page_size), slot_mask = d.page_size - 1, pages = d.pages;
   const float *scales = reinterpret_cast<const float *>(attn + d.scale_offset);
   const bool flip = d.softmax_scale < 0.0f;
   const int window = d.window > 0 ? d.window : INT32_MAX, sinks = d.sinks;
+  constexpr uint32_t kSize = E4M3 ? 1 : 2;
+  const uint32_t page_bytes = static_cast<uint32_t>(d.page_stride) * kSize, token_bytes = static_cast<uint32_t>(d.token_stride) * kSize;
+  const uint32_t head_bytes = static_cast<uint32_t>(d.head_stride) * kSize;
 
   PromptPair pair = pair_at(d, plan, row_offsets, lengths, page_offsets, prefix, u0);
   for (;;) {
@@ -180,236 +261,351 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       const int tokens = pk.last - pk.first_position + 1;
       const int head0 = h * group + sub * plan.tile.heads;
       const int heads = group - sub * plan.tile.heads < plan.tile.heads ? group - sub * plan.tile.heads : plan.tile.heads;
-      const int live_rows_here = tokens * heads;
       const int row0 = pair.p.row + pair.x * plan.tile.tokens;
       const int32_t *table = page_indices + pair.p.entry;
+      const int page_first = pk.lo >> shift, page_end = (pk.last >> shift) + 1, sink_end = (pk.sink + slot_mask) >> shift;
       // (a scale of zero as one that leaves -infinity, a masked score, what it is)
       const float factor = fmaxf(fabsf(d.softmax_scale) * 1.44269504088896341f * (CACHE == kCacheE4m3 ? scales[h] : 1.0f), 0x1p-126f);
+      const int n = k1 - k0;
+      auto base_of = [&](int i) { return kKeys * (k0 + i < pk.sink_tiles ? k0 + i : k0 + i + pk.first - pk.sink_tiles); };
 
-      // this lane's rows: query operands, positions, statistics
-      u32x4 qv[RT][kSteps];
-      int position[RT];
-      uint32_t row_at[RT];  // row and head of q and out, or none
-      float top[RT], sum[RT];
-      f32x16 o[RT][kBands];
+      // Pages of a tile's groups of eight keys, in lanes of every eight; of those that are this wave's rows of a tile,
+      // kKeys / 8 of them, the page itself.
+      constexpr int kWaveKeys = kKeys / P::kWaves;
+      auto pages_of_tile = [&](int i) {
+        return table[sink_entry_of(sink_end, page_first, page_end, shift, base_of(i < n ? i : n - 1) + 8 * (lane & (kKeys / 8 - 1)))];
+      };
+      struct TilePages {
+        int page;
+        uint32_t outside;  // groups whose page the cache does not have
+      } tile_pages[3];     // of the tile whose keys are loaded next, and of those before
+      int loading;         // its successor's, on their way
+      auto arrived = [&]() {
+        const int p = __builtin_amdgcn_readlane(loading, wave * kWaveKeys / 8);
+        tile_pages[2] = tile_pages[1];
+        tile_pages[1] = tile_pages[0];
+        tile_pages[0] = {static_cast<uint32_t>(p) < static_cast<uint32_t>(pages) ? p : 0,
+                         static_cast<uint32_t>(__ballot(static_cast<uint32_t>(loading) >= static_cast<uint32_t>(pages))) & ((1u << (kKeys / 8)) - 1)};
+      };
+      auto slot_of = [&](int i, int key) {
+        const int j = base_of(i) + key;
+        return (j < pk.last ? j : pk.last) & slot_mask;
+      };
+      const uint8_t *head_keys = kc + static_cast<uint64_t>(static_cast<uint32_t>(h)) * head_bytes;
+      const uint8_t *head_values = vc + static_cast<uint64_t>(static_cast<uint32_t>(h)) * head_bytes;
+      auto load_tile = [&](const uint8_t *cache, uint32_t to, int i, int p) {  // bf16
+        constexpr int kChunks = D / 8, kRowsAtOnce = 64 / kChunks;
+        int l = lane;
+        asm volatile("" : "+v"(l));  // what follows from it is computed here, not kept
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const int m = (wave * RT + rt) * 32 + c;
-        const int token = m / heads, head = m - token * heads;
-        const bool live = m < live_rows_here;
-        position[rt] = live ? pk.first_position + token : pk.first_position;
-        row_at[rt] = live ? static_cast<uint32_t>(row0 + token) * Hq + head0 + head : ~0u;
-        const uint16_t *src = q + static_cast<uint64_t>(live ? row_at[rt] : static_cast<uint32_t>(row0) * Hq + head0) * D + 8 * half;
+        for (int r = 0; r < kWaveKeys; r += kRowsAtOnce) {
+          const int key = wave * kWaveKeys + r + l / kChunks, chunk = l & (kChunks - 1);
+          const int from = chunk ^ (chunk_swizzle(key & 15) & (kChunks - 1));
+          load_to_lds(cache + row_byte(p, slot_of(i, key), page_bytes, token_bytes) + 16 * from, to + (wave * kWaveKeys + r) * D * 2);
+        }
+      };
+      // e4m3: through registers, 16 codes of a row or 8.
+      constexpr int kCodes = kKeys * D / P::kThreads, kWords = kCodes / 4;
+      struct Codes {
+        uint32_t w[kWords];
+        float scale;
+      };
+      const int code_key = static_cast<int>(threadIdx.x) / (D / kCodes), code_at = static_cast<int>(threadIdx.x) % (D / kCodes);
+      auto load_codes = [&](const uint8_t *cache, const uint8_t *table_of, int i, int p, Codes &x) {
+        const int slot = slot_of(i, code_key);
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(cache + row_byte(p, slot, page_bytes, token_bytes) + kCodes * code_at);
+        if constexpr (kWords == 4) {
+          const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x.w[e] = w[e];
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2 *>(src);
+          x.w[0] = w.x;
+          x.w[1] = w.y;
+        }
+        x.scale = 1.0f;
+        if constexpr (CACHE == kCacheBlocks) x.scale = reinterpret_cast<const float *>(table_of + d.block_scales)[scale_index(d, p, slot, h)];
+      };
+      auto store_codes = [&](uint32_t to, const Codes &x) {
+        uint32_t b[2 * kWords];
+#pragma unroll
+        for (int e = 0; e < kWords; ++e) {
+          b[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(x.w[e]), x.scale, false));
+          b[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(x.w[e]), x.scale, true));
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * kWords; e += 4)
+          lds_write(to + tile_byte<D>(code_key, (kCodes * code_at + 2 * e) / 8), u32x4{b[e], b[e + 1], b[e + 2], b[e + 3]});
+      };
+      Codes next_keys, next_values;
+      // Begins to load stage i, and for e4m3 stores it.
+      auto load_stage = [&](int i) {
+        if (i < n) {
+          if constexpr (E4M3) {
+            load_codes(head_keys, kc, i, tile_pages[0].page, next_keys);
+          } else {
+            load_tile(head_keys, keys_at(i), i, tile_pages[0].page);
+          }
+        }
+        if (i > 0 && i <= n) {
+          if constexpr (E4M3) {
+            load_codes(head_values, vc, i - 1, tile_pages[1].page, next_values);
+          } else {
+            load_tile(head_values, values_at(i - 1), i - 1, tile_pages[1].page);
+          }
+        }
+        loading = pages_of_tile(i + 1);
+      };
+      auto store_stage = [&](int i) {
+        if constexpr (E4M3) {
+          if (i < n) store_codes(keys_at(i), next_keys);
+          if (i > 0 && i <= n) store_codes(values_at(i - 1), next_values);
+        }
+      };
+
+      // this lane's row: query operand, position, statistics
+      u32x4 qv[kSteps];
+      const int m = wave * 32 + c, token = m / heads, head = m - token * heads;
+      const bool live = m < tokens * heads;
+      const int position = live ? pk.first_position + token : pk.first_position;
+      const uint32_t row_at = static_cast<uint32_t>(live ? row0 + token : row0) * Hq + head0 + (live ? head : 0);
+      {
+        const uint16_t *src = q + static_cast<uint64_t>(row_at) * D + 8 * half;
 #pragma unroll
         for (int t = 0; t < kSteps; ++t) {
           u32x4 w = *reinterpret_cast<const u32x4 *>(src + 16 * t);
           if (flip) w ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-          qv[rt][t] = w;
+          qv[t] = w;
         }
-        top[rt] = -INFINITY;
-        sum[rt] = 0.0f;
+      }
+      // Weights are relative to `top`, the row's maximum in the first tile that it counts a key of. It need not be
+      // the row's largest score, only near it: nothing is lost until one is 2^kNear larger. Then the tiles
+      // are gone through once more, with the largest that was seen. So the sums are never scaled.
+      constexpr float kNear = 40.0f;
+      float top = -INFINITY, seen = -INFINITY, sum;
+      f32x16 o[kBands];
+      do {
+      loading = pages_of_tile(0);
+      arrived();
+      load_stage(0);
+      top = seen;
+      sum = 0.0f;
+#pragma unroll
+      for (int b = 0; b < kBands; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+      store_stage(0);
+      arrived();
+      load_stage(1);
+      store_stage(1);
+      interval_end<true>();
+      if (late) arrived();
+      if (threadIdx.x == 0) once_more = 0;  // every wave has read it by now
+      if (late) interval_end<false>();
+
+      u32x4 weights[2 * KT];
+      f32x16 s[KT];
+      // This lane's place in a tile of keys (key c of 32, chunk `half`) and in one of values (key 4 half + .. of
+      // 16, its columns of 32). Other chunks and columns are the place with bits of it flipped, other keys are
+      // further on by a constant, so that a tile's reads share a few addresses.
+      const int l16 = lane & 15, value_key = 4 * half + (l16 >> 2), value_column = 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
+      const uint32_t key_place = tile_byte<D>(c, half), value_place = tile_byte<D>(value_key, value_column / 8) + (value_column % 8) * 2;
+      auto key_words = [&](uint32_t at, int st, int kt) { return lds_read<u32x4>((at ^ (st << 5)) + kt * 32 * D * 2); };
+      // values of keys 16 kk + 4 half + 0 .. 3 and of those 8 further, column 32 b + lane % 32
+      auto value_words = [&](uint32_t at, int kk, int b) {
+        const uint32_t band = at ^ (b << 6);
+        typedef __attribute__((address_space(3))) s16x4 *LdsWords;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)(band + kk * 16 * D * 2));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)((band ^ 32) + (kk * 16 + 8) * D * 2));
+        const uint2 w0 = __builtin_bit_cast(uint2, lo), w1 = __builtin_bit_cast(uint2, hi);
+        return u32x4{w0.x, w0.y, w1.x, w1.y};
+      };
+      auto is_masked = [&](int from, uint32_t outer) {  // some row of the tile does not count some key
+        return from + kKeys - 1 > pk.first_position || outer != 0 || (from <= pk.last - window && from + kKeys > sinks);
+      };
+      auto product = [&](u32x4 a, u32x4 b, f32x16 acc) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+      };
+      // Products of an interval: V^T P^T of tile i - 1 onto O^T (VALUES), then K Q^T of tile i (SCORES). Operands are
+      // read from LDS two steps of kBands products ahead.
+      auto products = [&](int i, auto with_values, auto with_scores) {
+        constexpr bool VALUES = decltype(with_values)::value, SCORES = decltype(with_scores)::value;
+        constexpr int kValueSteps = VALUES ? 2 * KT : 0, kAhead = 2;
+        uint32_t value_at = VALUES ? values_at(i - 1) + value_place : 0, key_at = SCORES ? keys_at(i) + key_place : 0;
+        asm volatile("" : "+v"(value_at), "+v"(key_at));  // or every address of both stages stays in a register
+        u32x4 v[kAhead][kBands], k[kAhead][KT];
+        if constexpr (VALUES) {
+#pragma unroll
+          for (int kk = 0; kk < kAhead; ++kk)
+#pragma unroll
+            for (int b = 0; b < kBands; ++b) v[kk][b] = value_words(value_at, kk, b);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead * kBands, 0);
+#pragma unroll
+          for (int kk = 0; kk < kValueSteps; ++kk) {
+#pragma unroll
+            for (int b = 0; b < kBands; ++b) {
+              o[b] = product(v[kk % kAhead][b], weights[kk], o[b]);
+              if (kk + kAhead < kValueSteps) v[kk % kAhead][b] = value_words(value_at, kk + kAhead, b);
+            }
+          }
+        }
+        if constexpr (SCORES) {
+#pragma unroll
+          for (int st = 0; st < kAhead; ++st)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) k[st][kt] = key_words(key_at, st, kt);
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              s[kt] = product(k[st % kAhead][kt], qv[st], s[kt]);
+              if (st + kAhead < kSteps) k[st % kAhead][kt] = key_words(key_at, st + kAhead, kt);
+            }
+        }
+        // the order: after the first reads, a product, then the reads that its operands' registers are free for
+#pragma unroll
+        for (int kk = 0; kk < kValueSteps; ++kk)
+#pragma unroll
+          for (int b = 0; b < kBands; ++b) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (kk + kAhead < kValueSteps) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            else if (SCORES && (kk + kAhead - kValueSteps) * kBands + b < kAhead * KT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
+        if constexpr (SCORES) {
+          if constexpr (!VALUES) __builtin_amdgcn_sched_group_barrier(0x100, kAhead * KT, 0);
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              if (st + kAhead < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        }
+      };
+      constexpr std::true_type kYes{};
+      constexpr std::false_type kNo{};
+      auto softmax = [&](int i) {
+        const int base = base_of(i);
+        const uint32_t out_of_cache = tile_pages[late ? 2 : 1].outside;
+        float z[16 * KT];
+#pragma unroll
+        for (int e = 0; e < 16 * KT; ++e) z[e] = s[e / 16][e % 16];
+        if (out_of_cache != 0) bad = true;
+        if (is_masked(base, out_of_cache)) {
+          // the row counts keys low < j <= position and j < sinks (no short circuits: each would be a branch)
+          const int to = position - base - 4 * half, low = to - window, sink = sinks - base - 4 * half;
+#pragma unroll
+          for (int e = 0; e < 16 * KT; ++e) {
+            const int j = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3);
+            const bool counts = (j <= to) & ((j > low) | (j < sink)) & (((out_of_cache >> (j >> 3)) & 1) == 0);
+            z[e] = counts ? z[e] : -INFINITY;
+          }
+        }
+        float most = z[0];
+#pragma unroll
+        for (int e = 1; e < 16 * KT; ++e) most = fmaxf(most, z[e]);
+        {
+          const uint32_t a = __float_as_uint(most);
+          const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+          most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * factor;
+        }
+        seen = fmaxf(seen, most);
+        top = top == -INFINITY ? most : top;
+        const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int e = 0; e < 8 * KT; ++e) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e], factor, -from));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e + 1], factor, -from));
+          const uint32_t w = pack_bf16(p0, p1);
+          weights[e / 4][e % 4] = w;
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * KT; ++e) asm volatile("" : "+v"(weights[e]));  // here, not with the products
+      };
+      // Intervals of this wave: products of tile i (and of tile i - 1's values), softmax of tile i. The
+      // first group's loads of stage i + 1 last from its i-th products on, the second's from the softmax before.
+      products(0, kNo, kYes);
+      interval_end<false>();
+      for (int i = 0; i < n;) {
+        if (late) load_stage(i + 2);
+        softmax(i);
+        if (late) {
+          interval_end<false>();
+        } else {
+          if (i > 0) store_stage(i + 1);
+          interval_end<true>();
+          arrived();
+        }
+        ++i;
+        if (!late) load_stage(i + 1);
+        products(i, kYes, kYes);  // behind the last tile's values, scores of no use
+        if (late) {
+          store_stage(i + 1);
+          interval_end<true>();
+          arrived();
+        } else {
+          interval_end<false>();
+        }
+      }
+      if (!late) interval_end<false>();
+      if (__ballot(live && seen > top + kNear) != 0 && lane == 0) once_more = 1;
+      interval_end<false>();
+      } while (__builtin_amdgcn_readfirstlane(once_more) != 0);
+
+      const uint32_t sum_bits = __float_as_uint(sum);
+      const auto both = __builtin_amdgcn_permlane32_swap(sum_bits, sum_bits, false, false);
+      const float total = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+      const bool whole = k0 == 0 && k1 == pk.tiles;
+      const float scale = whole ? (CACHE == kCacheE4m3 ? scales[Hkv + h] : 1.0f) / total : 1.0f;
+      uint16_t *dst = out + static_cast<uint64_t>(row_at) * D;
+      float *part = partial_of<D>(ws, prompt_slot(range, k0 > 0));
+      float finite = total;  // a NaN once a value is not: x - x is then
+#pragma unroll
+      for (int b = 0; b < kBands; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) finite += o[b][e] - o[b][e];
+      if (live && whole) {
 #pragma unroll
         for (int b = 0; b < kBands; ++b)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[rt][b][i] = 0.0f;
-      }
-
-      const int page_first = pk.lo >> shift, page_end = (pk.last >> shift) + 1, sink_end = (pk.sink + slot_mask) >> shift;
-      for (int t = k0; t < k1; ++t) {
-        const int base = kKeys * (t < pk.sink_tiles ? t : t + pk.first - pk.sink_tiles);
-        // pages of the tile's groups of eight keys
-        int page = 0;
-        bool in = true;
-        if (lane < kKeys / 8) {
-          page = table[sink_entry_of(sink_end, page_first, page_end, shift, base + 8 * lane)];
-          in = static_cast<uint32_t>(page) < static_cast<uint32_t>(d.pages);
-          page = in ? page : 0;
+          for (int e = 0; e < 16; e += 4) {
+            uint2 w = {pack_bf16(o[b][e] * scale, o[b][e + 1] * scale), pack_bf16(o[b][e + 2] * scale, o[b][e + 3] * scale)};
+            if (total == 0.0f) w = {0u, 0u};
+            *reinterpret_cast<uint2 *>(dst + 32 * b + 2 * e + 4 * half) = w;
+          }
+      } else if (live) {
+#pragma unroll
+        for (int b = 0; b < kBands; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<f32x4 *>(part + m * D + 32 * b + 2 * e + 4 * half) = f32x4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]};
+        if (half == 0) {
+          part[P::kRows * D + m] = top;
+          part[P::kRows * D + P::kRows + m] = total;
         }
-        const uint32_t outside = static_cast<uint32_t>(__ballot(!in));
-        if (outside != 0) bad = true;
-        constexpr int kChunks = D * (E4M3 ? 1 : 2) / 16;  // 16-byte chunks of a key in the cache
-        bool odd = false;
-        __syncthreads();  // the tile before has been read
-        for (int side = 0; side < 2; ++side) {
-#pragma unroll
-          for (int i = 0; i < kKeys * kChunks / 256; ++i) {
-            const int id = i * 256 + static_cast<int>(threadIdx.x), key = id / kChunks, chunk = id % kChunks;
-            const int p = __shfl(page, key >> 3);
-            const int j = base + key < pk.last ? base + key : pk.last, slot = j & slot_mask;
-            const uint8_t *src = (side == 0 ? kc : vc) + cache_byte<E4M3>(d, p, h, slot) + 16 * chunk;
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
-            uint8_t *dst = side == 0 ? keys : values;
-            if constexpr (E4M3) {
-              float scale = 1.0f;
-              if constexpr (CACHE == kCacheBlocks) {
-                scale = reinterpret_cast<const float *>((side == 0 ? kc : vc) + d.block_scales)[scale_index(d, p, slot, h)];
-              }
-              uint32_t b[8];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                b[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w[e]), scale, false));
-                b[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w[e]), scale, true));
-                odd |= odd_word(b[2 * e]) | odd_word(b[2 * e + 1]);
-              }
-              *reinterpret_cast<u32x4 *>(dst + tile_byte<D>(key, 2 * chunk)) = u32x4{b[0], b[1], b[2], b[3]};
-              *reinterpret_cast<u32x4 *>(dst + tile_byte<D>(key, 2 * chunk + 1)) = u32x4{b[4], b[5], b[6], b[7]};
+      }
+      if (__ballot(live && !(finite < INFINITY)) != 0) {
+        const CarefulRow r = {q + static_cast<uint64_t>(row_at) * D, kc, vc, table, pk, k0, k1, h, position, factor};
+        float acc[D / 2], careful_top, careful_sum;
+        careful_row<D, CACHE>(d, r, flip, acc, careful_top, careful_sum);
+        if (live) {
+          for (int e = 0; e < D / 2; ++e) {
+            const int column = half * (D / 2) + e;
+            if (whole) {
+              const float v = acc[e] * ((CACHE == kCacheE4m3 ? scales[Hkv + h] : 1.0f) / careful_sum);
+              dst[column] = static_cast<uint16_t>(careful_sum == 0.0f ? 0u : f32_to_bf16(v));
             } else {
-              odd |= odd_word(w[0]) | odd_word(w[1]) | odd_word(w[2]) | odd_word(w[3]);
-              *reinterpret_cast<u32x4 *>(dst + tile_byte<D>(key, chunk)) = w;
+              part[m * D + column] = acc[e];
             }
           }
-        }
-        odd = __syncthreads_or(odd) != 0;
-
-        // whether the row at `at` counts the tile's key `within` (no short circuits: each would be a branch)
-        auto counts_key = [&](int at, int within) {
-          const int j = base + within, low = at - window;
-          return static_cast<int>(j <= at) & (static_cast<int>(j > low) | static_cast<int>(j < sinks)) &
-                 static_cast<int>(((outside >> (within >> 3)) & 1) == 0);
-        };
-        const bool masked = base + kKeys - 1 > pk.first_position || outside != 0 ||
-                            (base <= pk.last - window && base + kKeys > sinks);
-        f32x16 s[RT][KT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[rt][kt][i] = 0.0f;
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            const bf16x8 a = *reinterpret_cast<const bf16x8 *>(keys + tile_byte<D>(32 * kt + c, 2 * st + half));
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              s[rt][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, qv[rt][st]), s[rt][kt], 0, 0, 0);
-          }
-        }
-        u32x4 weights[RT][2 * KT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          if (masked) {
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                s[rt][kt][i] = counts_key(position[rt], 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3)) != 0 ? s[rt][kt][i] : -INFINITY;
-              }
-          }
-          float most = s[rt][0][0];
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[rt][kt][i]);
-          {
-            const uint32_t a = __float_as_uint(most);
-            const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-            most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-          }
-          const float next = fmaxf(top[rt], most * factor), from = next == -INFINITY ? 0.0f : next;
-          const float shrink = __builtin_amdgcn_exp2f(top[rt] - from);
-          top[rt] = next;
-          sum[rt] *= shrink;
-#pragma unroll
-          for (int b = 0; b < kBands; ++b) o[rt][b] *= shrink;
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][kt][2 * i], factor, -from));
-              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][kt][2 * i + 1], factor, -from));
-              const uint32_t w = pack_bf16(p0, p1);
-              weights[rt][2 * kt + i / 4][i % 4] = w;
-              sum[rt] += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
-            }
-          }
-        }
-        // values of keys 16 kk + 4 half + 0 .. 3 and of those 8 further, column 32 b + lane % 32
-        auto values_at = [&](int kk, int b) {
-          const int l16 = lane & 15, key = 16 * kk + 4 * half + (l16 >> 2);
-          const int column = 32 * b + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
-          typedef __attribute__((address_space(3))) s16x4 *LdsWords;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)(values + tile_byte<D>(key, column / 8) + (column % 8) * 2));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)(values + tile_byte<D>(key + 8, column / 8) + (column % 8) * 2));
-          const uint2 w0 = __builtin_bit_cast(uint2, lo), w1 = __builtin_bit_cast(uint2, hi);
-          return u32x4{w0.x, w0.y, w1.x, w1.y};
-        };
-        if (odd) {
-          // Infinities and NaN among the values: a row that does not count their key, or gives it a weight that
-          // is zero in fp32, would take zero times those, which is NaN. Products of zeros and ones count the infinities and NaN that a row does count; they go to
-          // its sum by themselves, and the tile keeps its finite values.
-#pragma unroll
-          for (int b = 0; b < kBands; ++b)
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              f32x16 found;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) found[i] = 0.0f;
-#pragma unroll 1
-              for (int kk = 0; kk < 2 * KT; ++kk) {
-                uint32_t seen[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int within = 16 * kk + 8 * (i >> 1) + 4 * half + 2 * (i & 1);
-                  seen[i] = 0x3f80u * counts_key(position[rt], within) + 0x3f800000u * counts_key(position[rt], within + 1);
-                }
-                found = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, odd4(values_at(kk, b))),
-                                                                __builtin_bit_cast(bf16x8, u32x4{seen[0], seen[1], seen[2], seen[3]}), found, 0, 0, 0);
-              }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int n = static_cast<int>(found[i]), plus = n & 255, minus = (n >> 8) & 255;
-                if (n != 0) o[rt][b][i] += n >= 65536 || (plus != 0 && minus != 0) ? __builtin_nanf("") : plus != 0 ? INFINITY : -INFINITY;
-              }
-            }
-          __syncthreads();
-          for (int i = threadIdx.x; i < P::kTileBytes / 16; i += 256) {
-            u32x4 *w = reinterpret_cast<u32x4 *>(values) + i;
-            *w = finite4(*w);
-          }
-          __syncthreads();
-        }
-#pragma unroll
-        for (int b = 0; b < kBands; ++b) {
-#pragma unroll
-          for (int kk = 0; kk < 2 * KT; ++kk) {
-            const bf16x8 a = __builtin_bit_cast(bf16x8, values_at(kk, b));
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              o[rt][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, weights[rt][kk]), o[rt][b], 0, 0, 0);
-          }
-        }
-      }
-
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const uint32_t a = __float_as_uint(sum[rt]);
-        const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-        const float total = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-        if (row_at[rt] == ~0u) continue;
-        if (k0 == 0 && k1 == pk.tiles) {
-          const float scale = (CACHE == kCacheE4m3 ? scales[Hkv + h] : 1.0f) / total;
-          uint16_t *dst = out + static_cast<uint64_t>(row_at[rt]) * D + 4 * half;
-#pragma unroll
-          for (int b = 0; b < kBands; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              uint2 w = {pack_bf16(o[rt][b][i] * scale, o[rt][b][i + 1] * scale), pack_bf16(o[rt][b][i + 2] * scale, o[rt][b][i + 3] * scale)};
-              if (total == 0.0f) w = {0u, 0u};
-              *reinterpret_cast<uint2 *>(dst + 32 * b + 2 * i) = w;
-            }
-        } else {
-          float *part = partial_of<D>(ws, prompt_slot(range, k0 > 0));
-          const int m = (wave * RT + rt) * 32 + c;
-#pragma unroll
-          for (int b = 0; b < kBands; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<f32x4 *>(part + m * D + 32 * b + 2 * i + 4 * half) = f32x4{o[rt][b][i], o[rt][b][i + 1], o[rt][b][i + 2], o[rt][b][i + 3]};
-          if (half == 0) {
-            part[P::kRows * D + m] = top[rt];
-            part[P::kRows * D + P::kRows + m] = total;
+          if (!whole && half == 0) {
+            part[P::kRows * D + m] = careful_top;
+            part[P::kRows * D + P::kRows + m] = careful_sum;
           }
         }
       }
@@ -444,7 +640,7 @@ LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, c
   if (d.magic != kMagic) return;
   int64_t *prefix = reinterpret_cast<int64_t *>(lds);
   bool bad = false;  // reported by the launch before
-  const PromptPlan plan = plan_of<D>(d, counts, row_offsets, lengths, page_offsets, prefix, bad);
+  const PromptPlan plan = plan_of<D, 256>(d, counts, row_offsets, lengths, page_offsets, prefix, bad);
   const int range = blockIdx.x / kJoinSlices, slice = blockIdx.x % kJoinSlices;
   const int64_t u = range * plan.share;
   if (range == 0 || u >= plan.total) return;
@@ -506,7 +702,7 @@ LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, c
 }  // namespace attn
 
 #define LF_ATTN_PREFILL(D, TYPE, CACHE)                                                                        \
-  extern "C" __global__ __launch_bounds__(256, 1) void lf_attn_prefill_d##D##_##TYPE(                          \
+  extern "C" __global__ __launch_bounds__(512, 2) void lf_attn_prefill_d##D##_##TYPE(                          \
       const int32_t *__restrict__ counts, const int32_t *__restrict__ row_offsets,                             \
       const int32_t *__restrict__ lengths, const int32_t *__restrict__ page_offsets,                           \
       const int32_t *__restrict__ page_indices, const uint8_t *__restrict__ desc,                              \

@@ -106,7 +106,7 @@ static void entries_of(const Desc &d, const Prompt &p, const PromptKeys &k, int 
 static void hostile() {
   const Desc d = desc();
   const Step s = garbage(d);
-  const int tile_rows = d.head_dim == 256 ? 128 : 256, tile_keys = d.head_dim == 256 ? 32 : 64;
+  const int tile_rows = 256, tile_keys = d.head_dim == 256 ? 32 : 64;
   const QueryTile q = query_tile_of(d, tile_rows);
   for (int i = 0; i < s.n; ++i) {
     bool bad = false;
@@ -172,7 +172,7 @@ static void cut(int blocks) {
   Desc d = desc();
   d.table_entries = pick(1, 1000);
   const Step s = sound(d);
-  const int tile_rows = d.head_dim == 256 ? 128 : 256, tile_keys = d.head_dim == 256 ? 32 : 64;
+  const int tile_rows = 256, tile_keys = d.head_dim == 256 ? 32 : 64;
   const QueryTile q = query_tile_of(d, tile_rows);
   const int64_t heads = int64_t(d.kv_heads) * q.subs;
   CHECK(q.heads * q.tokens <= tile_rows && q.heads * q.subs >= d.query_heads / d.kv_heads);
