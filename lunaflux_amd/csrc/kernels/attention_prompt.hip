@@ -399,9 +399,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       load_stage(1);
       store_stage(1);
       interval_end<true>();
-      if (late) arrived();
       if (threadIdx.x == 0) once_more = 0;  // every wave has read it by now
-      if (late) interval_end<false>();
 
       u32x4 weights[2 * KT];
       f32x16 s[KT];
@@ -488,9 +486,9 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       };
       constexpr std::true_type kYes{};
       constexpr std::false_type kNo{};
-      auto softmax = [&](int i) {
+      auto softmax = [&](int i, const TilePages &of) {
         const int base = base_of(i);
-        const uint32_t out_of_cache = tile_pages[late ? 2 : 1].outside;
+        const uint32_t out_of_cache = of.outside;
         float z[16 * KT];
 #pragma unroll
         for (int e = 0; e < 16 * KT; ++e) z[e] = s[e / 16][e % 16];
@@ -527,32 +525,45 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
 #pragma unroll
         for (int e = 0; e < 2 * KT; ++e) asm volatile("" : "+v"(weights[e]));  // here, not with the products
       };
-      // Intervals of this wave: products of tile i (and of tile i - 1's values), softmax of tile i. The
-      // first group's loads of stage i + 1 last from its i-th products on, the second's from the softmax before.
-      products(0, kNo, kYes);
-      interval_end<false>();
-      for (int i = 0; i < n;) {
-        if (late) load_stage(i + 2);
-        softmax(i);
-        if (late) {
-          interval_end<false>();
-        } else {
-          if (i > 0) store_stage(i + 1);
-          interval_end<true>();
+      // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. Both
+      // groups load a stage between the same two barriers, in which the first has products and the second a
+      // softmax. (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
+      auto tiles = [&](auto behind) {
+        constexpr bool LATE = decltype(behind)::value;
+        if constexpr (LATE) {
           arrived();
-        }
-        ++i;
-        if (!late) load_stage(i + 1);
-        products(i, kYes, kYes);  // behind the last tile's values, scores of no use
-        if (late) {
-          store_stage(i + 1);
-          interval_end<true>();
-          arrived();
-        } else {
           interval_end<false>();
         }
+        products(0, kNo, kYes);
+        interval_end<false>();
+        for (int i = 0; i < n;) {
+          if constexpr (LATE) load_stage(i + 2);
+          softmax(i, tile_pages[LATE ? 2 : 1]);
+          if constexpr (LATE) {
+            interval_end<false>();
+          } else {
+            if (i > 0) store_stage(i + 1);
+            interval_end<true>();
+            arrived();
+          }
+          ++i;
+          if constexpr (!LATE) load_stage(i + 1);
+          products(i, kYes, kYes);  // behind the last tile's values, scores of no use
+          if constexpr (LATE) {
+            store_stage(i + 1);
+            interval_end<true>();
+            arrived();
+          } else {
+            interval_end<false>();
+          }
+        }
+        if constexpr (!LATE) interval_end<false>();
+      };
+      if (late) {
+        tiles(kYes);
+      } else {
+        tiles(kNo);
       }
-      if (!late) interval_end<false>();
       if (__ballot(live && seen > top + kNear) != 0 && lane == 0) once_more = 1;
       interval_end<false>();
       } while (__builtin_amdgcn_readfirstlane(once_more) != 0);
