@@ -425,63 +425,51 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
       };
       // Products of an interval: V^T P^T of tile i - 1 onto O^T (VALUES), then K Q^T of tile i (SCORES). Operands are
-      // read from LDS two steps of kBands products ahead.
+      // read from LDS kRing products ahead.
       auto products = [&](int i, auto with_values, auto with_scores) {
         constexpr bool VALUES = decltype(with_values)::value, SCORES = decltype(with_scores)::value;
-        constexpr int kValueSteps = VALUES ? 2 * KT : 0, kAhead = 2;
+        constexpr int kValues = VALUES ? 2 * KT * kBands : 0, kScores = SCORES ? kSteps * KT : 0;
+        constexpr int kRing = VALUES && D < 256 ? 8 : 4, kKeyRing = 4;
         uint32_t value_at = VALUES ? values_at(i - 1) + value_place : 0, key_at = SCORES ? keys_at(i) + key_place : 0;
         asm volatile("" : "+v"(value_at), "+v"(key_at));  // or every address of both stages stays in a register
-        u32x4 v[kAhead][kBands], k[kAhead][KT];
+        u32x4 v[kRing], k[kKeyRing];
         if constexpr (VALUES) {
 #pragma unroll
-          for (int kk = 0; kk < kAhead; ++kk)
+          for (int f = 0; f < kRing; ++f) v[f] = value_words(value_at, f / kBands, f % kBands);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kRing, 0);
 #pragma unroll
-            for (int b = 0; b < kBands; ++b) v[kk][b] = value_words(value_at, kk, b);
-          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead * kBands, 0);
-#pragma unroll
-          for (int kk = 0; kk < kValueSteps; ++kk) {
-#pragma unroll
-            for (int b = 0; b < kBands; ++b) {
-              o[b] = product(v[kk % kAhead][b], weights[kk], o[b]);
-              if (kk + kAhead < kValueSteps) v[kk % kAhead][b] = value_words(value_at, kk + kAhead, b);
-            }
+          for (int f = 0; f < kValues; ++f) {
+            o[f % kBands] = product(v[f % kRing], weights[f / kBands], o[f % kBands]);
+            if (f + kRing < kValues) v[f % kRing] = value_words(value_at, (f + kRing) / kBands, (f + kRing) % kBands);
           }
         }
         if constexpr (SCORES) {
 #pragma unroll
-          for (int st = 0; st < kAhead; ++st)
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) k[st][kt] = key_words(key_at, st, kt);
+          for (int f = 0; f < kKeyRing; ++f) k[f] = key_words(key_at, f / KT, f % KT);
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
 #pragma unroll
-          for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              s[kt] = product(k[st % kAhead][kt], qv[st], s[kt]);
-              if (st + kAhead < kSteps) k[st % kAhead][kt] = key_words(key_at, st + kAhead, kt);
-            }
+          for (int f = 0; f < kScores; ++f) {
+            s[f % KT] = product(k[f % kKeyRing], qv[f / KT], s[f % KT]);
+            if (f + kKeyRing < kScores) k[f % kKeyRing] = key_words(key_at, (f + kKeyRing) / KT, (f + kKeyRing) % KT);
+          }
         }
         // the order: after the first reads, a product, then the reads that its operands' registers are free for
 #pragma unroll
-        for (int kk = 0; kk < kValueSteps; ++kk)
-#pragma unroll
-          for (int b = 0; b < kBands; ++b) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (kk + kAhead < kValueSteps) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            else if (SCORES && (kk + kAhead - kValueSteps) * kBands + b < kAhead * KT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
+        for (int f = 0; f < kValues; ++f) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (f + kRing < kValues) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          else if (SCORES && f + kKeyRing >= kValues) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
         if constexpr (SCORES) {
-          if constexpr (!VALUES) __builtin_amdgcn_sched_group_barrier(0x100, kAhead * KT, 0);
+          if constexpr (!VALUES) __builtin_amdgcn_sched_group_barrier(0x100, kKeyRing, 0);
 #pragma unroll
-          for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-              if (st + kAhead < kSteps) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
+          for (int f = 0; f < kScores; ++f) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (f + kKeyRing < kScores) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
         }
       };
       constexpr std::true_type kYes{};
