@@ -21,7 +21,7 @@ constexpr int64_t kMostItems = kLimit32 - (1 << 22);  // attention_index.h
 constexpr int64_t kWaves = 4;
 // kernels/attention_prompt.hip
 constexpr int64_t kPromptBlocks = 256;
-constexpr int64_t kJoinSlices = 4;
+constexpr int64_t kJoinSlices = 8;
 constexpr int64_t kCut = 8;  // attention_index.h
 // Blocks of the append to an E4M3_BLOCKS cache that write keys and values; each goes on
 // in steps of the grid.

@@ -285,7 +285,7 @@ LF_DEVICE QueryTile query_tile_of(const Desc &d, int tile_rows) {
 // innermost. A pair weighs the keys that its tile sees, without their rounding to key tiles,
 // and kPairKeys for what it takes whatever its keys are: min(a + step x, cap) for tile x of a
 // sequence, so that sums over x have a closed form. The blocks take equal ranges of weight.
-constexpr int kPairKeys = 128;
+constexpr int kPairKeys = 256;
 struct Weights {
   int64_t a, step, cap;
   int tiles;

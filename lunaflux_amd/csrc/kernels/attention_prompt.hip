@@ -27,13 +27,15 @@ struct Prompts {
   static constexpr int kTileBytes = kKeys * D * 2;
   static constexpr int kFloats = kRows * (D + 2);  // of a partial result: sums, maxima, weight sums
 };
-constexpr int kJoinSlices = 4;
+constexpr int kJoinSlices = 8;
 
 // The step's prompts, their weights added up in LDS.
 struct PromptPlan {
   int n, rows;
   QueryTile tile;
-  int64_t heads, total, share;  // heads: pairs of key head and part of its group
+  int heads;             // pairs of key head and part of its group
+  int token_of;          // rows of a tile to tokens: row token_of >> 16 (exact: both are at most 256)
+  int64_t total, share;
 };
 
 template <int D, int THREADS>
@@ -45,7 +47,8 @@ LF_DEVICE PromptPlan plan_of(const Desc &d, const int32_t *counts, const int32_t
   plan.rows = live_rows(counts, d.max_tokens);
   plan.n = decoded_of(d, 0, counts[0], counts[2]).n;
   plan.tile = query_tile_of(d, Prompts<D>::kRows);
-  plan.heads = static_cast<int64_t>(d.kv_heads) * plan.tile.subs;
+  plan.heads = d.kv_heads * plan.tile.subs;
+  plan.token_of = plan.tile.subs > 1 ? 0 : (65536 + plan.tile.heads - 1) / plan.tile.heads;
   int64_t carry = 0, rows = 0;
   for (int base = 0; base < plan.n; base += THREADS) {
     const int i = base + static_cast<int>(threadIdx.x);
@@ -87,11 +90,21 @@ LF_DEVICE PromptPlan plan_of(const Desc &d, const int32_t *counts, const int32_t
 
 // A pair of the step: its sequence, head (key head and part of its group), query tile, and place in the weight.
 struct PromptPair {
-  int i, x;
-  int64_t head, begin, weight;
+  int i, x, head;
+  int64_t begin, weight;
   Prompt p;
   Weights w;
 };
+// Query heads of a pair: key head, first query head and number.
+struct PairHeads {
+  int h, first, count;
+};
+LF_DEVICE PairHeads heads_of(const Desc &d, const PromptPlan &plan, const PromptPair &pair) {
+  const int group = d.query_heads / d.kv_heads;
+  if (plan.tile.subs == 1) return {pair.head, pair.head * group, group};
+  const int h = pair.head / plan.tile.subs, from = (pair.head - h * plan.tile.subs) * plan.tile.heads;
+  return {h, h * group + from, group - from < plan.tile.heads ? group - from : plan.tile.heads};
+}
 LF_DEVICE void read_prompt(const Desc &d, const PromptPlan &plan, const int32_t *row_offsets, const int32_t *lengths,
                            const int32_t *page_offsets, PromptPair &pair) {
   bool unused = false;
@@ -104,7 +117,7 @@ LF_DEVICE PromptPair pair_at(const Desc &d, const PromptPlan &plan, const int32_
   pair.i = __builtin_amdgcn_readfirstlane(prompt_at(prefix, plan.n, plan.heads, u));
   read_prompt(d, plan, row_offsets, lengths, page_offsets, pair);
   const int64_t first = prefix[pair.i] * plan.heads, each = prefix[pair.i + 1] - prefix[pair.i];
-  pair.head = (u - first) / each;
+  pair.head = __builtin_amdgcn_readfirstlane(static_cast<int>((u - first) / each));
   const int64_t within = u - first - pair.head * each;
   pair.x = __builtin_amdgcn_readfirstlane(tile_at(pair.w, within));
   pair.begin = first + pair.head * each + weight_before(pair.w, pair.x);
@@ -132,14 +145,15 @@ LF_DEVICE float *partial_of(uint8_t *ws, int slot) {
 
 // One global_load_lds_dwordx4: every lane's 16 bytes from its address go to LDS at lds + 16 lane
 // (wave-uniform; M0). As assembly, so that the compiler does not make every LDS read wait for it:
-// the kernel orders it by itself, with vmcnt and barriers.
+// the kernel orders it by itself, with vmcnt and barriers. No read of the interval that it is issued in
+// touches what it writes, so the two may change places (interval_end holds both).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // M0 is listed as clobbered on purpose
 LF_DEVICE void load_to_lds(const uint8_t *src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
                :
                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
-               : "memory", "m0");
+               : "m0");
 }
 #pragma clang diagnostic pop
 LF_DEVICE uint32_t lds_at(const uint8_t *p) {
@@ -243,7 +257,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
   if (bad) flag_error(error);
   if (u0 >= u1) return;
 
-  const int Hq = d.query_heads, Hkv = d.kv_heads, group = Hq / Hkv;
+  const int Hq = d.query_heads, Hkv = d.kv_heads;
   const int shift = __builtin_ctz(d.page_size), slot_mask = d.page_size - 1, pages = d.pages;
   const float *scales = reinterpret_cast<const float *>(attn + d.scale_offset);
   const bool flip = d.softmax_scale < 0.0f;
@@ -257,10 +271,8 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
     const PromptKeys pk = keys_of(d, plan.tile, pair.p, pair.x, kKeys);
     const int k0 = cut_of(u0, pair.begin, pair.weight, pk.tiles), k1 = cut_of(u1, pair.begin, pair.weight, pk.tiles);
     if (k0 < k1) {
-      const int h = static_cast<int>(pair.head / plan.tile.subs), sub = static_cast<int>(pair.head - static_cast<int64_t>(h) * plan.tile.subs);
-      const int tokens = pk.last - pk.first_position + 1;
-      const int head0 = h * group + sub * plan.tile.heads;
-      const int heads = group - sub * plan.tile.heads < plan.tile.heads ? group - sub * plan.tile.heads : plan.tile.heads;
+      const PairHeads of = heads_of(d, plan, pair);
+      const int h = of.h, head0 = of.first, heads = of.count, tokens = pk.last - pk.first_position + 1;
       const int row0 = pair.p.row + pair.x * plan.tile.tokens;
       const int32_t *table = page_indices + pair.p.entry;
       const int page_first = pk.lo >> shift, page_end = (pk.last >> shift) + 1, sink_end = (pk.sink + slot_mask) >> shift;
@@ -269,39 +281,40 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       const int n = k1 - k0;
       auto base_of = [&](int i) { return kKeys * (k0 + i < pk.sink_tiles ? k0 + i : k0 + i + pk.first - pk.sink_tiles); };
 
-      // Pages of a tile's groups of eight keys, in lanes of every eight; of those that are this wave's rows of a tile,
-      // kKeys / 8 of them, the page itself.
-      constexpr int kWaveKeys = kKeys / P::kWaves;
+      // Tiles are loaded by the first group's waves, or by all of them where codes are converted on the way.
+      constexpr int kLoaders = E4M3 ? P::kWaves : P::kWaves / 2, kWaveKeys = kKeys / kLoaders, kGroups = (kWaveKeys + 7) / 8;
+      // Pages of a tile's groups of eight keys, in lanes of every eight; the loads take those of the wave's own rows. One
+      // that the cache does not have is read as page 0: the tiles' results are not used then.
       auto pages_of_tile = [&](int i) {
         return table[sink_entry_of(sink_end, page_first, page_end, shift, base_of(i < n ? i : n - 1) + 8 * (lane & (kKeys / 8 - 1)))];
       };
-      struct TilePages {
-        int page;
-        uint32_t outside;  // groups whose page the cache does not have
-      } tile_pages[3];     // of the tile whose keys are loaded next, and of those before
-      int loading;         // its successor's, on their way
+      int tile_pages[2][kGroups];  // of the tile whose keys are loaded next, and of the one before
+      int loading;                 // its successor's, on their way
+      bool outside = false;
       auto arrived = [&]() {
-        const int p = __builtin_amdgcn_readlane(loading, wave * kWaveKeys / 8);
-        tile_pages[2] = tile_pages[1];
-        tile_pages[1] = tile_pages[0];
-        tile_pages[0] = {static_cast<uint32_t>(p) < static_cast<uint32_t>(pages) ? p : 0,
-                         static_cast<uint32_t>(__ballot(static_cast<uint32_t>(loading) >= static_cast<uint32_t>(pages))) & ((1u << (kKeys / 8)) - 1)};
+        outside |= __ballot(static_cast<uint32_t>(loading) >= static_cast<uint32_t>(pages)) != 0;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const int p = __builtin_amdgcn_readlane(loading, (wave & (kLoaders - 1)) * kWaveKeys / 8 + g);
+          tile_pages[1][g] = tile_pages[0][g];
+          tile_pages[0][g] = static_cast<uint32_t>(p) < static_cast<uint32_t>(pages) ? p : 0;
+        }
       };
-      auto slot_of = [&](int i, int key) {
-        const int j = base_of(i) + key;
+      auto slot_of = [&](int base, int key) {
+        const int j = base + key;
         return (j < pk.last ? j : pk.last) & slot_mask;
       };
       const uint8_t *head_keys = kc + static_cast<uint64_t>(static_cast<uint32_t>(h)) * head_bytes;
       const uint8_t *head_values = vc + static_cast<uint64_t>(static_cast<uint32_t>(h)) * head_bytes;
-      auto load_tile = [&](const uint8_t *cache, uint32_t to, int i, int p) {  // bf16
+      auto load_tile = [&](const uint8_t *cache, uint32_t to, int base, const int (&p)[kGroups]) {  // bf16
         constexpr int kChunks = D / 8, kRowsAtOnce = 64 / kChunks;
-        int l = lane;
-        asm volatile("" : "+v"(l));  // what follows from it is computed here, not kept
+        const int first = wave * kWaveKeys;
 #pragma unroll
         for (int r = 0; r < kWaveKeys; r += kRowsAtOnce) {
-          const int key = wave * kWaveKeys + r + l / kChunks, chunk = l & (kChunks - 1);
+          const int key = first + r + lane / kChunks, chunk = lane & (kChunks - 1);
           const int from = chunk ^ (chunk_swizzle(key & 15) & (kChunks - 1));
-          load_to_lds(cache + row_byte(p, slot_of(i, key), page_bytes, token_bytes) + 16 * from, to + (wave * kWaveKeys + r) * D * 2);
+          const uint8_t *page = cache + static_cast<uint64_t>(static_cast<uint32_t>(p[r / 8])) * page_bytes;
+          load_to_lds(page + (static_cast<uint64_t>(static_cast<uint32_t>(slot_of(base, key))) * token_bytes + 16 * from), to + (first + r) * D * 2);
         }
       };
       // e4m3: through registers, 16 codes of a row or 8.
@@ -312,7 +325,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       };
       const int code_key = static_cast<int>(threadIdx.x) / (D / kCodes), code_at = static_cast<int>(threadIdx.x) % (D / kCodes);
       auto load_codes = [&](const uint8_t *cache, const uint8_t *table_of, int i, int p, Codes &x) {
-        const int slot = slot_of(i, code_key);
+        const int slot = slot_of(base_of(i), code_key);
         const uint32_t *src = reinterpret_cast<const uint32_t *>(cache + row_byte(p, slot, page_bytes, token_bytes) + kCodes * code_at);
         if constexpr (kWords == 4) {
           const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
@@ -338,34 +351,27 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
           lds_write(to + tile_byte<D>(code_key, (kCodes * code_at + 2 * e) / 8), u32x4{b[e], b[e + 1], b[e + 2], b[e + 3]});
       };
       Codes next_keys, next_values;
-      // Begins to load stage i, and for e4m3 stores it.
+      // Begins to load stage i <= n, and for e4m3 stores it (the last one's keys: those of the last tile, of no use).
       auto load_stage = [&](int i) {
-        if (i < n) {
-          if constexpr (E4M3) {
-            load_codes(head_keys, kc, i, tile_pages[0].page, next_keys);
-          } else {
-            load_tile(head_keys, keys_at(i), i, tile_pages[0].page);
-          }
-        }
-        if (i > 0 && i <= n) {
-          if constexpr (E4M3) {
-            load_codes(head_values, vc, i - 1, tile_pages[1].page, next_values);
-          } else {
-            load_tile(head_values, values_at(i - 1), i - 1, tile_pages[1].page);
-          }
+        if constexpr (E4M3) {
+          load_codes(head_keys, kc, i < n ? i : n - 1, tile_pages[0][0], next_keys);
+          if (i > 0) load_codes(head_values, vc, i - 1, tile_pages[1][0], next_values);
+        } else {
+          load_tile(head_keys, keys_at(i), base_of(i < n ? i : n - 1), tile_pages[0]);
+          if (i > 0) load_tile(head_values, values_at(i - 1), base_of(i - 1), tile_pages[1]);
         }
         loading = pages_of_tile(i + 1);
       };
       auto store_stage = [&](int i) {
         if constexpr (E4M3) {
-          if (i < n) store_codes(keys_at(i), next_keys);
-          if (i > 0 && i <= n) store_codes(values_at(i - 1), next_values);
+          store_codes(keys_at(i), next_keys);
+          if (i > 0) store_codes(values_at(i - 1), next_values);
         }
       };
 
       // this lane's row: query operand, position, statistics
       u32x4 qv[kSteps];
-      const int m = wave * 32 + c, token = m / heads, head = m - token * heads;
+      const int m = wave * 32 + c, token = (m * plan.token_of) >> 16, head = m - token * heads;
       const bool live = m < tokens * heads;
       const int position = live ? pk.first_position + token : pk.first_position;
       const uint32_t row_at = static_cast<uint32_t>(live ? row0 + token : row0) * Hq + head0 + (live ? head : 0);
@@ -383,21 +389,27 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       // are gone through once more, with the largest that was seen. So the sums are never scaled.
       constexpr float kNear = 40.0f;
       float top = -INFINITY, seen = -INFINITY, sum;
+      int redo;
       f32x16 o[kBands];
       do {
-      loading = pages_of_tile(0);
-      arrived();
-      load_stage(0);
+      const bool loads = wave < kLoaders;
+      if (loads) {
+        loading = pages_of_tile(0);
+        const int second = pages_of_tile(1);
+        arrived();
+        load_stage(0);
+        loading = second;
+        arrived();
+        if constexpr (E4M3) store_stage(0);
+        load_stage(1);
+      }
       top = seen;
       sum = 0.0f;
 #pragma unroll
       for (int b = 0; b < kBands; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-      store_stage(0);
-      arrived();
-      load_stage(1);
-      store_stage(1);
+      if (loads) store_stage(1);
       interval_end<true>();
       if (threadIdx.x == 0) once_more = 0;  // every wave has read it by now
 
@@ -417,9 +429,6 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)((band ^ 32) + (kk * 16 + 8) * D * 2));
         const uint2 w0 = __builtin_bit_cast(uint2, lo), w1 = __builtin_bit_cast(uint2, hi);
         return u32x4{w0.x, w0.y, w1.x, w1.y};
-      };
-      auto is_masked = [&](int from, uint32_t outer) {  // some row of the tile does not count some key
-        return from + kKeys - 1 > pk.first_position || outer != 0 || (from <= pk.last - window && from + kKeys > sinks);
       };
       auto product = [&](u32x4 a, u32x4 b, f32x16 acc) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
@@ -474,59 +483,65 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       };
       constexpr std::true_type kYes{};
       constexpr std::false_type kNo{};
-      auto softmax = [&](int i, const TilePages &of) {
+      // positions of the wave's rows
+      const int wave_first = pk.first_position + (wave * 32 < tokens * heads ? (wave * 32 * plan.token_of) >> 16 : 0);
+      const int wave_last = pk.first_position + (wave * 32 + 31 < tokens * heads ? ((wave * 32 + 31) * plan.token_of) >> 16 : tokens - 1);
+      auto softmax = [&](int i) {
         const int base = base_of(i);
-        const uint32_t out_of_cache = of.outside;
         float z[16 * KT];
 #pragma unroll
         for (int e = 0; e < 16 * KT; ++e) z[e] = s[e / 16][e % 16];
-        if (out_of_cache != 0) bad = true;
-        if (is_masked(base, out_of_cache)) {
-          // the row counts keys low < j <= position and j < sinks (no short circuits: each would be a branch)
+        if (base + kKeys - 1 > wave_first || (base <= wave_last - window && base + kKeys > sinks)) {
+          // some row does not count some key: it counts those low < j <= to and j < sink (no short circuits: each
+          // would be a branch)
           const int to = position - base - 4 * half, low = to - window, sink = sinks - base - 4 * half;
 #pragma unroll
           for (int e = 0; e < 16 * KT; ++e) {
             const int j = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3);
-            const bool counts = (j <= to) & ((j > low) | (j < sink)) & (((out_of_cache >> (j >> 3)) & 1) == 0);
+            const bool counts = (j <= to) & ((j > low) | (j < sink));
             z[e] = counts ? z[e] : -INFINITY;
           }
         }
-        float most = z[0];
+        float most = z[0], other = z[1];
 #pragma unroll
-        for (int e = 1; e < 16 * KT; ++e) most = fmaxf(most, z[e]);
+        for (int e = 2; e < 16 * KT; e += 2) most = fmaxf(most, z[e]), other = fmaxf(other, z[e + 1]);
         {
-          const uint32_t a = __float_as_uint(most);
+          const uint32_t a = __float_as_uint(fmaxf(most, other));
           const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
           most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * factor;
         }
         seen = fmaxf(seen, most);
         top = top == -INFINITY ? most : top;
         const float from = top == -INFINITY ? 0.0f : top;
+        float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < 8 * KT; ++e) {
           const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e], factor, -from));
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e + 1], factor, -from));
           const uint32_t w = pack_bf16(p0, p1);
           weights[e / 4][e % 4] = w;
-          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+          sums[e & 3] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sums[e & 3], false);
         }
+        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
         for (int e = 0; e < 2 * KT; ++e) asm volatile("" : "+v"(weights[e]));  // here, not with the products
       };
-      // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. Both
-      // groups load a stage between the same two barriers, in which the first has products and the second a
-      // softmax. (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
+      // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. A
+      // stage is loaded from the first group's products on, which the second begins a softmax with, through the
+      // interval after. (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
       auto tiles = [&](auto behind) {
-        constexpr bool LATE = decltype(behind)::value;
+        constexpr bool LATE = decltype(behind)::value, LOADS = !LATE || E4M3;
         if constexpr (LATE) {
-          arrived();
+          if constexpr (LOADS) arrived();
           interval_end<false>();
         }
         products(0, kNo, kYes);
         interval_end<false>();
         for (int i = 0; i < n;) {
-          if constexpr (LATE) load_stage(i + 2);
-          softmax(i, tile_pages[LATE ? 2 : 1]);
+          if constexpr (LATE && LOADS) {
+            if (i + 2 <= n) load_stage(i + 2);
+          }
+          softmax(i);
           if constexpr (LATE) {
             interval_end<false>();
           } else {
@@ -535,10 +550,12 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
             arrived();
           }
           ++i;
-          if constexpr (!LATE) load_stage(i + 1);
+          if constexpr (!LATE) {
+            if (i + 1 <= n) load_stage(i + 1);
+          }
           products(i, kYes, kYes);  // behind the last tile's values, scores of no use
-          if constexpr (LATE) {
-            store_stage(i + 1);
+          if constexpr (LATE && LOADS) {
+            if (i + 1 <= n) store_stage(i + 1);
             interval_end<true>();
             arrived();
           } else {
@@ -552,9 +569,13 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       } else {
         tiles(kNo);
       }
-      if (__ballot(live && seen > top + kNear) != 0 && lane == 0) once_more = 1;
+      // 1: once more; 2: a page outside the cache
+      const int after = outside ? 2 : __ballot(live && seen > top + kNear) != 0 ? 1 : 0;
+      if (after != 0 && lane == 0) atomicOr(&once_more, after);
       interval_end<false>();
-      } while (__builtin_amdgcn_readfirstlane(once_more) != 0);
+      redo = __builtin_amdgcn_readfirstlane(once_more);
+      } while (redo == 1);
+      if (redo >= 2) bad = true;
 
       const uint32_t sum_bits = __float_as_uint(sum);
       const auto both = __builtin_amdgcn_permlane32_swap(sum_bits, sum_bits, false, false);
@@ -572,10 +593,19 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
 #pragma unroll
         for (int b = 0; b < kBands; ++b)
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            uint2 w = {pack_bf16(o[b][e] * scale, o[b][e + 1] * scale), pack_bf16(o[b][e + 2] * scale, o[b][e + 3] * scale)};
-            if (total == 0.0f) w = {0u, 0u};
-            *reinterpret_cast<uint2 *>(dst + 32 * b + 2 * e + 4 * half) = w;
+          for (int e = 0; e < 16; e += 8) {
+            // columns 2 e + 4 half .. and 2 e + 8 + 4 half ..: the lanes of a row trade for eight in a row each
+            u32x4 w;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint32_t lo = pack_bf16(o[b][e + 2 * k] * scale, o[b][e + 2 * k + 1] * scale);
+              uint32_t hi = pack_bf16(o[b][e + 4 + 2 * k] * scale, o[b][e + 5 + 2 * k] * scale);
+              if (total == 0.0f) lo = hi = 0;
+              const auto x = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+              w[k] = x[0];
+              w[2 + k] = x[1];
+            }
+            *reinterpret_cast<u32x4 *>(dst + 32 * b + 2 * e + 8 * half) = w;
           }
       } else if (live) {
 #pragma unroll
@@ -588,7 +618,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
           part[P::kRows * D + P::kRows + m] = total;
         }
       }
-      if (__ballot(live && !(finite < INFINITY)) != 0) {
+      if (__ballot(live && !(finite < INFINITY)) != 0 || redo >= 2) {
         const CarefulRow r = {q + static_cast<uint64_t>(row_at) * D, kc, vc, table, pk, k0, k1, h, position, factor};
         float acc[D / 2], careful_top, careful_sum;
         careful_row<D, CACHE>(d, r, flip, acc, careful_top, careful_sum);
@@ -667,34 +697,48 @@ LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, c
   __syncthreads();
   const int worker = (own - 1) * kJoinSlices + slice, workers = (parts - 1) * kJoinSlices;
 
-  const int Hq = d.query_heads, group = Hq / d.kv_heads;
-  const int h = static_cast<int>(pair.head / plan.tile.subs), sub = static_cast<int>(pair.head - static_cast<int64_t>(h) * plan.tile.subs);
-  const int head0 = h * group + sub * plan.tile.heads;
-  const int heads = group - sub * plan.tile.heads < plan.tile.heads ? group - sub * plan.tile.heads : plan.tile.heads;
-  const int rows = (pk.last - pk.first_position + 1) * heads;
+  const int Hq = d.query_heads;
+  const PairHeads of = heads_of(d, plan, pair);
+  const int h = of.h, head0 = of.first, heads = of.count, rows = (pk.last - pk.first_position + 1) * heads;
   const int row0 = pair.p.row + pair.x * plan.tile.tokens;
   const float vscale = CACHE == kCacheE4m3 ? reinterpret_cast<const float *>(attn + d.scale_offset)[d.kv_heads + h] : 1.0f;
-  constexpr int kQuads = D / 4;
+  constexpr int kQuads = D / 4, kAtOnce = 4;
   const int m0 = rows * worker / workers, m1 = rows * (worker + 1) / workers;
-  for (int i = m0 * kQuads + static_cast<int>(threadIdx.x); i < m1 * kQuads; i += 256) {
-    const int m = i / kQuads, column = i % kQuads * 4;
-    float top = -INFINITY, sum = 0.0f;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int first_quad = m0 * kQuads + static_cast<int>(threadIdx.x); first_quad < m1 * kQuads; first_quad += kAtOnce * 256) {
+    float top[kAtOnce], sum[kAtOnce];
+    f32x4 acc[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) top[k] = -INFINITY, sum[k] = 0.0f, acc[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int p = 0; p < parts; ++p) {
       const float *part = partial_of<D>(ws, slots[p]);
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(part + m * D + column);
-      const float t = part[P::kRows * D + m], l = part[P::kRows * D + P::kRows + m];
-      const float next = fmaxf(top, t), base = next == -INFINITY ? 0.0f : next;
-      const float keep = __builtin_amdgcn_exp2f(top - base), f = __builtin_amdgcn_exp2f(t - base);
-      acc = acc * keep + v * f;
-      sum = sum * keep + l * f;
-      top = next;
+      f32x4 v[kAtOnce];
+      float t[kAtOnce], l[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int quad = first_quad + k * 256 < m1 * kQuads ? first_quad + k * 256 : first_quad, m = quad / kQuads;
+        v[k] = *reinterpret_cast<const f32x4 *>(part + 4 * quad);
+        t[k] = part[P::kRows * D + m];
+        l[k] = part[P::kRows * D + P::kRows + m];
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float next = fmaxf(top[k], t[k]), base = next == -INFINITY ? 0.0f : next;
+        const float keep = __builtin_amdgcn_exp2f(top[k] - base), f = __builtin_amdgcn_exp2f(t[k] - base);
+        acc[k] = acc[k] * keep + v[k] * f;
+        sum[k] = sum[k] * keep + l[k] * f;
+        top[k] = next;
+      }
     }
-    const float scale = vscale / sum;
-    uint2 w = {pack_bf16(acc[0] * scale, acc[1] * scale), pack_bf16(acc[2] * scale, acc[3] * scale)};
-    if (sum == 0.0f) w = {0u, 0u};
-    const int token = m / heads;
-    *reinterpret_cast<uint2 *>(out + (static_cast<uint64_t>(row0 + token) * Hq + head0 + m - token * heads) * D + column) = w;
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int quad = first_quad + k * 256, m = quad / kQuads, column = quad % kQuads * 4;
+      if (quad >= m1 * kQuads) break;
+      const float scale = vscale / sum[k];
+      uint2 w = {pack_bf16(acc[k][0] * scale, acc[k][1] * scale), pack_bf16(acc[k][2] * scale, acc[k][3] * scale)};
+      if (sum[k] == 0.0f) w = {0u, 0u};
+      const int token = (m * plan.token_of) >> 16;
+      *reinterpret_cast<uint2 *>(out + (static_cast<uint64_t>(row0 + token) * Hq + head0 + m - token * heads) * D + column) = w;
+    }
   }
 }
 
