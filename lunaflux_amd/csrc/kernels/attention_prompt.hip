@@ -117,7 +117,10 @@ LF_DEVICE PromptPair pair_at(const Desc &d, const PromptPlan &plan, const int32_
   pair.i = __builtin_amdgcn_readfirstlane(prompt_at(prefix, plan.n, plan.heads, u));
   read_prompt(d, plan, row_offsets, lengths, page_offsets, pair);
   const int64_t first = prefix[pair.i] * plan.heads, each = prefix[pair.i + 1] - prefix[pair.i];
-  pair.head = __builtin_amdgcn_readfirstlane(static_cast<int>((u - first) / each));
+  int64_t head = quotient(u - first, each);  // up to one off where the weights pass 2^52
+  if (head * each > u - first) --head;
+  if ((head + 1) * each <= u - first) ++head;
+  pair.head = __builtin_amdgcn_readfirstlane(static_cast<int>(head));
   const int64_t within = u - first - pair.head * each;
   pair.x = __builtin_amdgcn_readfirstlane(tile_at(pair.w, within));
   pair.begin = first + pair.head * each + weight_before(pair.w, pair.x);
@@ -702,42 +705,85 @@ LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, c
   const int h = of.h, head0 = of.first, heads = of.count, rows = (pk.last - pk.first_position + 1) * heads;
   const int row0 = pair.p.row + pair.x * plan.tile.tokens;
   const float vscale = CACHE == kCacheE4m3 ? reinterpret_cast<const float *>(attn + d.scale_offset)[d.kv_heads + h] : 1.0f;
-  constexpr int kQuads = D / 4, kAtOnce = 4;
+  constexpr int kQuads = D / 4;
   const int m0 = rows * worker / workers, m1 = rows * (worker + 1) / workers;
-  for (int first_quad = m0 * kQuads + static_cast<int>(threadIdx.x); first_quad < m1 * kQuads; first_quad += kAtOnce * 256) {
-    float top[kAtOnce], sum[kAtOnce];
-    f32x4 acc[kAtOnce];
+  struct Joined {
+    f32x4 acc;
+    float top, sum;
+  };
+  auto add = [](Joined &x, const f32x4 &v, float t, float l) {
+    const float next = fmaxf(x.top, t), base = next == -INFINITY ? 0.0f : next;
+    const float keep = __builtin_amdgcn_exp2f(x.top - base), f = __builtin_amdgcn_exp2f(t - base);
+    x.acc = x.acc * keep + v * f;
+    x.sum = x.sum * keep + l * f;
+    x.top = next;
+  };
+  auto finish = [&](int quad, const Joined &x) {
+    const int m = quad / kQuads, column = quad % kQuads * 4, token = (m * plan.token_of) >> 16;
+    const float scale = vscale / x.sum;
+    uint2 w = {pack_bf16(x.acc[0] * scale, x.acc[1] * scale), pack_bf16(x.acc[2] * scale, x.acc[3] * scale)};
+    if (x.sum == 0.0f) w = {0u, 0u};
+    *reinterpret_cast<uint2 *>(out + (static_cast<uint64_t>(row0 + token) * Hq + head0 + m - token * heads) * D + column) = w;
+  };
+  // Few parts: two of them at a time for four values of a thread. Many: eight groups of threads share them, and
+  // their sums are added up in their order.
+  constexpr Joined kNone = {{0.0f, 0.0f, 0.0f, 0.0f}, -INFINITY, 0.0f};
+  if (parts <= 4) {
+    constexpr int kAtOnce = 4;
+    for (int q0 = m0 * kQuads + static_cast<int>(threadIdx.x); q0 < m1 * kQuads; q0 += kAtOnce * 256) {
+      Joined x[kAtOnce] = {kNone, kNone, kNone, kNone};
+      for (int p0 = 0; p0 < parts; p0 += 2) {
+        f32x4 v[2][kAtOnce];
+        float t[2][kAtOnce], l[2][kAtOnce];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) top[k] = -INFINITY, sum[k] = 0.0f, acc[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < parts; ++p) {
-      const float *part = partial_of<D>(ws, slots[p]);
-      f32x4 v[kAtOnce];
-      float t[kAtOnce], l[kAtOnce];
+        for (int p = 0; p < 2; ++p) {
+          const float *part = partial_of<D>(ws, slots[p0 + p < parts ? p0 + p : p0]);
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const int quad = first_quad + k * 256 < m1 * kQuads ? first_quad + k * 256 : first_quad, m = quad / kQuads;
-        v[k] = *reinterpret_cast<const f32x4 *>(part + 4 * quad);
-        t[k] = part[P::kRows * D + m];
-        l[k] = part[P::kRows * D + P::kRows + m];
+          for (int k = 0; k < kAtOnce; ++k) {
+            const int quad = q0 + k * 256 < m1 * kQuads ? q0 + k * 256 : q0;
+            v[p][k] = *reinterpret_cast<const f32x4 *>(part + 4 * quad);
+            t[p][k] = part[P::kRows * D + quad / kQuads];
+            l[p][k] = part[P::kRows * D + P::kRows + quad / kQuads];
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k)
+            if (p0 + p < parts) add(x[k], v[p][k], t[p][k], l[p][k]);
       }
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const float next = fmaxf(top[k], t[k]), base = next == -INFINITY ? 0.0f : next;
-        const float keep = __builtin_amdgcn_exp2f(top[k] - base), f = __builtin_amdgcn_exp2f(t[k] - base);
-        acc[k] = acc[k] * keep + v[k] * f;
-        sum[k] = sum[k] * keep + l[k] * f;
-        top[k] = next;
-      }
+      for (int k = 0; k < kAtOnce; ++k)
+        if (q0 + k * 256 < m1 * kQuads) finish(q0 + k * 256, x[k]);
     }
+  } else {
+    constexpr int kGroups = 8, kItems = 256 / kGroups, kAtOnce = 4;
+    __shared__ Joined joined[kGroups][kItems];
+    const int g = static_cast<int>(threadIdx.x) / kItems, item = static_cast<int>(threadIdx.x) % kItems;
+    for (int q0 = m0 * kQuads; q0 < m1 * kQuads; q0 += kItems) {
+      const int quad = q0 + item < m1 * kQuads ? q0 + item : q0;
+      Joined x = kNone;
+      for (int p0 = g; p0 < parts; p0 += kAtOnce * kGroups) {
+        f32x4 v[kAtOnce];
+        float t[kAtOnce], l[kAtOnce];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int quad = first_quad + k * 256, m = quad / kQuads, column = quad % kQuads * 4;
-      if (quad >= m1 * kQuads) break;
-      const float scale = vscale / sum[k];
-      uint2 w = {pack_bf16(acc[k][0] * scale, acc[k][1] * scale), pack_bf16(acc[k][2] * scale, acc[k][3] * scale)};
-      if (sum[k] == 0.0f) w = {0u, 0u};
-      const int token = (m * plan.token_of) >> 16;
-      *reinterpret_cast<uint2 *>(out + (static_cast<uint64_t>(row0 + token) * Hq + head0 + m - token * heads) * D + column) = w;
+        for (int k = 0; k < kAtOnce; ++k) {
+          const float *part = partial_of<D>(ws, slots[p0 + k * kGroups < parts ? p0 + k * kGroups : p0]);
+          v[k] = *reinterpret_cast<const f32x4 *>(part + 4 * quad);
+          t[k] = part[P::kRows * D + quad / kQuads];
+          l[k] = part[P::kRows * D + P::kRows + quad / kQuads];
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+          if (p0 + k * kGroups < parts) add(x, v[k], t[k], l[k]);
+      }
+      joined[g][item] = x;
+      __syncthreads();
+      if (g == 0) {
+        for (int k = 1; k < kGroups; ++k) add(x, joined[k][item].acc, joined[k][item].top, joined[k][item].sum);
+        if (q0 + item < m1 * kQuads) finish(quad, x);
+      }
+      __syncthreads();
     }
   }
 }
