@@ -244,12 +244,11 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
       break;
     case LF_FP8_ATTN_PREFILL:
       gx = kPromptBlocks;
-      lds = (int64_t(d->max_sequences) + 1) / 2 * 16 + 16 + 2 * prompt_keys(d) * d->head_dim * 2 * 2;
+      lds = (d->cache == LF_FP8_CACHE_BF16 ? 3 : 2) * 2 * prompt_keys(d) * d->head_dim * 2;
       std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_prefill_d%d_%s", d->head_dim, type);
       break;
     case LF_FP8_ATTN_PREFILL_JOIN:
       gx = prompt_cuts(d) ? kPromptBlocks * kJoinSlices : 0;
-      lds = (int64_t(d->max_sequences) + 1) / 2 * 16 + 16;
       std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_prefill_join_d%d_%s", d->head_dim, type);
       break;
     default: return LF_INVALID_ARGUMENT;

@@ -27,7 +27,7 @@ struct Prompts {
   static constexpr int kTileBytes = kKeys * D * 2;
   static constexpr int kFloats = kRows * (D + 2);  // of a partial result: sums, maxima, weight sums
 };
-constexpr int kJoinSlices = 8;
+constexpr int kJoinSlices = 8, kMostSequences = 2048;  // LF_FP8_ATTN_MAX_SEQUENCES
 
 // The step's prompts, their weights added up in LDS.
 struct PromptPlan {
@@ -172,12 +172,12 @@ LF_DEVICE void lds_write(uint32_t at, T v) {
 }
 
 // The block's barrier between intervals: this wave's LDS accesses are over, and no instruction
-// moves past it. LOADS: its loads to LDS have arrived too.
-template <bool LOADS>
+// moves past it. LOADS: its loads have arrived too, but for the last LEFT.
+template <bool LOADS, int LEFT = 0>
 LF_DEVICE void interval_end() {
   __builtin_amdgcn_sched_barrier(0);
   if constexpr (LOADS) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
   } else {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
@@ -244,11 +244,13 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
   const Desc &d = desc_of(attn);
   if (d.magic != kMagic) return;
   int *error = reinterpret_cast<int *>(ws);
-  // stage i & 1: the keys of tile i and the values of tile i - 1; behind the stages the prefix of weights
-  int64_t *prefix = reinterpret_cast<int64_t *>(stages + 4 * P::kTileBytes);
+  // Stage i: the keys of tile i and the values of tile i - 1. Three of them where tiles go straight to LDS, so that
+  // two are on their way.
+  constexpr int kStages = E4M3 ? 2 : 3;
+  __shared__ int64_t prefix[kMostSequences + 1];
   const uint32_t stages_at = lds_at(stages);
-  auto keys_at = [&](int i) { return stages_at + (i & 1) * 2 * P::kTileBytes; };
-  auto values_at = [&](int i) { return stages_at + ((i + 1) & 1) * 2 * P::kTileBytes + P::kTileBytes; };
+  auto keys_at = [&](int i) { return stages_at + i % kStages * 2 * P::kTileBytes; };
+  auto values_at = [&](int i) { return stages_at + (i + 1) % kStages * 2 * P::kTileBytes + P::kTileBytes; };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   __shared__ int once_more;
   const bool late = wave >= P::kWaves / 2;  // the group that is half a tile behind
@@ -286,21 +288,29 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
 
       // Tiles are loaded by the first group's waves, or by all of them where codes are converted on the way.
       constexpr int kLoaders = E4M3 ? P::kWaves : P::kWaves / 2, kWaveKeys = kKeys / kLoaders, kGroups = (kWaveKeys + 7) / 8;
-      // Pages of a tile's groups of eight keys, in lanes of every eight; the loads take those of the wave's own rows. One
-      // that the cache does not have is read as page 0: the tiles' results are not used then.
-      auto pages_of_tile = [&](int i) {
-        return table[sink_entry_of(sink_end, page_first, page_end, shift, base_of(i < n ? i : n - 1) + 8 * (lane & (kKeys / 8 - 1)))];
-      };
+      // Pages of the groups of eight keys of a tile that are this wave's to load, by scalar loads, so that no wait
+      // for them is one for the tiles on their way (they share a counter with LDS reads, so they are on their way
+      // only during a softmax). One that the cache does not have is read as page 0: the
+      // tiles' results are not used then.
       int tile_pages[2][kGroups];  // of the tile whose keys are loaded next, and of the one before
-      int loading;                 // its successor's, on their way
+      int loading[kGroups];
       bool outside = false;
-      auto arrived = [&]() {
-        outside |= __ballot(static_cast<uint32_t>(loading) >= static_cast<uint32_t>(pages)) != 0;
+      auto pages_of_tile = [&](int i) {
+        typedef const __attribute__((address_space(4))) int32_t *Constant;
+        const int base = base_of(i < n ? i : n - 1);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-          const int p = __builtin_amdgcn_readlane(loading, (wave & (kLoaders - 1)) * kWaveKeys / 8 + g);
+          const int j = base + ((wave & (kLoaders - 1)) * kWaveKeys & ~7) + 8 * g;
+          loading[g] = ((Constant)table)[__builtin_amdgcn_readfirstlane(sink_entry_of(sink_end, page_first, page_end, shift, j))];
+        }
+      };
+      auto arrived = [&]() {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const bool in = static_cast<uint32_t>(loading[g]) < static_cast<uint32_t>(pages);
+          outside |= !in;
           tile_pages[1][g] = tile_pages[0][g];
-          tile_pages[0][g] = static_cast<uint32_t>(p) < static_cast<uint32_t>(pages) ? p : 0;
+          tile_pages[0][g] = in ? loading[g] : 0;
         }
       };
       auto slot_of = [&](int base, int key) {
@@ -363,7 +373,6 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
           load_tile(head_keys, keys_at(i), base_of(i < n ? i : n - 1), tile_pages[0]);
           if (i > 0) load_tile(head_values, values_at(i - 1), base_of(i - 1), tile_pages[1]);
         }
-        loading = pages_of_tile(i + 1);
       };
       auto store_stage = [&](int i) {
         if constexpr (E4M3) {
@@ -397,13 +406,12 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       do {
       const bool loads = wave < kLoaders;
       if (loads) {
-        loading = pages_of_tile(0);
-        const int second = pages_of_tile(1);
+        pages_of_tile(0);
         arrived();
+        pages_of_tile(1);
         load_stage(0);
-        loading = second;
-        arrived();
         if constexpr (E4M3) store_stage(0);
+        arrived();
         load_stage(1);
       }
       top = seen;
@@ -530,13 +538,22 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
         for (int e = 0; e < 2 * KT; ++e) asm volatile("" : "+v"(weights[e]));  // here, not with the products
       };
       // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. A
-      // stage is loaded from the first group's products on, which the second begins a softmax with, through the
-      // interval after. (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
+      // stage's place is free when the first group begins the products two stages later (three: two before the
+      // stage), which the second begins a softmax with, and it has to be there one interval before its own.
+      // (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
+      constexpr int kStageLoads = 2 * kWaveKeys * (D / 8) / 64;
       auto tiles = [&](auto behind) {
         constexpr bool LATE = decltype(behind)::value, LOADS = !LATE || E4M3;
+        // the stage that is loaded next once softmax i is over: kNext after i
+        constexpr int kNext = LATE || !E4M3 ? 3 : 2;
+        if constexpr (LOADS && kNext == 3) {
+          pages_of_tile(2);
+          arrived();
+        }
         if constexpr (LATE) {
-          if constexpr (LOADS) arrived();
           interval_end<false>();
+        } else if constexpr (!E4M3) {
+          if (2 <= n) load_stage(2);
         }
         products(0, kNo, kYes);
         interval_end<false>();
@@ -544,23 +561,27 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
           if constexpr (LATE && LOADS) {
             if (i + 2 <= n) load_stage(i + 2);
           }
+          if constexpr (LOADS) pages_of_tile(i + kNext);
           softmax(i);
+          if constexpr (!LATE && E4M3) {
+            if (i > 0) store_stage(i + 1);
+          }
+          if constexpr (LOADS) arrived();
           if constexpr (LATE) {
             interval_end<false>();
+          } else if (!E4M3 && i + 2 <= n) {
+            interval_end<true, kStageLoads>();
           } else {
-            if (i > 0) store_stage(i + 1);
             interval_end<true>();
-            arrived();
           }
           ++i;
           if constexpr (!LATE) {
-            if (i + 1 <= n) load_stage(i + 1);
+            if (i + kStages - 1 <= n) load_stage(i + kStages - 1);
           }
           products(i, kYes, kYes);  // behind the last tile's values, scores of no use
           if constexpr (LATE && LOADS) {
             if (i + 1 <= n) store_stage(i + 1);
             interval_end<true>();
-            arrived();
           } else {
             interval_end<false>();
           }
@@ -666,11 +687,10 @@ template <int D, int CACHE>
 LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths,
                             const int32_t *page_offsets, const uint8_t *attn, uint16_t *out, uint8_t *ws) {
   using P = Prompts<D>;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int64_t prefix[kMostSequences + 1];
   __shared__ int slots[P::kBlocks], counted[4], own;
   const Desc &d = desc_of(attn);
   if (d.magic != kMagic) return;
-  int64_t *prefix = reinterpret_cast<int64_t *>(lds);
   bool bad = false;  // reported by the launch before
   const PromptPlan plan = plan_of<D, 256>(d, counts, row_offsets, lengths, page_offsets, prefix, bad);
   const int range = blockIdx.x / kJoinSlices, slice = blockIdx.x % kJoinSlices;
