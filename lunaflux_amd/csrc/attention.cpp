@@ -244,7 +244,7 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
       break;
     case LF_FP8_ATTN_PREFILL:
       gx = kPromptBlocks;
-      lds = (d->cache == LF_FP8_CACHE_BF16 ? 3 : 2) * 2 * prompt_keys(d) * d->head_dim * 2;
+      lds = 6 * prompt_keys(d) * d->head_dim * 2;
       std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_prefill_d%d_%s", d->head_dim, type);
       break;
     case LF_FP8_ATTN_PREFILL_JOIN:

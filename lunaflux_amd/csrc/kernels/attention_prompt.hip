@@ -158,6 +158,18 @@ LF_DEVICE void load_to_lds(const uint8_t *src, uint32_t lds) {
                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "m0");
 }
+// The same for 4 bytes a lane.
+LF_DEVICE void load_word_to_lds(const float *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+               :
+               : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "m0");
+}
+// All but the last LEFT of this wave's loads to LDS have arrived.
+template <int LEFT>
+LF_DEVICE void loads_arrived() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
 #pragma clang diagnostic pop
 LF_DEVICE uint32_t lds_at(const uint8_t *p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t *)p));
@@ -245,10 +257,11 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
   if (d.magic != kMagic) return;
   int *error = reinterpret_cast<int *>(ws);
   // Stage i: the keys of tile i and the values of tile i - 1. Three of them where tiles go straight to LDS, so that
-  // two are on their way.
+  // two are on their way; of codes two, and two more of the codes themselves, which their waves convert.
   constexpr int kStages = E4M3 ? 2 : 3;
   __shared__ int64_t prefix[kMostSequences + 1];
-  const uint32_t stages_at = lds_at(stages);
+  __shared__ float code_scales[CACHE == kCacheBlocks ? 2 * 2 * P::kThreads : 1];
+  const uint32_t stages_at = lds_at(stages), codes_at = stages_at + 4 * P::kTileBytes, scales_at = lds_at(reinterpret_cast<const uint8_t *>(code_scales));
   auto keys_at = [&](int i) { return stages_at + i % kStages * 2 * P::kTileBytes; };
   auto values_at = [&](int i) { return stages_at + (i + 1) % kStages * 2 * P::kTileBytes + P::kTileBytes; };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -270,6 +283,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
   constexpr uint32_t kSize = E4M3 ? 1 : 2;
   const uint32_t page_bytes = static_cast<uint32_t>(d.page_stride) * kSize, token_bytes = static_cast<uint32_t>(d.token_stride) * kSize;
   const uint32_t head_bytes = static_cast<uint32_t>(d.head_stride) * kSize;
+  const int64_t d_block_scales = d.block_scales;
 
   PromptPair pair = pair_at(d, plan, row_offsets, lengths, page_offsets, prefix, u0);
   for (;;) {
@@ -286,8 +300,9 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       const int n = k1 - k0;
       auto base_of = [&](int i) { return kKeys * (k0 + i < pk.sink_tiles ? k0 + i : k0 + i + pk.first - pk.sink_tiles); };
 
-      // Tiles are loaded by the first group's waves, or by all of them where codes are converted on the way.
-      constexpr int kLoaders = E4M3 ? P::kWaves : P::kWaves / 2, kWaveKeys = kKeys / kLoaders, kGroups = (kWaveKeys + 7) / 8;
+      // Tiles are loaded by the first group's waves, or by all of them where codes are converted (of heads of 64 keys
+      // by the first group's and values by the second's); kLoaders waves share a tile's rows.
+      constexpr int kLoaders = E4M3 && D != 64 ? P::kWaves : P::kWaves / 2, kWaveKeys = kKeys / kLoaders, kGroups = (kWaveKeys + 7) / 8;
       // Pages of the groups of eight keys of a tile that are this wave's to load, by scalar loads, so that no wait
       // for them is one for the tiles on their way (they share a counter with LDS reads, so they are on their way
       // only during a softmax). One that the cache does not have is read as page 0: the
@@ -330,55 +345,57 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
           load_to_lds(page + (static_cast<uint64_t>(static_cast<uint32_t>(slot_of(base, key))) * token_bytes + 16 * from), to + (first + r) * D * 2);
         }
       };
-      // e4m3: through registers, 16 codes of a row or 8.
-      constexpr int kCodes = kKeys * D / P::kThreads, kWords = kCodes / 4;
+      // e4m3: a thread's 16 codes of a row of keys and of one of values (heads of 64: of either, by the wave's group).
+      constexpr int kSides = D == 64 ? 1 : 2, kKeyLanes = D / 16, kSideBytes = kKeys * D;
+      const int code_thread = D == 64 ? static_cast<int>(threadIdx.x) & 255 : static_cast<int>(threadIdx.x);
+      const int code_key = code_thread / kKeyLanes, code_at = code_thread % kKeyLanes;
+      auto load_codes = [&](const uint8_t *head, const uint8_t *cache, bool value, int stage, int base, const int (&of_groups)[kGroups]) {
+        const int p = kGroups == 2 && (code_key & 8) != 0 ? of_groups[kGroups - 1] : of_groups[0];
+        const int slot = slot_of(base, code_key), place = (stage & 1) * 2 + value;
+        load_to_lds(head + (row_byte(p, slot, page_bytes, token_bytes) + 16 * code_at), codes_at + place * kSideBytes + (code_thread & ~63) * 16);
+        if constexpr (CACHE == kCacheBlocks) {
+          load_word_to_lds(reinterpret_cast<const float *>(cache + d_block_scales) + scale_index(d, p, slot, h),
+                           scales_at + place * P::kThreads * 4 + (code_thread & ~63) * 4);
+        }
+      };
       struct Codes {
-        uint32_t w[kWords];
+        u32x4 w;
         float scale;
       };
-      const int code_key = static_cast<int>(threadIdx.x) / (D / kCodes), code_at = static_cast<int>(threadIdx.x) % (D / kCodes);
-      auto load_codes = [&](const uint8_t *cache, const uint8_t *table_of, int i, int p, Codes &x) {
-        const int slot = slot_of(base_of(i), code_key);
-        const uint32_t *src = reinterpret_cast<const uint32_t *>(cache + row_byte(p, slot, page_bytes, token_bytes) + kCodes * code_at);
-        if constexpr (kWords == 4) {
-          const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x.w[e] = w[e];
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2 *>(src);
-          x.w[0] = w.x;
-          x.w[1] = w.y;
-        }
+      auto read_codes = [&](bool value, int stage, Codes &x) {
+        const int place = (stage & 1) * 2 + value;
+        x.w = lds_read<u32x4>(codes_at + place * kSideBytes + code_thread * 16);
         x.scale = 1.0f;
-        if constexpr (CACHE == kCacheBlocks) x.scale = reinterpret_cast<const float *>(table_of + d.block_scales)[scale_index(d, p, slot, h)];
+        if constexpr (CACHE == kCacheBlocks) x.scale = lds_read<float>(scales_at + (place * P::kThreads + code_thread) * 4);
       };
-      auto store_codes = [&](uint32_t to, const Codes &x) {
-        uint32_t b[2 * kWords];
+      auto convert = [&](const Codes &x, uint32_t to) {
+        uint32_t b[8];
 #pragma unroll
-        for (int e = 0; e < kWords; ++e) {
+        for (int e = 0; e < 4; ++e) {
           b[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(x.w[e]), x.scale, false));
           b[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(x.w[e]), x.scale, true));
         }
-#pragma unroll
-        for (int e = 0; e < 2 * kWords; e += 4)
-          lds_write(to + tile_byte<D>(code_key, (kCodes * code_at + 2 * e) / 8), u32x4{b[e], b[e + 1], b[e + 2], b[e + 3]});
+        lds_write(to + tile_byte<D>(code_key, 2 * code_at), u32x4{b[0], b[1], b[2], b[3]});
+        lds_write(to + tile_byte<D>(code_key, 2 * code_at + 1), u32x4{b[4], b[5], b[6], b[7]});
       };
-      Codes next_keys, next_values;
-      // Begins to load stage i <= n, and for e4m3 stores it (the last one's keys: those of the last tile, of no use).
+      // Begins to load stage i (behind the last tile the last one's keys, of no use).
       auto load_stage = [&](int i) {
-        if constexpr (E4M3) {
-          load_codes(head_keys, kc, i < n ? i : n - 1, tile_pages[0][0], next_keys);
-          if (i > 0) load_codes(head_values, vc, i - 1, tile_pages[1][0], next_values);
+        const int key_base = base_of(i < n ? i : n - 1), value_base = base_of(i > 0 ? i - 1 : 0);
+        if constexpr (!E4M3) {
+          load_tile(head_keys, keys_at(i), key_base, tile_pages[0]);
+          if (i > 0) load_tile(head_values, values_at(i - 1), value_base, tile_pages[1]);
         } else {
-          load_tile(head_keys, keys_at(i), base_of(i < n ? i : n - 1), tile_pages[0]);
-          if (i > 0) load_tile(head_values, values_at(i - 1), base_of(i - 1), tile_pages[1]);
+          if (kSides == 2 || !late) load_codes(head_keys, kc, false, i, key_base, tile_pages[0]);
+          if (kSides == 2 || late) load_codes(head_values, vc, true, i, value_base, tile_pages[1]);
         }
       };
-      auto store_stage = [&](int i) {
-        if constexpr (E4M3) {
-          store_codes(keys_at(i), next_keys);
-          if (i > 0) store_codes(values_at(i - 1), next_values);
-        }
+      // Codes that have arrived to their places as bf16 values.
+      auto convert_stage = [&](int i) {
+        Codes keys, values;
+        if (kSides == 2 || !late) read_codes(false, i, keys);
+        if (i > 0 && (kSides == 2 || late)) read_codes(true, i, values);
+        if (kSides == 2 || !late) convert(keys, keys_at(i));
+        if (i > 0 && (kSides == 2 || late)) convert(values, values_at(i - 1));
       };
 
       // this lane's row: query operand, position, statistics
@@ -404,15 +421,25 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       int redo;
       f32x16 o[kBands];
       do {
-      const bool loads = wave < kLoaders;
+      const bool loads = E4M3 || !late;
+      constexpr int kStageLoads = E4M3 ? kSides * (CACHE == kCacheBlocks ? 2 : 1) : 2 * kWaveKeys * (D / 8) / 64;
       if (loads) {
         pages_of_tile(0);
         arrived();
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) tile_pages[1][g] = tile_pages[0][g];  // stage 0 of codes has values too, of no use
         pages_of_tile(1);
         load_stage(0);
-        if constexpr (E4M3) store_stage(0);
         arrived();
         load_stage(1);
+        if constexpr (E4M3) {
+          pages_of_tile(2);
+          loads_arrived<kStageLoads>();
+          convert_stage(0);
+          arrived();
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes of stage 0 have been read
+          if (2 <= n) load_stage(2);
+        }
       }
       top = seen;
       sum = 0.0f;
@@ -420,8 +447,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       for (int b = 0; b < kBands; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-      if (loads) store_stage(1);
-      interval_end<true>();
+      interval_end<!E4M3>();
       if (threadIdx.x == 0) once_more = 0;  // every wave has read it by now
 
       u32x4 weights[2 * KT];
@@ -537,54 +563,60 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
 #pragma unroll
         for (int e = 0; e < 2 * KT; ++e) asm volatile("" : "+v"(weights[e]));  // here, not with the products
       };
-      // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. A
-      // stage's place is free when the first group begins the products two stages later (three: two before the
-      // stage), which the second begins a softmax with, and it has to be there one interval before its own.
+      // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. Stage i
+      // is read in the products i of both groups. Its place is free once the first group begins products i + 1,
+      // for which the stage after has to be there: the first group then loads stage i + 3 into it, or both turn
+      // the codes of stage i + 2 into it in their products i + 1 and load those of stage i + 4.
       // (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
-      constexpr int kStageLoads = 2 * kWaveKeys * (D / 8) / 64;
       auto tiles = [&](auto behind) {
         constexpr bool LATE = decltype(behind)::value, LOADS = !LATE || E4M3;
-        // the stage that is loaded next once softmax i is over: kNext after i
-        constexpr int kNext = LATE || !E4M3 ? 3 : 2;
-        if constexpr (LOADS && kNext == 3) {
-          pages_of_tile(2);
+        auto convert_next = [&](int i) {  // beside the other group's products i or its own
+          if (i + 1 <= n) {
+            if (i + 2 <= n) {
+              loads_arrived<kStageLoads>();
+            } else {
+              loads_arrived<0>();
+            }
+            convert_stage(i + 1);
+          }
+          if (i + 3 <= n) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes of stage i + 1 have been read
+            load_stage(i + 3);
+          }
+        };
+        if constexpr (LOADS) {
+          pages_of_tile(E4M3 ? 3 : 2);
           arrived();
         }
-        if constexpr (LATE) {
-          interval_end<false>();
-        } else if constexpr (!E4M3) {
+        if constexpr (LATE) interval_end<false>();
+        if constexpr (!LATE && !E4M3) {
           if (2 <= n) load_stage(2);
         }
         products(0, kNo, kYes);
+        if constexpr (LATE && E4M3) convert_next(0);
         interval_end<false>();
         for (int i = 0; i < n;) {
-          if constexpr (LATE && LOADS) {
-            if (i + 2 <= n) load_stage(i + 2);
-          }
-          if constexpr (LOADS) pages_of_tile(i + kNext);
+          if constexpr (LOADS && !(E4M3 && !LATE)) pages_of_tile(i + (E4M3 ? 4 : 3));
           softmax(i);
           if constexpr (!LATE && E4M3) {
-            if (i > 0) store_stage(i + 1);
+            convert_next(i);
+            pages_of_tile(i + 4);
           }
           if constexpr (LOADS) arrived();
-          if constexpr (LATE) {
+          if constexpr (E4M3 || LATE) {
             interval_end<false>();
-          } else if (!E4M3 && i + 2 <= n) {
+          } else if (i + 2 <= n) {
             interval_end<true, kStageLoads>();
           } else {
             interval_end<true>();
           }
           ++i;
-          if constexpr (!LATE) {
-            if (i + kStages - 1 <= n) load_stage(i + kStages - 1);
+          if constexpr (!LATE && !E4M3) {
+            if (i + 2 <= n) load_stage(i + 2);
           }
           products(i, kYes, kYes);  // behind the last tile's values, scores of no use
-          if constexpr (LATE && LOADS) {
-            if (i + 1 <= n) store_stage(i + 1);
-            interval_end<true>();
-          } else {
-            interval_end<false>();
-          }
+          if constexpr (LATE && E4M3) convert_next(i);
+          interval_end<false>();
         }
         if constexpr (!LATE) interval_end<false>();
       };
