@@ -570,7 +570,10 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
       // (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
       auto tiles = [&](auto behind) {
         constexpr bool LATE = decltype(behind)::value, LOADS = !LATE || E4M3;
-        auto convert_next = [&](int i) {  // beside the other group's products i or its own
+        // Converts stage i + 1, and loads stage i + 3: the first group behind softmax i, the second behind its
+        // products i, or, where products are the longer part, behind the softmax before them.
+        constexpr bool kEarly = E4M3 && LATE && D == 256;
+        auto convert_next = [&](int i) {
           if (i + 1 <= n) {
             if (i + 2 <= n) {
               loads_arrived<kStageLoads>();
@@ -588,12 +591,13 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
           pages_of_tile(E4M3 ? 3 : 2);
           arrived();
         }
+        if constexpr (kEarly) convert_next(0);
         if constexpr (LATE) interval_end<false>();
         if constexpr (!LATE && !E4M3) {
           if (2 <= n) load_stage(2);
         }
         products(0, kNo, kYes);
-        if constexpr (LATE && E4M3) convert_next(0);
+        if constexpr (LATE && E4M3 && !kEarly) convert_next(0);
         interval_end<false>();
         for (int i = 0; i < n;) {
           if constexpr (LOADS && !(E4M3 && !LATE)) pages_of_tile(i + (E4M3 ? 4 : 3));
@@ -603,6 +607,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
             pages_of_tile(i + 4);
           }
           if constexpr (LOADS) arrived();
+          if constexpr (kEarly) convert_next(i + 1);
           if constexpr (E4M3 || LATE) {
             interval_end<false>();
           } else if (i + 2 <= n) {
@@ -615,7 +620,7 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
             if (i + 2 <= n) load_stage(i + 2);
           }
           products(i, kYes, kYes);  // behind the last tile's values, scores of no use
-          if constexpr (LATE && E4M3) convert_next(i);
+          if constexpr (LATE && E4M3 && !kEarly) convert_next(i);
           interval_end<false>();
         }
         if constexpr (!LATE) interval_end<false>();
