@@ -513,7 +513,7 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
 /*
  * The steps from the packed Q|K|V rows of a QKV projection to the rows the
  * output projection reads, over a paged key / value cache:
- *  lf_attn_qk_norm_rope_{bf16,e4m3,e4m3_blocks}
+ *  lf_attn_qk_norm_rope_{bf16,e4m3,e4m3_blocks_d64,_d128,_d256}
  *      (counts, positions, row_offsets, lengths, page_offsets, page_indices,
  *       attn, qkv, gq, gk, q, k_cache, v_cache, status)
  *  lf_attn_decode_d{64,128,256}_{bf16,bf16_sinks,e4m3,e4m3_sinks,e4m3_blocks}

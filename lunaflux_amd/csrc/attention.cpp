@@ -234,7 +234,11 @@ int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc 
   switch (entry) {
     case LF_FP8_ATTN_QK_NORM_ROPE:
       gx = d->max_tokens + (d->cache == LF_FP8_CACHE_E4M3_BLOCKS ? append_blocks(d) : 0);
-      std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_qk_norm_rope_%s", type);
+      if (d->cache == LF_FP8_CACHE_E4M3_BLOCKS) {
+        std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_qk_norm_rope_%s_d%d", type, d->head_dim);
+      } else {
+        std::snprintf(symbol, LF_FP8_SYMBOL_BYTES, "lf_attn_qk_norm_rope_%s", type);
+      }
       break;
     case LF_FP8_ATTN_DECODE:
       gx = decode_blocks(d);

@@ -139,7 +139,7 @@ LF_DEVICE float2 turn_of(const Desc &d, const uint8_t *attn, const int32_t *posi
 // Keys and values of the rows go to the cache too (CACHE kCacheBf16, kCacheE4m3), or are
 // append_blocks' part (kCacheBlocks).
 template <int CACHE>
-LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, const int32_t *row_offsets,
+LF_DEVICE void qk_norm_rope(int row, const int32_t *counts, const int32_t *positions, const int32_t *row_offsets,
                             const int32_t *lengths, const int32_t *page_offsets, const int32_t *page_indices,
                             const uint8_t *attn, const uint16_t *qkv, const uint16_t *gq, const uint16_t *gk,
                             uint16_t *q, uint8_t *kc, uint8_t *vc, int *status) {
@@ -147,7 +147,6 @@ LF_DEVICE void qk_norm_rope(const int32_t *counts, const int32_t *positions, con
   const Desc &d = desc_of(attn);
   if (d.magic != kMagic) return;
   const int rows = live_rows(counts, d.max_tokens);
-  const int row = blockIdx.x;
   if (row >= rows) return;
   int sequences = counts[2];
   sequences = sequences < 0 ? 0 : sequences > d.max_sequences ? d.max_sequences : sequences;
@@ -302,6 +301,7 @@ LF_DEVICE void append_rows(const Desc &d, const uint16_t *qkv, const uint16_t *g
   if (lane == 0) *scales = scale;
 }
 
+template <int D>
 LF_DEVICE void append_blocks(const int32_t *counts, const int32_t *positions, const int32_t *row_offsets,
                              const int32_t *lengths, const int32_t *page_offsets, const int32_t *page_indices,
                              const uint8_t *attn, const uint16_t *qkv, const uint16_t *gk, uint8_t *kc, uint8_t *vc,
@@ -344,7 +344,7 @@ LF_DEVICE void append_blocks(const int32_t *counts, const int32_t *positions, co
   }
   const int Hkv = d.kv_heads, groups = (Hkv + 3) / 4;
   const int64_t items = carry * 2 * groups;
-  for (int64_t u = blockIdx.x - d.max_tokens; u < items; u += gridDim.x - d.max_tokens) {
+  for (int64_t u = blockIdx.x; u < items; u += gridDim.x - d.max_tokens) {
     const int b = static_cast<int>(u / (2 * groups)), unit = static_cast<int>(u - static_cast<int64_t>(b) * 2 * groups);
     const bool value = unit >= groups;
     int s = 0;  // the last with prefix[s] <= b, so one with blocks
@@ -376,13 +376,7 @@ LF_DEVICE void append_blocks(const int32_t *counts, const int32_t *positions, co
     const int h = (value ? unit - groups : unit) * 4 + wave;
     if (h >= Hkv) continue;
     uint8_t *cache = value ? vc : kc;
-    if (d.head_dim == 64) {
-      append_rows<64>(d, qkv, gk, turn, x, page, h, value, cache);
-    } else if (d.head_dim == 128) {
-      append_rows<128>(d, qkv, gk, turn, x, page, h, value, cache);
-    } else {
-      append_rows<256>(d, qkv, gk, turn, x, page, h, value, cache);
-    }
+    append_rows<D>(d, qkv, gk, turn, x, page, h, value, cache);
   }
   if (bad) flag_error(status);
 }
@@ -1123,27 +1117,38 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
 
 }  // namespace attn
 
-#define LF_ATTN_ROPE(TYPE, CACHE)                                                                              \
-  extern "C" __global__ __launch_bounds__(256, CACHE == attn::kCacheBf16 ? 8 : CACHE == attn::kCacheE4m3 ? 7 : 3) void lf_attn_qk_norm_rope_##TYPE( \
-      const int32_t *__restrict__ counts, const int32_t *__restrict__ positions,                               \
+#define LF_ATTN_ROPE_ARGUMENTS                                                                                 \
+  const int32_t *__restrict__ counts, const int32_t *__restrict__ positions,                                   \
       const int32_t *__restrict__ row_offsets, const int32_t *__restrict__ lengths,                            \
       const int32_t *__restrict__ page_offsets, const int32_t *__restrict__ page_indices,                      \
       const uint8_t *__restrict__ desc, const uint16_t *__restrict__ qkv,                                      \
       const uint16_t *__restrict__ gq, const uint16_t *__restrict__ gk, uint16_t *__restrict__ q,              \
-      uint8_t *__restrict__ kc, uint8_t *__restrict__ vc, int *__restrict__ status) {                          \
-    if constexpr (CACHE == attn::kCacheBlocks) {                                                               \
-      if (static_cast<int>(blockIdx.x) >= attn::desc_of(desc).max_tokens) {                                    \
-        attn::append_blocks(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv,    \
-                            gk, kc, vc, status);                                                               \
-        return;                                                                                                \
-      }                                                                                                        \
-    }                                                                                                          \
-    attn::qk_norm_rope<CACHE>(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv,  \
-                              gq, gk, q, kc, vc, status);                                                      \
+      uint8_t *__restrict__ kc, uint8_t *__restrict__ vc, int *__restrict__ status
+#define LF_ATTN_ROPE(TYPE, CACHE)                                                                              \
+  extern "C" __global__ __launch_bounds__(256, CACHE == attn::kCacheBf16 ? 8 : 7)                              \
+  void lf_attn_qk_norm_rope_##TYPE(LF_ATTN_ROPE_ARGUMENTS) {                                                   \
+    attn::qk_norm_rope<CACHE>(blockIdx.x, counts, positions, row_offsets, lengths, page_offsets, page_indices, \
+                              desc, qkv, gq, gk, q, kc, vc, status);                                           \
   }
 LF_ATTN_ROPE(bf16, attn::kCacheBf16)
 LF_ATTN_ROPE(e4m3, attn::kCacheE4m3)
-LF_ATTN_ROPE(e4m3_blocks, attn::kCacheBlocks)
+
+// The first blocks of the grid write the cache, the last max_tokens the queries.
+#define LF_ATTN_ROPE_BLOCKS(D)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256)                                                                 \
+  void lf_attn_qk_norm_rope_e4m3_blocks_d##D(LF_ATTN_ROPE_ARGUMENTS) {                                         \
+    const int row = static_cast<int>(blockIdx.x) - static_cast<int>(gridDim.x) + attn::desc_of(desc).max_tokens; \
+    if (row < 0) {                                                                                             \
+      attn::append_blocks<D>(counts, positions, row_offsets, lengths, page_offsets, page_indices, desc, qkv,   \
+                             gk, kc, vc, status);                                                              \
+    } else {                                                                                                   \
+      attn::qk_norm_rope<attn::kCacheBlocks>(row, counts, positions, row_offsets, lengths, page_offsets,       \
+                                             page_indices, desc, qkv, gq, gk, q, kc, vc, status);              \
+    }                                                                                                          \
+  }
+LF_ATTN_ROPE_BLOCKS(64)
+LF_ATTN_ROPE_BLOCKS(128)
+LF_ATTN_ROPE_BLOCKS(256)
 
 #define LF_ATTN_DECODE(D, TYPE, ...)                                                                           \
   extern "C" __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void lf_attn_decode_d##D##_##TYPE(            \
