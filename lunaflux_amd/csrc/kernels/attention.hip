@@ -130,7 +130,7 @@ LF_DEVICE void turn_head(const HeadLane &w, const float (&c)[8], const float (&s
 LF_DEVICE float2 turn_of(const Desc &d, const uint8_t *attn, const int32_t *positions, int row, int i) {
   const double *turns = reinterpret_cast<const double *>(attn + d.turns_offset);
   const int32_t *axis = reinterpret_cast<const int32_t *>(attn + d.axis_offset);
-  const double t = static_cast<double>(positions[static_cast<int64_t>(row) * d.axes + axis[i]]) * turns[i];
+  const double t = static_cast<double>(positions[row * d.axes + axis[i]]) * turns[i];
   float sin_t, cos_t;
   sincospif(static_cast<float>(2.0 * (t - rint(t))), &sin_t, &cos_t);
   return make_float2(cos_t, sin_t);
@@ -628,12 +628,14 @@ LF_DEVICE float max_over_groups(float v) {
 // A part of a pair: the tiles of keys [base, stop) of a sequence whose keys [lo,
 // len) count, stop at most len, for `live` query heads from head `row0` of key
 // head h's group on.
-struct Piece {
+struct PlainPiece {
   const int32_t *table;
   int lo, len, base, stop;
   int h, row0, live, row;  // row of q and out, or -1
   int pair, tiles;         // its pair's first item and tiles
-  int sink, edge, jump;    // the first keys that count too; from `edge` on, keys are `jump` further
+};
+struct SinkPiece : PlainPiece {
+  int sink, edge, jump;  // the first keys that count too; from `edge` on, keys are `jump` further
 };
 
 // What a block keeps of each of the first sequences in LDS.
@@ -654,6 +656,7 @@ template <int D, bool E4M3, bool BLOCKS, bool SINKS>
 LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths,
                       const int32_t *page_offsets, const int32_t *page_indices, const uint8_t *attn,
                       const uint16_t *q, uint16_t *out, const uint8_t *kc, const uint8_t *vc, uint8_t *ws) {
+  using Piece = std::conditional_t<SINKS, SinkPiece, PlainPiece>;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   __shared__ int wave_total[kWaves], wave_long[kWaves];
   __shared__ int arrived;
@@ -810,11 +813,20 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
     return false;
   };
   // the key that a tile counted along the piece begins with
-  auto key_of = [&](const Piece &x, int base) { return SINKS ? base + (base >= x.edge ? x.jump : 0) : base; };
-  auto indices = [&](const Piece &x, int base) {
-    const int j = key_of(x, base) + 8 * (lane & 3), first = x.lo >> shift, end = (x.len + slot_mask) >> shift;
-    if constexpr (SINKS) return x.table[sink_entry_of((x.sink + slot_mask) >> shift, first, end, shift, j)];
-    return x.table[entry_of(first, end, shift, j)];
+  auto key_of = [&](const Piece &x, int base) {
+    if constexpr (SINKS) base += base >= x.edge ? x.jump : 0;
+    return base;
+  };
+  auto indices = [&](const int32_t *table, int lo, int len, int base) {
+    return table[entry_of(lo >> shift, (len + slot_mask) >> shift, shift, base + 8 * (lane & 3))];
+  };
+  auto pages_at = [&](const Piece &x, int base) {
+    if constexpr (SINKS) {
+      return x.table[sink_entry_of((x.sink + slot_mask) >> shift, x.lo >> shift, (x.len + slot_mask) >> shift, shift,
+                                   key_of(x, base) + 8 * (lane & 3))];
+    } else {
+      return indices(x.table, x.lo, x.len, base);
+    }
   };
   auto tile_groups = [&](int page, int base) {
     return groups_of(page, pages, page_bytes, token_bytes, slot_mask, base);
@@ -866,19 +878,19 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       return 1.0f;
     }
   };
-  const int first_page = indices(now, now.base);
+  const int first_page = pages_at(now, now.base);
   Groups at = tile_groups(first_page, key_of(now, now.base));
   load_keys(x, keys_of(now.h), at, c);
   steps = load_steps(first_page, now.h, key_of(now, now.base));
   load_queries(now);
-  int ahead = indices(now, now.base + kStep);
+  int ahead = pages_at(now, now.base + kStep);
   asm volatile("" ::: "memory");  // values last, as in the loop
   load_values(x, values_of(now.h), at, token_bytes, g);
   bool has_next = take_mine(next);
   if (!has_next) next = now;  // what is loaded behind the last tile
   auto after_one_tile = [&]() {  // a piece of one tile: the tile ahead is the next piece's
     if (now.base + kStep >= now.stop) {
-      ahead = indices(next, next.base);
+      ahead = pages_at(next, next.base);
       asm volatile("" : "+v"(ahead));  // waited for here, not where every tile's is
     }
   };
@@ -932,10 +944,10 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       {
         const bool same = base + 2 * kStep < now.stop;
         if constexpr (SINKS) {
-          ahead = indices(same ? now : next, same ? base + 2 * kStep : more ? next.base : next.base + kStep);
+          ahead = pages_at(same ? now : next, same ? base + 2 * kStep : more ? next.base : next.base + kStep);
         } else {
-          Piece of = same ? now : next;
-          ahead = indices(of, same ? base + 2 * kStep : more ? next.base : next.base + kStep);
+          ahead = indices(same ? now.table : next.table, same ? now.lo : next.lo, same ? now.len : next.len,
+                          same ? base + 2 * kStep : more ? next.base : next.base + kStep);
         }
       }
       float z[8];
@@ -943,11 +955,13 @@ LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const i
       for (int e = 0; e < 8; ++e) z[e] = sc[e >> 2][e & 3] * (BLOCKS ? factor * step[0][e >> 2] : factor);
       if (at.in != 15 && base < now.stop) bad = true;
       const int key = key_of(now, base);
-      if ((key < now.lo && (!SINKS || key + kTileKeys > now.sink)) || base + kTileKeys > now.stop || at.in != 15) {
+      int sink = 0;
+      if constexpr (SINKS) sink = now.sink;
+      if ((key < now.lo && (!SINKS || key + kTileKeys > sink)) || base + kTileKeys > now.stop || at.in != 15) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int within = 16 * (e >> 2) + 4 * g + (e & 3), j = key + within;
-          const bool live = (j >= now.lo || (SINKS && j < now.sink)) && base + within < now.stop &&
+          const bool live = (j >= now.lo || (SINKS && j < sink)) && base + within < now.stop &&
                             ((at.in >> (2 * (e >> 2) + (g >> 1))) & 1) != 0;
           z[e] = live ? z[e] : -INFINITY;
           // a weight of zero times what the place holds would let an infinity or NaN through
