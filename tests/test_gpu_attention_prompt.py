@@ -90,6 +90,27 @@ def test_flat_peaked_and_negative_scores(rt, amplitude, scale):
     run(rt, rng, st.make_step(rt, rng, rows=[150], before=[65], page=16, head_dim=128, softmax_scale=scale), amplitude)
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3_blocks"])
+@pytest.mark.parametrize("growing", [True, False])
+def test_scores_that_change_along_the_keys(rt, growing, cache):
+    """Scores that pass the first tile's maximum by far, and ones that fall short of it: later keys are multiples."""
+    rng = np.random.default_rng(15)
+    s = st.make_step(rt, rng, rows=[70, 5], before=[400, 1200], page=16, cache=cache)
+    codes, table = s.codes(s.host["k"])
+    for i in range(2):
+        for j in range(s.before[i] + s.rows[i]):
+            page, slot = s.place(i, j)
+            step = 2.0 ** ((j // 64 if growing else 8 - j // 64) % 9)
+            if table is not None:
+                table[page, slot // 16] = step * 2.0 ** -6
+                continue
+            for h in range(2):
+                at = s.element(page, h, slot)
+                codes[at:at + 64] = synth.bf16_bits(synth.bf16_values(codes[at:at + 64]) * np.float32(step))
+    s.device["k"].copy_from_host(s.host["k"])
+    run(rt, rng, s)
+
+
 def test_many_sequences(rt):
     """More sequences than threads, few rows each."""
     rng = np.random.default_rng(8)
