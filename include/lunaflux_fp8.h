@@ -522,7 +522,7 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
  *  lf_attn_prefill_d{64,128,256}_{bf16,e4m3,e4m3_blocks}
  *      (the same), then, where the geometry has blocks for it,
  *  lf_attn_prefill_join_d{64,128,256}_{bf16,e4m3,e4m3_blocks}
- *      (counts, row_offsets, lengths, page_offsets, attn, out, ws)
+ *      (attn, out, ws)
  *
  * Runtime inputs, int32, in the vocabulary of a paged step (model/plan
  * runtime inputs): counts = StepCounts; row_offsets [total_rows + 1], the
@@ -559,9 +559,10 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
  * decode, the sequences prefill_rows .. prefill_rows + decode_rows - 1, one
  * row each (the first of its range): out[row] = sum_j p_j v_j over the keys j
  * of [max(0, length - window), length) (window 0: all) and, behind a window,
- * of [0, min(sinks, length)), p = softmax of softmax_scale q.k_j. Query head h reads key head h / (Hq / Hkv). The scores
- * and the softmax statistics are fp32; the weights p go to the second product
- * as two bf16 terms (all but 2^-15 of them). A row without keys (or
+ * of [0, min(sinks, length)), p = softmax of softmax_scale q.k_j. Query head h
+ * reads key head h / (Hq / Hkv). The scores and the softmax statistics are fp32;
+ * the weights p go to the second product as two bf16 terms (all but 2^-15 of
+ * them). A row without keys (or
  * all of whose scores are -inf) gives zeros; values at keys that do not count
  * are not read into the sum, whatever they hold. Other rows of out stay as
  * they were.
@@ -590,9 +591,9 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
 enum lf_fp8_attn_cache { LF_FP8_CACHE_BF16 = 1, LF_FP8_CACHE_E4M3 = 2, LF_FP8_CACHE_E4M3_BLOCKS = 3 };
 enum lf_fp8_attn_pairing { LF_FP8_PAIR_HALF = 0, LF_FP8_PAIR_NEIGHBOUR = 1 };
 
-/* E4M3_BLOCKS: scales by blocks of tokens, in the cache regions themselves.
- * The descriptor region: this structure, then (offsets from its start) the
- * cache scales fp32 [2][kv_heads] (keys, values), turns fp64 [rotary_dim / 2]
+/* The descriptor region: this structure, then (offsets from its start) the
+ * cache scales fp32 [2][kv_heads] (keys, values; ones for an E4M3_BLOCKS cache,
+ * whose scales are in the cache regions), turns fp64 [rotary_dim / 2]
  * (turns per position) and axis int32 [rotary_dim / 2]. */
 typedef struct lf_fp8_attn_desc {
   uint32_t magic;

@@ -397,7 +397,8 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     of every row of the step. gq, gk: the norm weights [D], given if and only if
     the layer normalizes its heads. q and the caches may overlap neither each
     other nor what is read. Over an e4m3_blocks cache a step that writes to one
-    page for two sequences, or twice for one, refuses to launch."""
+    page for two sequences, or twice for one, refuses to launch (by what `stage` wrote;
+    where a caller writes the regions by itself, such a page's codes are undefined)."""
     d = layer.desc
     _step_fits(layer, step)
     heads = d.query_heads + 2 * d.kv_heads
@@ -423,19 +424,21 @@ def bind_qk_norm_rope(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
                           scales=step if d.block_tokens else None)
 
 
-def _attention_args(layer: AttentionLayer, step: PagedStep, q: KernelArgument, out: KernelArgument,
-                    k_cache: KernelArgument, v_cache: KernelArgument, ws: Allocation) -> list:
-    """Checked operands of an attention launch; out is at 7."""
+def _attention_args(rt: ProjectionRuntime, entry: int, layer: AttentionLayer, step: PagedStep, q: KernelArgument,
+                    out: KernelArgument, k_cache: KernelArgument, v_cache: KernelArgument) -> tuple:
+    """Checked operands of an attention launch (out is at 7), and its workspace."""
     d = layer.desc
+    _step_fits(layer, step)
     _holds("q", q, 2 * d.max_tokens * d.query_heads * d.head_dim)
     _holds("out", out, 2 * d.max_tokens * d.query_heads * d.head_dim)
     _holds("k_cache", k_cache, layer.cache_bytes)
     _holds("v_cache", v_cache, layer.cache_bytes)
+    ws = _workspace(rt, entry, d)
     args = [_region(step.counts, alignment=4), _region(step.row_offsets, alignment=4), _region(step.lengths, alignment=4),
             _region(step.page_offsets, alignment=4), _region(step.page_indices, alignment=4), layer.region, q, out,
             k_cache, v_cache, _region(ws, alignment=256)]
     _apart("out and what is read", [out], [a for i, a in enumerate(args) if i != 7])
-    return args
+    return args, ws
 
 
 def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedStep, q: KernelArgument,
@@ -444,9 +447,7 @@ def bind_paged_decode(rt: ProjectionRuntime, layer: AttentionLayer, step: PagedS
     rotated) against the cached keys of each, out [max_tokens, Hq D] as the
     output projection reads it. Rows of other sequences stay as they were. out
     may not overlap what is read."""
-    _step_fits(layer, step)
-    ws = _workspace(rt, _abi.ATTN_DECODE, layer.desc)
-    args = _attention_args(layer, step, q, out, k_cache, v_cache, ws)
+    args, ws = _attention_args(rt, _abi.ATTN_DECODE, layer, step, q, out, k_cache, v_cache)
     dims, symbol = launch_geometry(_abi.ATTN_DECODE, layer.desc)
     return BoundAttention([LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)], workspace=ws,
                           keep=[layer, step])
@@ -460,13 +461,18 @@ def bind_paged_prefill(rt: ProjectionRuntime, layer: AttentionLayer, step: Paged
     decoded sequences stay as they were. out may not overlap what is read. One
     launch, or two where the layer's sizes let a row have 1024 keys or more (512
     for heads of 256): then work is split over the keys, and joined. The
-    workspace is 34 to 68 MB then."""
-    _step_fits(layer, step)
-    ws = _workspace(rt, _abi.ATTN_PREFILL, layer.desc)
-    args = _attention_args(layer, step, q, out, k_cache, v_cache, ws)
+    workspace is 35 MB then for heads of 64, 68 of 128 and 135 of 256.
+
+    The rows' statistics are fp32, their weights bf16 in the second product: where
+    values differ freely from key to key, that is as large an error as the
+    rounding of out, and smaller the less they differ. A row that an infinity or a
+    NaN reaches, in keys or values that it counts or in others of its tiles, and a
+    table with pages that the cache does not have take a path without the matrix
+    units, which is right and some 300 times slower."""
+    args, ws = _attention_args(rt, _abi.ATTN_PREFILL, layer, step, q, out, k_cache, v_cache)
     dims, symbol = launch_geometry(_abi.ATTN_PREFILL, layer.desc)
     steps = [LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)]
     join = launch_geometry(_abi.ATTN_PREFILL_JOIN, layer.desc)
     if join is not None:
-        steps.append(LaunchStep(rt.function(join[1]), join[0], KernelArguments([*args[:4], layer.region, out, args[10]]), join[1]))
+        steps.append(LaunchStep(rt.function(join[1]), join[0], KernelArguments([layer.region, out, args[10]]), join[1]))
     return BoundAttention(steps, workspace=ws, keep=[layer, step])

@@ -10,6 +10,9 @@
 #include <cstdio>
 #include <cstring>
 
+#define LF_DEVICE static inline
+#include "kernels/attention_index.h"
+
 namespace {
 
 constexpr int64_t kLimit32 = (int64_t(1) << 31) - 1;
@@ -22,7 +25,6 @@ constexpr int64_t kWaves = 4;
 // kernels/attention_prompt.hip
 constexpr int64_t kPromptBlocks = 256;
 constexpr int64_t kJoinSlices = 8;
-constexpr int64_t kCut = 8;  // attention_index.h
 // Blocks of the append to an E4M3_BLOCKS cache that write keys and values; each goes on
 // in steps of the grid.
 constexpr int64_t kMostAppendBlocks = 1 << 14;
@@ -129,19 +131,13 @@ int64_t decode_bytes(const lf_fp8_attn_desc *d) {
 }
 
 // kernels/attention_prompt.hip: query rows and keys of a block's tiles.
-constexpr int64_t kPromptRows = 256;
+constexpr int kPromptRows = 256;
 int64_t prompt_keys(const lf_fp8_attn_desc *d) { return d->head_dim == 256 ? 32 : 64; }
 
-// Whether a query tile can be cut: it has to have 2 kCut key tiles (attention_index.h).
-bool prompt_cuts(const lf_fp8_attn_desc *d) {
-  int64_t longest = int64_t(d->table_entries) * d->page_size;
-  const int64_t tokens = std::max<int64_t>(1, kPromptRows / (d->query_heads / d->kv_heads));
-  if (d->window > 0) longest = std::min(longest, int64_t(d->window) + tokens + d->sinks + 2 * prompt_keys(d));
-  return (longest + prompt_keys(d) - 1) / prompt_keys(d) >= 2 * kCut;
-}
+bool prompt_cuts(const lf_fp8_attn_desc *d) { return attn::cuts_prompts(*d, kPromptRows, static_cast<int>(prompt_keys(d))); }
 
 // Its workspace: a line with the error word, and, if tiles can be cut, two partial results per block (fp32 [rows][D]
-// sums, maxima and weight sums).
+// sums, maxima and weight sums; the first, of no use, has the starts of the blocks' ranges).
 int64_t prompt_bytes(const lf_fp8_attn_desc *d) {
   return LF_FP8_ATTN_STATUS_BYTES +
          (prompt_cuts(d) ? 2 * kPromptBlocks * kPromptRows * (d->head_dim + 2) * 4 : 0);

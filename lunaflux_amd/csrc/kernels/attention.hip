@@ -236,6 +236,10 @@ LF_DEVICE u32x2 raised(u32x2 codes, float ratio) {
 // registers: their largest magnitude, the scale, the codes. Blocks of the grid take four heads
 // of one block of tokens, found by the number of blocks that the sequences before have. A block
 // of tokens that holds older ones keeps its scale or raises it, and then their codes.
+// HBM bounds it: 8191 rows of 32/8 heads of 128 with norm and rotation 44.6 us with the queries, 4.2 TB/s
+// (a copy of as many bytes 36). The grid's blocks of the cache come before the rows of queries, whose
+// work is shorter, so that the launch does not end with them: 52 us the other way round, with one kernel for
+// all head sizes.
 template <int D>
 LF_DEVICE void append_rows(const Desc &d, const uint16_t *qkv, const uint16_t *gk, const float2 (*turn)[128],
                            const Block &x, int page, int unit_head, bool value, uint8_t *cache) {
@@ -650,8 +654,10 @@ struct Sinks {
 // BLOCKS: an e4m3 cache with scales by blocks of tokens. A lane's keys of a half of the tile
 // lie in one block, so its key scale multiplies the half's scores and its value scale the
 // weights, which are powers of two and leave the weights' mantissas; the sum of the weights
-// takes its ones divided by them. SINKS: Piece's base, stop and the tiles are counted along the
-// keys that are read, the sinks' tiles and then the window's.
+// takes its ones divided by them. 96 sequences of up to 5003 keys, 32/8 heads of 128: 115 us, 1 to 3 more
+// than with scales per head for 1.6 % more bytes and the loads of the scales.
+// SINKS: Piece's base, stop and the tiles are counted along the keys that are read, the sinks' tiles and
+// then the window's (64 sequences, windows of 4093 and 5 sinks in bf16 98 us, HBM at the copy's rate).
 template <int D, bool E4M3, bool BLOCKS, bool SINKS>
 LF_DEVICE void decode(const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths,
                       const int32_t *page_offsets, const int32_t *page_indices, const uint8_t *attn,

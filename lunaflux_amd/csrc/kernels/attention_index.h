@@ -372,11 +372,23 @@ LF_DEVICE int cut_of(int64_t u, int64_t begin, int64_t weight, int tiles) {
   return tiles - c < kCut ? tiles : c;
 }
 
+// Whether the rows of a query tile can count keys enough for it to be cut: 2 kCut key tiles. (The host sizes the
+// workspace and leaves out the join by it. T: Desc, or the structure that it mirrors.)
+template <class T>
+LF_DEVICE bool cuts_prompts(const T &d, int tile_rows, int tile_keys) {
+  const int group = d.query_heads / d.kv_heads;
+  int64_t longest = static_cast<int64_t>(d.table_entries) * d.page_size;
+  const int64_t seen = static_cast<int64_t>(d.window) + (group > tile_rows ? 1 : tile_rows / group) + d.sinks + 2 * tile_keys;
+  if (d.window > 0 && seen < longest) longest = seen;
+  return (longest + tile_keys - 1) / tile_keys >= 2 * kCut;
+}
+
 // Block b of the grid (as many blocks as CUs) takes the b-th range of weight of those with
 // the XCD in the upper bits: neighbours in weight, which share keys, share an XCD's L2.
 LF_DEVICE int range_of_block(int b, int blocks) { return (b & 7) * (blocks >> 3) + (b >> 3); }
 
-// Partial result of range b: of a pair cut before it, or of one that it begins and does not end.
+// Partial result of range b: of a pair cut before it, or of one that it begins and does not end. (The first, of a
+// pair cut before range 0, never is.)
 LF_DEVICE int prompt_slot(int b, bool begun_before) { return 2 * b + (begun_before ? 0 : 1); }
 
 }  // namespace attn

@@ -18,6 +18,21 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 // barriers one group's waves have the products of a tile and the other's its softmax.
 // Blocks are dealt equal ranges of the step's weight (attention_index.h); a query tile cut
 // between ranges leaves fp32 partial results, which a second launch adds up in their order.
+//
+// Weights are rounded to bf16 once, for the second product, and their sum is of the rounded ones, so
+// that equal values come out equal. A weight is off by 2^-9 of itself, as a value of out is: for values
+// without a common part the errors are as large as out's own rounding (1.9e-3 of out in all against 64
+// bits, 1.6e-3 where only out is rounded). A second bf16 term would take that away for half as many
+// products again.
+//
+// Matrix products bound it, with the softmax close behind: of a tile of heads of 128 a wave has 32 products,
+// 1024 cycles of the matrix unit, and some 190 vector instructions, 900 of the vector unit. 8192 rows, 32/8 heads
+// of 128: 551 us, 1.00 PFLOP/s of 1.39 that an 8192^3 product reaches; 49 % of the cycles of the matrix
+// units at the 1.9 GHz that the card holds under it, LDS reads 19-25 % without conflicts. By steps: waves
+// of 16 rows with tiles through registers 1652 us; two groups of waves with 32 rows and loads that go
+// straight to LDS 696; operands read ahead and code of their own for the groups 584; a third stage of
+// tiles 551. Loads issued by the second group instead of the first: 591 at the time of 554. Tiles of 32 keys
+// for heads of 256, whose sums and queries take 192 registers of a lane: 177 us for 2045 rows.
 template <int D>
 struct Prompts {
   static constexpr int kWaves = 8, kThreads = 64 * kWaves, kBlocks = 256;
@@ -140,11 +155,22 @@ LF_DEVICE uint32_t tile_byte(int key, int chunk) {
   return static_cast<uint32_t>(key * D * 2 + ((chunk ^ (chunk_swizzle(key & 15) & (D / 8 - 1))) << 4));
 }
 
-// Partial results, their maxima and their weight sums in the workspace.
+// Partial results, their maxima and their weight sums in the workspace, behind a line with the error word.
 template <int D>
 LF_DEVICE float *partial_of(uint8_t *ws, int slot) {
   return reinterpret_cast<float *>(ws + 256) + static_cast<uint64_t>(slot) * Prompts<D>::kFloats;
 }
+
+// What the join has to know of a range: the first query tile in it, of weights [begin, begin + weight) of the step's.
+// The first launch writes it (weight 0 where the range is empty) in the place of partial result 0, so that the
+// second, of whose blocks a CU holds eight, does not look for it once more: 20 and 9 us for four prompts, 27 and 16
+// for 8192 rows.
+struct RangeStart {
+  int64_t share, begin, weight;
+  int tiles, row0, head0, heads, rows, token_of, h;
+};
+LF_DEVICE RangeStart *start_of(uint8_t *ws, int range) { return reinterpret_cast<RangeStart *>(ws + 256) + range; }
+static_assert(Prompts<64>::kBlocks * sizeof(RangeStart) <= Prompts<64>::kFloats * 4, "");
 
 // One global_load_lds_dwordx4: every lane's 16 bytes from its address go to LDS at lds + 16 lane
 // (wave-uniform; M0). As assembly, so that the compiler does not make every LDS read wait for it:
@@ -198,8 +224,9 @@ LF_DEVICE void interval_end() {
 
 // The rows of a query tile that one wave has, without the matrix units: for rows that some infinity or NaN
 // reached, since in products of tiles zero times such a value of a key that a row does not count is NaN
-// too. Here only the keys that it counts enter. Lanes c and c + 32 hold the halves of row c. Slow, and
-// apart from the kernel's registers.
+// too, and for tables with pages outside the cache. Here only the keys that it counts enter. Lanes c and
+// c + 32 hold the halves of row c. Apart from the kernel's registers, and slow, which such rows bear: a
+// prompt of 8192 rows that all hold a NaN takes 208 ms, 380 times as long as without.
 struct CarefulRow {
   const uint16_t *q;
   const uint8_t *kc, *vc;
@@ -273,7 +300,11 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
   const int range = range_of_block(blockIdx.x, P::kBlocks);
   const int64_t u0 = range * plan.share, u1 = u0 + plan.share < plan.total ? u0 + plan.share : plan.total;
   if (bad) flag_error(error);
-  if (u0 >= u1) return;
+  const bool cuts = cuts_prompts(d, P::kRows, kKeys);
+  if (u0 >= u1) {
+    if (cuts && threadIdx.x == 0) start_of(ws, range)->weight = 0;
+    return;
+  }
 
   const int Hq = d.query_heads, Hkv = d.kv_heads;
   const int shift = __builtin_ctz(d.page_size), slot_mask = d.page_size - 1, pages = d.pages;
@@ -289,10 +320,13 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
   for (;;) {
     const PromptKeys pk = keys_of(d, plan.tile, pair.p, pair.x, kKeys);
     const int k0 = cut_of(u0, pair.begin, pair.weight, pk.tiles), k1 = cut_of(u1, pair.begin, pair.weight, pk.tiles);
+    const PairHeads of = heads_of(d, plan, pair);
+    const int h = of.h, head0 = of.first, heads = of.count, tokens = pk.last - pk.first_position + 1;
+    const int row0 = pair.p.row + pair.x * plan.tile.tokens;
+    if (cuts && pair.begin <= u0 && threadIdx.x == 0) {
+      *start_of(ws, range) = {plan.share, pair.begin, pair.weight, pk.tiles, row0, head0, heads, tokens * heads, plan.token_of, h};
+    }
     if (k0 < k1) {
-      const PairHeads of = heads_of(d, plan, pair);
-      const int h = of.h, head0 = of.first, heads = of.count, tokens = pk.last - pk.first_position + 1;
-      const int row0 = pair.p.row + pair.x * plan.tile.tokens;
       const int32_t *table = page_indices + pair.p.entry;
       const int page_first = pk.lo >> shift, page_end = (pk.last >> shift) + 1, sink_end = (pk.sink + slot_mask) >> shift;
       // (a scale of zero as one that leaves -infinity, a masked score, what it is)
@@ -414,227 +448,230 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
         }
       }
       // Weights are relative to `top`, the row's maximum in the first tile that it counts a key of. It need not be
-      // the row's largest score, only near it: nothing is lost until one is 2^kNear larger. Then the tiles
-      // are gone through once more, with the largest that was seen. So the sums are never scaled.
+      // the row's largest score, only near it: a weight of 2^kNear and sums of 2^31 of them are as exact in fp32
+      // and bf16 as ones. Past that the tiles are gone through once more, with the largest that was seen. So the
+      // sums are never scaled, which would take a multiplication of each for every tile (heads of 128: 64 of a
+      // lane's; with them the kernel did not fit its registers).
       constexpr float kNear = 40.0f;
       float top = -INFINITY, seen = -INFINITY, sum;
       int redo;
       f32x16 o[kBands];
       do {
-      const bool loads = E4M3 || !late;
-      constexpr int kStageLoads = E4M3 ? kSides * (CACHE == kCacheBlocks ? 2 : 1) : 2 * kWaveKeys * (D / 8) / 64;
-      if (loads) {
-        pages_of_tile(0);
-        arrived();
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) tile_pages[1][g] = tile_pages[0][g];  // stage 0 of codes has values too, of no use
-        pages_of_tile(1);
-        load_stage(0);
-        arrived();
-        load_stage(1);
-        if constexpr (E4M3) {
-          pages_of_tile(2);
-          loads_arrived<kStageLoads>();
-          convert_stage(0);
+        const bool loads = E4M3 || !late;
+        constexpr int kStageLoads = E4M3 ? kSides * (CACHE == kCacheBlocks ? 2 : 1) : 2 * kWaveKeys * (D / 8) / 64;
+        if (loads) {
+          pages_of_tile(0);
           arrived();
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes of stage 0 have been read
-          if (2 <= n) load_stage(2);
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) tile_pages[1][g] = tile_pages[0][g];  // stage 0 of codes has values too, of no use
+          pages_of_tile(1);
+          load_stage(0);
+          arrived();
+          load_stage(1);
+          if constexpr (E4M3) {
+            pages_of_tile(2);
+            loads_arrived<kStageLoads>();
+            convert_stage(0);
+            arrived();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes of stage 0 have been read
+            if (2 <= n) load_stage(2);
+          }
         }
-      }
-      top = seen;
-      sum = 0.0f;
+        top = seen;
+        sum = 0.0f;
 #pragma unroll
-      for (int b = 0; b < kBands; ++b)
+        for (int b = 0; b < kBands; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-      interval_end<!E4M3>();
-      if (threadIdx.x == 0) once_more = 0;  // every wave has read it by now
+          for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+        interval_end<!E4M3>();
+        if (threadIdx.x == 0) once_more = 0;  // every wave has read it by now
 
-      u32x4 weights[2 * KT];
-      f32x16 s[KT];
-      // This lane's place in a tile of keys (key c of 32, chunk `half`) and in one of values (key 4 half + .. of
-      // 16, its columns of 32). Other chunks and columns are the place with bits of it flipped, other keys are
-      // further on by a constant, so that a tile's reads share a few addresses.
-      const int l16 = lane & 15, value_key = 4 * half + (l16 >> 2), value_column = 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
-      const uint32_t key_place = tile_byte<D>(c, half), value_place = tile_byte<D>(value_key, value_column / 8) + (value_column % 8) * 2;
-      auto key_words = [&](uint32_t at, int st, int kt) { return lds_read<u32x4>((at ^ (st << 5)) + kt * 32 * D * 2); };
-      // values of keys 16 kk + 4 half + 0 .. 3 and of those 8 further, column 32 b + lane % 32
-      auto value_words = [&](uint32_t at, int kk, int b) {
-        const uint32_t band = at ^ (b << 6);
-        typedef __attribute__((address_space(3))) s16x4 *LdsWords;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)(band + kk * 16 * D * 2));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)((band ^ 32) + (kk * 16 + 8) * D * 2));
-        const uint2 w0 = __builtin_bit_cast(uint2, lo), w1 = __builtin_bit_cast(uint2, hi);
-        return u32x4{w0.x, w0.y, w1.x, w1.y};
-      };
-      auto product = [&](u32x4 a, u32x4 b, f32x16 acc) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
-      };
-      // Products of an interval: V^T P^T of tile i - 1 onto O^T (VALUES), then K Q^T of tile i (SCORES). Operands are
-      // read from LDS kRing products ahead.
-      auto products = [&](int i, auto with_values, auto with_scores) {
-        constexpr bool VALUES = decltype(with_values)::value, SCORES = decltype(with_scores)::value;
-        constexpr int kValues = VALUES ? 2 * KT * kBands : 0, kScores = SCORES ? kSteps * KT : 0;
-        constexpr int kRing = VALUES && D < 256 ? 8 : 4, kKeyRing = 4;
-        uint32_t value_at = VALUES ? values_at(i - 1) + value_place : 0, key_at = SCORES ? keys_at(i) + key_place : 0;
-        asm volatile("" : "+v"(value_at), "+v"(key_at));  // or every address of both stages stays in a register
-        u32x4 v[kRing], k[kKeyRing];
-        if constexpr (VALUES) {
+        u32x4 weights[2 * KT];
+        f32x16 s[KT];
+        // This lane's place in a tile of keys (key c of 32, chunk `half`) and in one of values (key 4 half + .. of
+        // 16, its columns of 32). Other chunks and columns are the place with bits of it flipped, other keys are
+        // further on by a constant, so that a tile's reads share a few addresses.
+        const int l16 = lane & 15, value_key = 4 * half + (l16 >> 2), value_column = 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
+        const uint32_t key_place = tile_byte<D>(c, half), value_place = tile_byte<D>(value_key, value_column / 8) + (value_column % 8) * 2;
+        auto key_words = [&](uint32_t at, int st, int kt) { return lds_read<u32x4>((at ^ (st << 5)) + kt * 32 * D * 2); };
+        // values of keys 16 kk + 4 half + 0 .. 3 and of those 8 further, column 32 b + lane % 32
+        auto value_words = [&](uint32_t at, int kk, int b) {
+          const uint32_t band = at ^ (b << 6);
+          typedef __attribute__((address_space(3))) s16x4 *LdsWords;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)(band + kk * 16 * D * 2));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsWords)((band ^ 32) + (kk * 16 + 8) * D * 2));
+          const uint2 w0 = __builtin_bit_cast(uint2, lo), w1 = __builtin_bit_cast(uint2, hi);
+          return u32x4{w0.x, w0.y, w1.x, w1.y};
+        };
+        auto product = [&](u32x4 a, u32x4 b, f32x16 acc) {
+          return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+        };
+        // Products of an interval: V^T P^T of tile i - 1 onto O^T (VALUES), then K Q^T of tile i (SCORES). Operands are
+        // read from LDS kRing products ahead.
+        auto products = [&](int i, auto with_values, auto with_scores) {
+          constexpr bool VALUES = decltype(with_values)::value, SCORES = decltype(with_scores)::value;
+          constexpr int kValues = VALUES ? 2 * KT * kBands : 0, kScores = SCORES ? kSteps * KT : 0;
+          constexpr int kRing = VALUES && D < 256 ? 8 : 4, kKeyRing = 4;
+          uint32_t value_at = VALUES ? values_at(i - 1) + value_place : 0, key_at = SCORES ? keys_at(i) + key_place : 0;
+          asm volatile("" : "+v"(value_at), "+v"(key_at));  // or every address of both stages stays in a register
+          u32x4 v[kRing], k[kKeyRing];
+          if constexpr (VALUES) {
 #pragma unroll
-          for (int f = 0; f < kRing; ++f) v[f] = value_words(value_at, f / kBands, f % kBands);
-          __builtin_amdgcn_sched_group_barrier(0x100, 2 * kRing, 0);
+            for (int f = 0; f < kRing; ++f) v[f] = value_words(value_at, f / kBands, f % kBands);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * kRing, 0);
+#pragma unroll
+            for (int f = 0; f < kValues; ++f) {
+              o[f % kBands] = product(v[f % kRing], weights[f / kBands], o[f % kBands]);
+              if (f + kRing < kValues) v[f % kRing] = value_words(value_at, (f + kRing) / kBands, (f + kRing) % kBands);
+            }
+          }
+          if constexpr (SCORES) {
+#pragma unroll
+            for (int f = 0; f < kKeyRing; ++f) k[f] = key_words(key_at, f / KT, f % KT);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
+#pragma unroll
+            for (int f = 0; f < kScores; ++f) {
+              s[f % KT] = product(k[f % kKeyRing], qv[f / KT], s[f % KT]);
+              if (f + kKeyRing < kScores) k[f % kKeyRing] = key_words(key_at, (f + kKeyRing) / KT, (f + kKeyRing) % KT);
+            }
+          }
+          // the order: after the first reads, a product, then the reads that its operands' registers are free for
 #pragma unroll
           for (int f = 0; f < kValues; ++f) {
-            o[f % kBands] = product(v[f % kRing], weights[f / kBands], o[f % kBands]);
-            if (f + kRing < kValues) v[f % kRing] = value_words(value_at, (f + kRing) / kBands, (f + kRing) % kBands);
-          }
-        }
-        if constexpr (SCORES) {
-#pragma unroll
-          for (int f = 0; f < kKeyRing; ++f) k[f] = key_words(key_at, f / KT, f % KT);
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
-#pragma unroll
-          for (int f = 0; f < kScores; ++f) {
-            s[f % KT] = product(k[f % kKeyRing], qv[f / KT], s[f % KT]);
-            if (f + kKeyRing < kScores) k[f % kKeyRing] = key_words(key_at, (f + kKeyRing) / KT, (f + kKeyRing) % KT);
-          }
-        }
-        // the order: after the first reads, a product, then the reads that its operands' registers are free for
-#pragma unroll
-        for (int f = 0; f < kValues; ++f) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          if (f + kRing < kValues) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-          else if (SCORES && f + kKeyRing >= kValues) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        if constexpr (SCORES) {
-          if constexpr (!VALUES) __builtin_amdgcn_sched_group_barrier(0x100, kKeyRing, 0);
-#pragma unroll
-          for (int f = 0; f < kScores; ++f) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (f + kKeyRing < kScores) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (f + kRing < kValues) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            else if (SCORES && f + kKeyRing >= kValues) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
-        }
-      };
-      constexpr std::true_type kYes{};
-      constexpr std::false_type kNo{};
-      // positions of the wave's rows
-      const int wave_first = pk.first_position + (wave * 32 < tokens * heads ? (wave * 32 * plan.token_of) >> 16 : 0);
-      const int wave_last = pk.first_position + (wave * 32 + 31 < tokens * heads ? ((wave * 32 + 31) * plan.token_of) >> 16 : tokens - 1);
-      auto softmax = [&](int i) {
-        const int base = base_of(i);
-        float z[16 * KT];
+          if constexpr (SCORES) {
+            if constexpr (!VALUES) __builtin_amdgcn_sched_group_barrier(0x100, kKeyRing, 0);
 #pragma unroll
-        for (int e = 0; e < 16 * KT; ++e) z[e] = s[e / 16][e % 16];
-        if (base + kKeys - 1 > wave_first || (base <= wave_last - window && base + kKeys > sinks)) {
-          // some row does not count some key: it counts those low < j <= to and j < sink (no short circuits: each
-          // would be a branch)
-          const int to = position - base - 4 * half, low = to - window, sink = sinks - base - 4 * half;
-#pragma unroll
-          for (int e = 0; e < 16 * KT; ++e) {
-            const int j = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3);
-            const bool counts = (j <= to) & ((j > low) | (j < sink));
-            z[e] = counts ? z[e] : -INFINITY;
-          }
-        }
-        float most = z[0], other = z[1];
-#pragma unroll
-        for (int e = 2; e < 16 * KT; e += 2) most = fmaxf(most, z[e]), other = fmaxf(other, z[e + 1]);
-        {
-          const uint32_t a = __float_as_uint(fmaxf(most, other));
-          const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-          most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * factor;
-        }
-        seen = fmaxf(seen, most);
-        top = top == -INFINITY ? most : top;
-        const float from = top == -INFINITY ? 0.0f : top;
-        float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int e = 0; e < 8 * KT; ++e) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e], factor, -from));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e + 1], factor, -from));
-          const uint32_t w = pack_bf16(p0, p1);
-          weights[e / 4][e % 4] = w;
-          sums[e & 3] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sums[e & 3], false);
-        }
-        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-#pragma unroll
-        for (int e = 0; e < 2 * KT; ++e) asm volatile("" : "+v"(weights[e]));  // here, not with the products
-      };
-      // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. Stage i
-      // is read in the products i of both groups. Its place is free once the first group begins products i + 1,
-      // for which the stage after has to be there: the first group then loads stage i + 3 into it, or both turn
-      // the codes of stage i + 2 into it in their products i + 1 and load those of stage i + 4.
-      // (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
-      auto tiles = [&](auto behind) {
-        constexpr bool LATE = decltype(behind)::value, LOADS = !LATE || E4M3;
-        // Converts stage i + 1, and loads stage i + 3: the first group behind softmax i, the second behind its
-        // products i, or, where products are the longer part, behind the softmax before them.
-        constexpr bool kEarly = E4M3 && LATE && D == 256;
-        auto convert_next = [&](int i) {
-          if (i + 1 <= n) {
-            if (i + 2 <= n) {
-              loads_arrived<kStageLoads>();
-            } else {
-              loads_arrived<0>();
+            for (int f = 0; f < kScores; ++f) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              if (f + kKeyRing < kScores) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            convert_stage(i + 1);
-          }
-          if (i + 3 <= n) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes of stage i + 1 have been read
-            load_stage(i + 3);
           }
         };
-        if constexpr (LOADS) {
-          pages_of_tile(E4M3 ? 3 : 2);
-          arrived();
-        }
-        if constexpr (kEarly) convert_next(0);
-        if constexpr (LATE) interval_end<false>();
-        if constexpr (!LATE && !E4M3) {
-          if (2 <= n) load_stage(2);
-        }
-        products(0, kNo, kYes);
-        if constexpr (LATE && E4M3 && !kEarly) convert_next(0);
-        interval_end<false>();
-        for (int i = 0; i < n;) {
-          if constexpr (LOADS && !(E4M3 && !LATE)) pages_of_tile(i + (E4M3 ? 4 : 3));
-          softmax(i);
-          if constexpr (!LATE && E4M3) {
-            convert_next(i);
-            pages_of_tile(i + 4);
+        constexpr std::true_type kYes{};
+        constexpr std::false_type kNo{};
+        // positions of the wave's rows
+        const int wave_first = pk.first_position + (wave * 32 < tokens * heads ? (wave * 32 * plan.token_of) >> 16 : 0);
+        const int wave_last = pk.first_position + (wave * 32 + 31 < tokens * heads ? ((wave * 32 + 31) * plan.token_of) >> 16 : tokens - 1);
+        auto softmax = [&](int i) {
+          const int base = base_of(i);
+          float z[16 * KT];
+#pragma unroll
+          for (int e = 0; e < 16 * KT; ++e) z[e] = s[e / 16][e % 16];
+          if (base + kKeys - 1 > wave_first || (base <= wave_last - window && base + kKeys > sinks)) {
+            // some row does not count some key: it counts those low < j <= to and j < sink (no short circuits: each
+            // would be a branch)
+            const int to = position - base - 4 * half, sink = sinks - base - 4 * half;
+            const int low = static_cast<int>(static_cast<uint32_t>(to) - static_cast<uint32_t>(window));  // (of no use for to < 0)
+#pragma unroll
+            for (int e = 0; e < 16 * KT; ++e) {
+              const int j = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3);
+              const bool counts = (j <= to) & ((j > low) | (j < sink));
+              z[e] = counts ? z[e] : -INFINITY;
+            }
           }
-          if constexpr (LOADS) arrived();
-          if constexpr (kEarly) convert_next(i + 1);
-          if constexpr (E4M3 || LATE) {
-            interval_end<false>();
-          } else if (i + 2 <= n) {
-            interval_end<true, kStageLoads>();
-          } else {
-            interval_end<true>();
+          float most = z[0], other = z[1];
+#pragma unroll
+          for (int e = 2; e < 16 * KT; e += 2) most = fmaxf(most, z[e]), other = fmaxf(other, z[e + 1]);
+          {
+            const uint32_t a = __float_as_uint(fmaxf(most, other));
+            const auto x = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+            most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * factor;
           }
-          ++i;
+          seen = fmaxf(seen, most);
+          top = top == -INFINITY ? most : top;
+          const float from = top == -INFINITY ? 0.0f : top;
+          float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int e = 0; e < 8 * KT; ++e) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e], factor, -from));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[2 * e + 1], factor, -from));
+            const uint32_t w = pack_bf16(p0, p1);
+            weights[e / 4][e % 4] = w;
+            sums[e & 3] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sums[e & 3], false);
+          }
+          sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+#pragma unroll
+          for (int e = 0; e < 2 * KT; ++e) asm volatile("" : "+v"(weights[e]));  // here, not with the products
+        };
+        // Intervals of a wave, by its group: products of tile i (and of tile i - 1's values), softmax of tile i. Stage i
+        // is read in the products i of both groups. Its place is free once the first group begins products i + 1,
+        // for which the stage after has to be there: the first group then loads stage i + 3 into it, or both turn
+        // the codes of stage i + 2 into it in their products i + 1 and load those of stage i + 4.
+        // (Code of their own: where paths meet, the compiler waits for what either may have on its way.)
+        auto tiles = [&](auto behind) {
+          constexpr bool LATE = decltype(behind)::value, LOADS = !LATE || E4M3;
+          // Converts stage i + 1, and loads stage i + 3: the first group behind softmax i, the second behind its
+          // products i, or, where products are the longer part, behind the softmax before them.
+          constexpr bool kEarly = E4M3 && LATE && D == 256;
+          auto convert_next = [&](int i) {
+            if (i + 1 <= n) {
+              if (i + 2 <= n) {
+                loads_arrived<kStageLoads>();
+              } else {
+                loads_arrived<0>();
+              }
+              convert_stage(i + 1);
+            }
+            if (i + 3 <= n) {
+              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the codes of stage i + 1 have been read
+              load_stage(i + 3);
+            }
+          };
+          if constexpr (LOADS) {
+            pages_of_tile(E4M3 ? 3 : 2);
+            arrived();
+          }
+          if constexpr (kEarly) convert_next(0);
+          if constexpr (LATE) interval_end<false>();
           if constexpr (!LATE && !E4M3) {
-            if (i + 2 <= n) load_stage(i + 2);
+            if (2 <= n) load_stage(2);
           }
-          products(i, kYes, kYes);  // behind the last tile's values, scores of no use
-          if constexpr (LATE && E4M3 && !kEarly) convert_next(i);
+          products(0, kNo, kYes);
+          if constexpr (LATE && E4M3 && !kEarly) convert_next(0);
           interval_end<false>();
+          for (int i = 0; i < n;) {
+            if constexpr (LOADS && !(E4M3 && !LATE)) pages_of_tile(i + (E4M3 ? 4 : 3));
+            softmax(i);
+            if constexpr (!LATE && E4M3) {
+              convert_next(i);
+              pages_of_tile(i + 4);
+            }
+            if constexpr (LOADS) arrived();
+            if constexpr (kEarly) convert_next(i + 1);
+            if constexpr (E4M3 || LATE) {
+              interval_end<false>();
+            } else if (i + 2 <= n) {
+              interval_end<true, kStageLoads>();
+            } else {
+              interval_end<true>();
+            }
+            ++i;
+            if constexpr (!LATE && !E4M3) {
+              if (i + 2 <= n) load_stage(i + 2);
+            }
+            products(i, kYes, kYes);  // behind the last tile's values, scores of no use
+            if constexpr (LATE && E4M3 && !kEarly) convert_next(i);
+            interval_end<false>();
+          }
+          if constexpr (!LATE) interval_end<false>();
+        };
+        if (late) {
+          tiles(kYes);
+        } else {
+          tiles(kNo);
         }
-        if constexpr (!LATE) interval_end<false>();
-      };
-      if (late) {
-        tiles(kYes);
-      } else {
-        tiles(kNo);
-      }
-      // 1: once more; 2: a page outside the cache
-      const int after = outside ? 2 : __ballot(live && seen > top + kNear) != 0 ? 1 : 0;
-      if (after != 0 && lane == 0) atomicOr(&once_more, after);
-      interval_end<false>();
-      redo = __builtin_amdgcn_readfirstlane(once_more);
+        // 1: once more; 2: a page outside the cache
+        const int after = outside ? 2 : __ballot(live && seen > top + kNear) != 0 ? 1 : 0;
+        if (after != 0 && lane == 0) atomicOr(&once_more, after);
+        interval_end<false>();
+        redo = __builtin_amdgcn_readfirstlane(once_more);
       } while (redo == 1);
       if (redo >= 2) bad = true;
 
@@ -719,27 +756,22 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
 }
 
 // Adds up the parts of the query tiles that were cut: the block of range b and slice k takes its
-// part of the rows of a tile of which range b holds a part that is not its first.
+// part of the rows of a tile of which range b holds a part that is not its first. HBM bounds
+// it where there are many parts: heads of 256, 512 of 2045 rows behind 2500 tokens 20 us for 105 MB, four
+// prompts of up to 2039 rows of heads of 128 9 us, of which a launch that does nothing is 4.
 template <int D, int CACHE>
-LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, const int32_t *lengths,
-                            const int32_t *page_offsets, const uint8_t *attn, uint16_t *out, uint8_t *ws) {
+LF_DEVICE void prefill_join(const uint8_t *attn, uint16_t *out, uint8_t *ws) {
   using P = Prompts<D>;
-  __shared__ int64_t prefix[kMostSequences + 1];
   __shared__ int slots[P::kBlocks], counted[4], own;
   const Desc &d = desc_of(attn);
-  if (d.magic != kMagic) return;
-  bool bad = false;  // reported by the launch before
-  const PromptPlan plan = plan_of<D, 256>(d, counts, row_offsets, lengths, page_offsets, prefix, bad);
   const int range = blockIdx.x / kJoinSlices, slice = blockIdx.x % kJoinSlices;
-  const int64_t u = range * plan.share;
-  if (range == 0 || u >= plan.total) return;
-  const PromptPair pair = pair_at(d, plan, row_offsets, lengths, page_offsets, prefix, u);
-  const PromptKeys pk = keys_of(d, plan.tile, pair.p, pair.x, P::kKeys);
-  auto cut = [&](int b) { return cut_of(b * plan.share, pair.begin, pair.weight, pk.tiles); };
+  const RangeStart tile = *start_of(ws, range);
+  if (d.magic != kMagic || tile.weight == 0) return;
+  auto cut = [&](int b) { return cut_of(b * tile.share, tile.begin, tile.weight, tile.tiles); };
   if (cut(range) == 0 || cut(range) >= cut(range + 1)) return;
 
   // the ranges with a part of the tile, in order
-  const int first = static_cast<int>(pair.begin / plan.share);
+  const int first = static_cast<int>(tile.begin / tile.share);
   const int mine = first + static_cast<int>(threadIdx.x);
   const int from = cut(mine), to = cut(mine + 1);
   const bool some = mine < P::kBlocks && from < to;
@@ -757,11 +789,8 @@ LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, c
   __syncthreads();
   const int worker = (own - 1) * kJoinSlices + slice, workers = (parts - 1) * kJoinSlices;
 
-  const int Hq = d.query_heads;
-  const PairHeads of = heads_of(d, plan, pair);
-  const int h = of.h, head0 = of.first, heads = of.count, rows = (pk.last - pk.first_position + 1) * heads;
-  const int row0 = pair.p.row + pair.x * plan.tile.tokens;
-  const float vscale = CACHE == kCacheE4m3 ? reinterpret_cast<const float *>(attn + d.scale_offset)[d.kv_heads + h] : 1.0f;
+  const int Hq = d.query_heads, head0 = tile.head0, heads = tile.heads, rows = tile.rows, row0 = tile.row0;
+  const float vscale = CACHE == kCacheE4m3 ? reinterpret_cast<const float *>(attn + d.scale_offset)[d.kv_heads + tile.h] : 1.0f;
   constexpr int kQuads = D / 4;
   const int m0 = rows * worker / workers, m1 = rows * (worker + 1) / workers;
   struct Joined {
@@ -776,7 +805,7 @@ LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, c
     x.top = next;
   };
   auto finish = [&](int quad, const Joined &x) {
-    const int m = quad / kQuads, column = quad % kQuads * 4, token = (m * plan.token_of) >> 16;
+    const int m = quad / kQuads, column = quad % kQuads * 4, token = (m * tile.token_of) >> 16;
     const float scale = vscale / x.sum;
     uint2 w = {pack_bf16(x.acc[0] * scale, x.acc[1] * scale), pack_bf16(x.acc[2] * scale, x.acc[3] * scale)};
     if (x.sum == 0.0f) w = {0u, 0u};
@@ -858,10 +887,8 @@ LF_DEVICE void prefill_join(const int32_t *counts, const int32_t *row_offsets, c
                                   vc, ws);                                                                     \
   }                                                                                                            \
   extern "C" __global__ __launch_bounds__(256) void lf_attn_prefill_join_d##D##_##TYPE(                        \
-      const int32_t *__restrict__ counts, const int32_t *__restrict__ row_offsets,                             \
-      const int32_t *__restrict__ lengths, const int32_t *__restrict__ page_offsets,                           \
       const uint8_t *__restrict__ desc, uint16_t *__restrict__ out, uint8_t *__restrict__ ws) {                \
-    attn::prefill_join<D, attn::CACHE>(counts, row_offsets, lengths, page_offsets, desc, out, ws);             \
+    attn::prefill_join<D, attn::CACHE>(desc, out, ws);                                                         \
   }
 LF_ATTN_PREFILL(64, bf16, kCacheBf16)
 LF_ATTN_PREFILL(128, bf16, kCacheBf16)

@@ -131,6 +131,41 @@ def test_only_the_prompts_of_a_mixed_step(rt):
     st.check(s, st.read(s, same), q, [2, 3])
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3_blocks"])
+def test_sequences_that_share_pages(rt, cache):
+    """A common beginning that is cached once, read by two prompts and a decoded sequence; one of its pages stands
+    in a table twice."""
+    rng = np.random.default_rng(16)
+    s = st.make_step(rt, rng, rows=[9, 70, 1], before=[80, 64, 90], prefill=2, page=16, cache=cache)
+    for i in (1, 2):
+        s.tables[i][:4] = s.tables[0][:4]
+    s.tables[2][2] = s.tables[2][1]
+    s.step.stage(s.row_offsets, [89, 134, 91], s.tables, prefill_rows=2)
+    q = st.queries(rng, s)
+    for prompts, sequences in ((True, [0, 1]), (False, [2])):
+        op, out = st.bind(rt, s, q, prompts)
+        op.launch(rt.stream, synchronous=True)
+        st.check(s, st.read(s, out), q, sequences)
+
+
+def test_two_bindings_on_two_streams(rt):
+    """Calls of two layers at once, each with a workspace of its own, many times over; cut prompts in both."""
+    rng = np.random.default_rng(17)
+    steps = [st.make_step(rt, rng, rows=[33, 2], before=[2500, 1800], query_heads=4, kv_heads=2, page=16, cache=cache)
+             for cache in ("bf16", "e4m3_blocks")]
+    queries = [st.queries(rng, s) for s in steps]
+    bound = [st.bind(rt, s, q) for s, q in zip(steps, queries)]
+    streams = [rt.stream, rt.context.create_stream()]
+    for _ in range(8):
+        for (op, _), stream in zip(bound, streams):
+            op.launch(stream, synchronous=False)
+    for stream in streams:
+        stream.synchronize()
+    for s, q, (op, out) in zip(steps, queries, bound):
+        op.check()
+        st.check(s, st.read(s, out), q, [0, 1])
+
+
 def test_a_step_without_prompts_writes_nothing(rt):
     rng = np.random.default_rng(10)
     s = st.make_step(rt, rng, rows=[1, 1], before=[3, 40], prefill=0)
