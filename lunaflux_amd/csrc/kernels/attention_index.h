@@ -365,16 +365,23 @@ LF_DEVICE PromptKeys keys_of(const Desc &d, const QueryTile &q, const Prompt &p,
 }
 
 // Where weight u cuts a pair of [begin, begin + weight) with `tiles` key tiles: at a multiple
-// of kCut of them, so that no part is shorter (but a pair itself may be). Does not fall as u rises.
+// of `cut` of them, so that no part is shorter (but a pair itself may be). Does not fall as u rises.
 // (Shorter parts cost their beginning, end and place in the join, longer ones equal ranges. us with 8 and 16:
 // windows of 1021 172 and 161, four prompts 174 and 178, heads of 256 180 and 189.)
 constexpr int kCut = 8;
-LF_DEVICE int cut_of(int64_t u, int64_t begin, int64_t weight, int tiles) {
+// In steps of little work (share, a block's weight, below 8 tiles of 64 keys) long pairs are cut at every fourth
+// tile instead. us with 8 and 4: 69 rows behind 3244 tokens, 28/4 heads of 128, 50 and 39; 3 prompts of 8 rows
+// behind 6566, 16/2, 42 and 32; 2 of 14 behind 40776, 5/1 of 64, 40 and 35; beyond it windows of 1021 156 and 166,
+// pairs of up to 24 tiles (1506 rows of 8 heads of 64) 35 and 42, tiles of 32 keys (1209 rows, 16/8 heads of 256)
+// 69 and 102.
+LF_DEVICE int cut_tiles(int64_t share, int tile_keys) { return tile_keys == 64 && share < kCut * 64 ? kCut / 2 : kCut; }
+LF_DEVICE int cut_of(int64_t u, int64_t begin, int64_t weight, int tiles, int cut = kCut) {
   if (u <= begin) return 0;
   if (u >= begin + weight) return tiles;
   const int k = static_cast<int>(static_cast<double>(u - begin) * tiles / static_cast<double>(weight) + 0.5);
-  const int c = (k + kCut / 2) / kCut * kCut;
-  return tiles - c < kCut ? tiles : c;
+  if (tiles < 4 * kCut) cut = kCut;
+  const int c = (k + cut / 2) / cut * cut;
+  return tiles - c < cut ? tiles : c;
 }
 
 // Whether the rows of a query tile can count keys enough for it to be cut: 2 kCut key tiles. (The host sizes the

@@ -20,7 +20,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 // between ranges leaves fp32 partial results, which a second launch adds up in their order.
 //
 // Weights are rounded to bf16 once, for the second product, and their sum is of the rounded ones, so
-// that equal values come out equal. A weight is off by 2^-9 of itself, as a value of out is: for values
+// that equal values come out equal. A weight is off by up to 2^-8 of itself, as a value of out is: for values
 // without a common part the errors are as large as out's own rounding (1.9e-3 of out in all against 64
 // bits, 1.6e-3 where only out is rounded). A second bf16 term would take that away for half as many
 // products again.
@@ -319,7 +319,8 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
   PromptPair pair = pair_at(d, plan, row_offsets, lengths, page_offsets, prefix, u0);
   for (;;) {
     const PromptKeys pk = keys_of(d, plan.tile, pair.p, pair.x, kKeys);
-    const int k0 = cut_of(u0, pair.begin, pair.weight, pk.tiles), k1 = cut_of(u1, pair.begin, pair.weight, pk.tiles);
+    const int cut = cut_tiles(plan.share, kKeys);
+    const int k0 = cut_of(u0, pair.begin, pair.weight, pk.tiles, cut), k1 = cut_of(u1, pair.begin, pair.weight, pk.tiles, cut);
     const PairHeads of = heads_of(d, plan, pair);
     const int h = of.h, head0 = of.first, heads = of.count, tokens = pk.last - pk.first_position + 1;
     const int row0 = pair.p.row + pair.x * plan.tile.tokens;
@@ -767,7 +768,7 @@ LF_DEVICE void prefill_join(const uint8_t *attn, uint16_t *out, uint8_t *ws) {
   const int range = blockIdx.x / kJoinSlices, slice = blockIdx.x % kJoinSlices;
   const RangeStart tile = *start_of(ws, range);
   if (d.magic != kMagic || tile.weight == 0) return;
-  auto cut = [&](int b) { return cut_of(b * tile.share, tile.begin, tile.weight, tile.tiles); };
+  auto cut = [&](int b) { return cut_of(b * tile.share, tile.begin, tile.weight, tile.tiles, cut_tiles(tile.share, P::kKeys)); };
   if (cut(range) == 0 || cut(range) >= cut(range + 1)) return;
 
   // the ranges with a part of the tile, in order
