@@ -173,20 +173,21 @@ LF_DEVICE RangeStart *start_of(uint8_t *ws, int range) { return reinterpret_cast
 static_assert(Prompts<64>::kBlocks * sizeof(RangeStart) <= Prompts<64>::kFloats * 4, "");
 
 // One global_load_lds_dwordx4: every lane's 16 bytes from its address go to LDS at lds + 16 lane
-// (wave-uniform; M0). As assembly, so that the compiler does not make every LDS read wait for it:
+// (wave-uniform; M0, whose write has to be a wait state before the load, which the compiler does not
+// see to inside an asm). As assembly, so that the compiler does not make every LDS read wait for it:
 // the kernel orders it by itself, with vmcnt and barriers. No read of the interval that it is issued in
 // touches what it writes, so the two may change places (interval_end holds both).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // M0 is listed as clobbered on purpose
 LF_DEVICE void load_to_lds(const uint8_t *src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                :
                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "m0");
 }
 // The same for 4 bytes a lane.
 LF_DEVICE void load_word_to_lds(const float *src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                :
                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "m0");

@@ -85,11 +85,13 @@ LF_DEVICE void wait_vmcnt() {
 // the LDS reads itself (s_waitcnt vmcnt + block barrier). M0 carries the
 // LDS offset, which must be wave-uniform (the compiler cannot prove that of
 // values derived from threadIdx.x, hence the readfirstlane); no other code in
-// these kernels uses M0.
+// these kernels uses M0. A load to LDS may come one wait state behind a scalar
+// write of M0 at the earliest, or it may take the place that M0 held before; the
+// compiler keeps that for its own instructions, not inside an asm (s_nop 0).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // M0 is listed as clobbered on purpose
 LF_DEVICE void dma16(const uint8_t *src, uint32_t lds_offset) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                :
                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds_offset))
                : "memory", "m0");
@@ -107,14 +109,14 @@ LF_DEVICE const uint8_t *uniform_ptr(const uint8_t *p) {
 // instruction group and a 32-bit register per lane instead of a 64-bit
 // address per lane and instruction.
 LF_DEVICE void dma16(const uint8_t *base, uint32_t offset, uint32_t lds_offset) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :
                : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds_offset))
                : "memory", "m0");
 }
 // The same for 4 bytes per lane: lane l's dword lands at lds_offset + 4 l.
 LF_DEVICE void dma4(const uint8_t *base, uint32_t offset, uint32_t lds_offset) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
                :
                : "v"(offset), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds_offset))
                : "memory", "m0");

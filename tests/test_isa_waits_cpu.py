@@ -1,0 +1,59 @@
+"""CPU checks of wait states in our own gfx950 build that the compiler does not place around inline assembly (the
+CDNA ISA's table of manually inserted wait states; the compiler keeps both for its own instructions)."""
+import re
+
+import pytest
+
+import test_isa_cpu as isa
+
+pytestmark = isa.pytestmark
+
+
+@pytest.fixture(scope="module")
+def kernels(tmp_path_factory):
+    return isa.disassemble(isa.CODE_OBJECT, tmp_path_factory.mktemp("waits"))
+
+
+def predecessors(ins):
+    """Of each instruction of a kernel, those that may run right before it."""
+    index, base = {a: i for i, (a, *_) in enumerate(ins)}, ins[0][0]
+    before = [[] for _ in ins]
+    for i, (_, m, _, target) in enumerate(ins):
+        if m not in ("s_branch", "s_endpgm") and i + 1 < len(ins):
+            before[i + 1].append(i)
+        if target is not None and base + target[1] in index:
+            before[index[base + target[1]]].append(i)
+    return before
+
+
+def too_early(ins, before, i, least, writes):
+    """The last instruction for which `writes` holds with fewer than `least` wait states between it and instruction i."""
+    todo = [(p, 0) for p in before[i]]
+    while todo:
+        at, waited = todo.pop()
+        mnemonic, operands = ins[at][1:3]
+        if writes(mnemonic, operands):
+            return ins[at]
+        waited += isa._waits(mnemonic, operands)
+        if waited < least:
+            todo += [(p, waited) for p in before[at]]
+    return None
+
+
+def loads_to_lds(mnemonic, operands):
+    return mnemonic.startswith("global_load_lds") or mnemonic.startswith("buffer_load") and re.search(r"\blds\b", operands)
+
+
+def test_a_load_to_lds_waits_for_m0(kernels):
+    """A scalar write of M0, one wait state, a load to LDS, which takes its place there from M0."""
+    seen, flagged = 0, []
+    for name, ins in kernels.items():
+        before = predecessors(ins)
+        for i, (address, mnemonic, operands, _) in enumerate(ins):
+            if loads_to_lds(mnemonic, operands):
+                seen += 1
+                at = too_early(ins, before, i, 1, lambda m, ops: m.startswith("s_") and ops.split(",")[0].strip() == "m0")
+                if at is not None:
+                    flagged.append(f"{name}+{address - ins[0][0]:#x}: {mnemonic} behind {at[1]} {at[2]}")
+    assert seen > 1000
+    assert not flagged, f"{len(flagged)}: " + "\n".join(flagged[:20])
