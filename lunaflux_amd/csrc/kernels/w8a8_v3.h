@@ -96,11 +96,14 @@ LF_DEVICE void dma16(const uint8_t *src, uint32_t lds_offset) {
                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds_offset))
                : "memory", "m0");
 }
-// A pointer every lane of the wave holds, moved to scalar registers.
+// A pointer every lane of the wave holds, moved to scalar registers. A vector memory
+// instruction may read those five wait states later at the earliest, which the compiler
+// does not see to before an asm (the loads below): they pass here.
 LF_DEVICE const uint8_t *uniform_ptr(const uint8_t *p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  asm("s_nop 4" : "+s"(lo), "+s"(hi));
   return reinterpret_cast<const uint8_t *>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 

@@ -57,3 +57,36 @@ def test_a_load_to_lds_waits_for_m0(kernels):
                     flagged.append(f"{name}+{address - ins[0][0]:#x}: {mnemonic} behind {at[1]} {at[2]}")
     assert seen > 1000
     assert not flagged, f"{len(flagged)}: " + "\n".join(flagged[:20])
+
+
+def scalar_registers(token):
+    m = re.match(r"s\[(\d+):(\d+)\]$", token) or re.match(r"s(\d+)()$", token)
+    return set(range(int(m.group(1)), int(m.group(2) or m.group(1)) + 1)) if m else set()
+
+
+def scalars_of_valu(mnemonic, operands):
+    """Scalar registers that a vector instruction writes."""
+    if not mnemonic.startswith("v_"):
+        return set()
+    tokens = isa._operands(operands)
+    carry = tokens[1:2] if "_co_" in mnemonic or mnemonic.startswith("v_mad_u64") or mnemonic.startswith("v_div_scale") else []
+    return set().union(*(scalar_registers(t) for t in tokens[:1] + carry))
+
+
+def test_memory_instructions_wait_for_scalars_that_vector_instructions_wrote(kernels):
+    """A vector instruction's write of a scalar register (v_readfirstlane), five wait states, a vector memory
+    instruction that reads it: before, the register may hold an older address."""
+    seen, flagged = 0, []
+    for name, ins in kernels.items():
+        before = predecessors(ins)
+        for i, (address, mnemonic, operands, _) in enumerate(ins):
+            if not mnemonic.startswith(("global_", "buffer_", "flat_", "scratch_")):
+                continue
+            read = set().union(*(scalar_registers(t) for t in re.split(r",\s*|\s+", operands)))
+            if read:
+                seen += 1
+                at = too_early(ins, before, i, 5, lambda m, ops: read & scalars_of_valu(m, ops))
+                if at is not None:
+                    flagged.append(f"{name}+{address - ins[0][0]:#x}: {mnemonic} {operands} behind {at[1]} {at[2]}")
+    assert seen > 1000
+    assert not flagged, f"{len(flagged)}: " + "\n".join(flagged[:20])
