@@ -621,7 +621,8 @@ typedef struct lf_fp8_attn_desc {
   int64_t turns_offset;
   int64_t axis_offset;
   int64_t region_bytes;
-  int32_t sinks;         /* first tokens that stay visible behind a window; 0: none */
+  int32_t sinks;         /* first tokens that stay visible behind a window, as lunaflux_fp8_attn_descriptor_sinks
+                            was given them; 0: none */
   int32_t block_tokens;  /* of an E4M3_BLOCKS cache: 16, or 8 where pages are of 8; else 0 */
   int64_t block_scales;  /* bytes, its table of scales in a cache region; else 0 */
   uint8_t padding[112];
@@ -631,9 +632,14 @@ typedef struct lf_fp8_attn_desc {
  * region offsets. LF_INVALID_ARGUMENT for values outside the ranges above,
  * strides that overlap or are not multiples of 16 bytes, or bounds past 32
  * bits (table_entries * page_size, the 32-key tiles of a step times heads).
- * The functions below take a descriptor as this one left it: one whose region
- * offsets do not follow from its fields is refused. */
+ * What the structure holds behind token_stride, and magic and reserved, is
+ * written, not read: it need not be set. The functions below take a descriptor
+ * as this one left it: one whose region offsets do not follow from its fields is
+ * refused. */
 int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *desc);
+/* The same for a window that leaves the first `sinks` tokens visible (sinks >= 0;
+ * lunaflux_fp8_attn_descriptor has none, whatever the field held). */
+int32_t lunaflux_fp8_attn_descriptor_sinks(lf_fp8_attn_desc *desc, int32_t sinks);
 /* Writes the descriptor region (desc->region_bytes bytes). scales: 2 kv_heads
  * values, finite and above zero (null for a bf16 cache, or E4M3_BLOCKS: ones); turns and axis:
  * rotary_dim / 2 each, turns finite, 0 <= axis < axes (null without rotation). */

@@ -141,6 +141,7 @@ SIGNATURES = {
     "lunaflux_fp8_moe_launch_geometry": (_i32, [_i32, _vp, _i32, _i32p, ctypes.c_char_p]),
     "lunaflux_fp8_moe_step_geometry": (_i32, [_i32, _vp, _i32, _i32p, ctypes.c_char_p]),
     "lunaflux_fp8_attn_descriptor": (_i32, [_vp]),
+    "lunaflux_fp8_attn_descriptor_sinks": (_i32, [_vp, _i32]),
     "lunaflux_fp8_attn_region": (_i32, [_vp, _f32p, _i64, _f64p, _i32p, _i64, _u8p, _i64]),
     "lunaflux_fp8_attn_cache_bytes": (_i64, [_vp]),
     "lunaflux_fp8_attn_workspace_bytes": (_i64, [_i32, _vp]),

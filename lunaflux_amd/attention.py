@@ -138,7 +138,7 @@ def attention_descriptor(*, query_heads: int, kv_heads: int, head_dim: int, page
                          rotary: Rotary | None = None, norm_epsilon: float | None = None,
                          softmax_scale: float | None = None, window: int = 0, strides=None,
                          sinks: int = 0) -> AttentionDescriptor:
-    """lunaflux_fp8_attn_descriptor. norm_epsilon None: heads are not
+    """lunaflux_fp8_attn_descriptor_sinks. norm_epsilon None: heads are not
     normalized; softmax_scale None: 1 / sqrt(head_dim); strides: (page, head,
     token) strides of the caches in elements, None: [page][head][token]; window 0:
     none; sinks: first tokens that a window leaves visible."""
@@ -170,7 +170,7 @@ def attention_descriptor(*, query_heads: int, kv_heads: int, head_dim: int, page
             raise _invalid("strides")
     except TypeError as e:
         raise _invalid(str(e)) from None
-    _check("attention_descriptor", _abi.lib().lunaflux_fp8_attn_descriptor(ctypes.byref(d)))
+    _check("attention_descriptor", _abi.lib().lunaflux_fp8_attn_descriptor_sinks(ctypes.byref(d), d.sinks))
     return d
 
 

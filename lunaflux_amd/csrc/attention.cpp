@@ -157,12 +157,16 @@ const char *cache_name(const lf_fp8_attn_desc *d) {
 
 extern "C" {
 
-int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *d) {
-  if (d == nullptr || !fields_ok(d)) return LF_INVALID_ARGUMENT;
+int32_t lunaflux_fp8_attn_descriptor(lf_fp8_attn_desc *d) { return lunaflux_fp8_attn_descriptor_sinks(d, 0); }
+
+int32_t lunaflux_fp8_attn_descriptor_sinks(lf_fp8_attn_desc *d, int32_t sinks) {
+  if (d == nullptr) return LF_INVALID_ARGUMENT;
   lf_fp8_attn_desc r = *d;
   r.magic = LF_FP8_ATTN_MAGIC;
   r.reserved = 0;
+  r.sinks = sinks;
   std::memset(r.padding, 0, sizeof(r.padding));
+  if (!fields_ok(&r)) return LF_INVALID_ARGUMENT;
   if (r.page_stride == 0 && r.head_stride == 0 && r.token_stride == 0) {
     r.token_stride = r.head_dim;
     r.head_stride = int64_t(r.page_size) * r.head_dim;
