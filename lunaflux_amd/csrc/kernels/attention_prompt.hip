@@ -225,7 +225,8 @@ LF_DEVICE void interval_end() {
 
 // The rows of a query tile that one wave has, without the matrix units: for rows that some infinity or NaN
 // reached, since in products of tiles zero times such a value of a key that a row does not count is NaN
-// too, and for tables with pages outside the cache. Here only the keys that it counts enter. Lanes c and
+// too, for ones with scores so large that their differences need the scores rounded as the maximum is, and
+// for tables with pages outside the cache. Here only the keys that it counts enter. Lanes c and
 // c + 32 hold the halves of row c. Apart from the kernel's registers, and slow, which such rows bear: a
 // prompt of 8192 rows that all hold a NaN takes 208 ms, 380 times as long as without.
 struct CarefulRow {
@@ -264,7 +265,9 @@ __device__ __attribute__((noinline)) void careful_row(const Desc &d, const Caref
       for (int e = 0; e < D / 2; ++e) score += bf16_to_f32(r.q[half * (D / 2) + e]) * value(r.kc, page, slot, half * (D / 2) + e);
       score += __shfl_xor(score, 32);
       if (j > r.position || !(d.window == 0 || j > r.position - d.window || j < d.sinks)) continue;
-      const float z = (flip ? -score : score) * r.factor, next = fmaxf(top, z), from = next == -INFINITY ? 0.0f : next;
+      float z = (flip ? -score : score) * r.factor;
+      asm("" : "+v"(z));  // rounded, for the difference below too: a fused one is not zero at the maximum
+      const float next = fmaxf(top, z), from = next == -INFINITY ? 0.0f : next;
       const float keep = __builtin_amdgcn_exp2f(top - from), p = __builtin_amdgcn_exp2f(z - from);
       top = next;
       sum = sum * keep + p;
@@ -718,7 +721,10 @@ LF_DEVICE void prefill(const int32_t *counts, const int32_t *row_offsets, const 
           part[P::kRows * D + P::kRows + m] = total;
         }
       }
-      if (__ballot(live && !(finite < INFINITY)) != 0 || redo >= 2) {
+      // A maximum of 2^29 or more is rounded by 16 or more, and a score, whose product is not, may be as far from it:
+      // from 2^31 on, weights relative to it could all be zero.
+      const bool coarse = !(fabsf(top) < 0x1p29f) && top != -INFINITY;
+      if (__ballot(live && (!(finite < INFINITY) || coarse)) != 0 || redo >= 2) {
         const CarefulRow r = {q + static_cast<uint64_t>(row_at) * D, kc, vc, table, pk, k0, k1, h, position, factor};
         float acc[D / 2], careful_top, careful_sum;
         careful_row<D, CACHE>(d, r, flip, acc, careful_top, careful_sum);
