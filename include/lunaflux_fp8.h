@@ -571,9 +571,11 @@ int32_t lunaflux_fp8_moe_step_geometry(int32_t entry,
  * of a sequence of n is at p = length - n + i and counts the keys j <= p, with a
  * window those with j > p - window or j < sinks; the rest as for decode, except
  * that the weights go to the second product as bf16 values (their sum is of the
- * same values). A sequence whose rows leave the batch or outnumber its tokens,
- * or whose tokens outnumber its pages' slots, is left out. The join launch
- * follows the other on the same stream.
+ * same values), and that an infinite value of a key that counts, with a score
+ * above -inf, is that infinity in out however small its weight (both signs:
+ * NaN). A sequence whose rows leave the batch or outnumber its tokens, or whose
+ * tokens outnumber its pages' slots, is left out. The join launch follows the
+ * other on the same stream.
  *
  * The cache regions hold, for page p, head h and slot i, D elements at
  * p * page_stride + h * head_stride + i * token_stride (elements; any order of

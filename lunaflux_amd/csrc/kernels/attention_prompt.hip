@@ -223,6 +223,10 @@ LF_DEVICE void interval_end() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// v times a weight above zero that may have vanished in fp32: an infinite value stays what it is. So a row that counts
+// one has the same result wherever its largest score is and wherever its keys are cut.
+LF_DEVICE float weighted(float v, float weight) { return fabsf(v) == INFINITY ? v : v * weight; }
+
 // The rows of a query tile that one wave has, without the matrix units: for rows that some infinity or NaN
 // reached, since in products of tiles zero times such a value of a key that a row does not count is NaN
 // too, for ones with scores so large that their differences need the scores rounded as the maximum is, and
@@ -271,7 +275,10 @@ __device__ __attribute__((noinline)) void careful_row(const Desc &d, const Caref
       const float keep = __builtin_amdgcn_exp2f(top - from), p = __builtin_amdgcn_exp2f(z - from);
       top = next;
       sum = sum * keep + p;
-      for (int e = 0; e < D / 2; ++e) acc[e] = acc[e] * keep + fmaxf(p, 0x1p-126f) * value(r.vc, page, slot, half * (D / 2) + e);
+      for (int e = 0; e < D / 2; ++e) {
+        const float v = value(r.vc, page, slot, half * (D / 2) + e);
+        acc[e] = weighted(acc[e], keep) + (z == -INFINITY ? v * p : weighted(v, p));
+      }
     }
   }
 }
@@ -812,7 +819,23 @@ LF_DEVICE void prefill_join(const uint8_t *attn, uint16_t *out, uint8_t *ws) {
     x.sum = x.sum * keep + l * f;
     x.top = next;
   };
-  auto finish = [&](int quad, const Joined &x) {
+  // The parts of a row that has an infinity, once more. (All parts so take 1 to 2 us more: 170 and 172 for 61 rows behind
+  // 131010 tokens; this way they take what they did without it.)
+  auto odd_values = [&](int quad) {
+    Joined x = {{0.0f, 0.0f, 0.0f, 0.0f}, -INFINITY, 0.0f};
+    for (int p = 0; p < parts; ++p) {
+      const float *part = partial_of<D>(ws, slots[p]);
+      const float t = part[P::kRows * D + quad / kQuads], next = fmaxf(x.top, t), base = next == -INFINITY ? 0.0f : next;
+      const float keep = __builtin_amdgcn_exp2f(x.top - base), f = __builtin_amdgcn_exp2f(t - base);
+      for (int e = 0; e < 4; ++e) x.acc[e] = weighted(x.acc[e], keep) + weighted(part[4 * quad + e], f);
+      x.sum = x.sum * keep + part[P::kRows * D + P::kRows + quad / kQuads] * f;
+      x.top = next;
+    }
+    return x;
+  };
+  auto finish = [&](int quad, Joined x) {
+    const float some = (x.acc[0] + x.acc[1]) + (x.acc[2] + x.acc[3]);
+    if (some != some) x = odd_values(quad);
     const int m = quad / kQuads, column = quad % kQuads * 4, token = (m * tile.token_of) >> 16;
     const float scale = vscale / x.sum;
     uint2 w = {pack_bf16(x.acc[0] * scale, x.acc[1] * scale), pack_bf16(x.acc[2] * scale, x.acc[3] * scale)};
