@@ -658,9 +658,9 @@ enum lf_fp8_attn_entry {
   LF_FP8_ATTN_PREFILL_JOIN = 4
 };
 /* Workspace of DECODE or PREFILL (ws; its join's is the same one) or of
- * QK_NORM_ROPE (status): zero-filled once when
- * allocated (its counters return to zero at the end of every launch; launches
- * sharing one must not overlap). -1 if invalid. */
+ * QK_NORM_ROPE (status): zero-filled once when allocated, PREFILL's first
+ * LF_FP8_ATTN_STATUS_BYTES at least (counters return to zero at the end of every
+ * launch; launches sharing one must not overlap). -1 if invalid. */
 int64_t lunaflux_fp8_attn_workspace_bytes(int32_t entry, const lf_fp8_attn_desc *desc);
 /* dims[0] is 0 for a PREFILL_JOIN that the descriptor's sizes never need. */
 int32_t lunaflux_fp8_attn_launch_geometry(int32_t entry, const lf_fp8_attn_desc *desc,

@@ -156,6 +156,7 @@ MOE_SORT_COUNT = 8
 LF_FP8_CACHE_BF16, LF_FP8_CACHE_E4M3, LF_FP8_CACHE_E4M3_BLOCKS = 1, 2, 3
 LF_FP8_PAIR_HALF, LF_FP8_PAIR_NEIGHBOUR = 0, 1
 LF_FP8_ATTN_MAX_SEQUENCES = 2048
+LF_FP8_ATTN_STATUS_BYTES = 256
 ATTN_QK_NORM_ROPE, ATTN_DECODE, ATTN_PREFILL, ATTN_PREFILL_JOIN = 1, 2, 3, 4
 LOW_RANK_ONE_LAUNCH, LOW_RANK_SHRINK, LOW_RANK_EXPAND = 1, 2, 3
 

@@ -385,7 +385,8 @@ def _step_fits(layer: AttentionLayer, step: PagedStep):
 def _workspace(rt: ProjectionRuntime, entry: int, desc: AttentionDescriptor) -> Allocation:
     nbytes = workspace_bytes(entry, desc)
     ws = rt.context.allocate(nbytes)
-    ws.copy_from_host(np.zeros(nbytes, np.uint8))
+    # (a prompt's partial results, up to 135 MB, are written before they are read)
+    ws.copy_from_host(np.zeros(_abi.LF_FP8_ATTN_STATUS_BYTES if entry == _abi.ATTN_PREFILL else nbytes, np.uint8))
     return ws
 
 
