@@ -460,16 +460,20 @@ def bind_paged_prefill(rt: ProjectionRuntime, layer: AttentionLayer, step: Paged
     [max_tokens, Hq, D] (bf16, rotated) against the cached keys of each up to the
     row's own, which the append has written, out [max_tokens, Hq D]. Rows of
     decoded sequences stay as they were. out may not overlap what is read. One
-    launch, or two where the layer's sizes let a row have 1024 keys or more (512
-    for heads of 256): then work is split over the keys, and joined. The
-    workspace is 35 MB then for heads of 64, 68 of 128 and 135 of 256.
+    launch, or two where the layer's sizes let a query tile have 16 key tiles: if
+    table_entries * page_size (of all sequences: a table may belong to one of them)
+    passes 960, 480 for heads of 256, and so do, under a window, window + sinks +
+    a tile's rows + two key tiles. Then work is split over the keys, and joined, and
+    the workspace, one for each binding, is 35 MB for heads of 64, 68 of 128 and 135
+    of 256.
 
     The rows' statistics are fp32, their weights bf16 in the second product: where
     values differ freely from key to key, that is as large an error as the
     rounding of out, and smaller the less they differ. A row that an infinity or a
-    NaN reaches, in keys or values that it counts or in others of its tiles, and a
-    table with pages that the cache does not have take a path without the matrix
-    units, which is right and some 300 times slower."""
+    NaN reaches, in keys or values that it counts or in others of its tiles, one
+    whose largest score times log2 e is 2^29 or more (or at most -2^29), and a table
+    with pages that the cache does not have take a path without the matrix units, which is right and
+    some 400 times slower."""
     args, ws = _attention_args(rt, _abi.ATTN_PREFILL, layer, step, q, out, k_cache, v_cache)
     dims, symbol = launch_geometry(_abi.ATTN_PREFILL, layer.desc)
     steps = [LaunchStep(rt.function(symbol), dims, KernelArguments(args), symbol)]

@@ -285,9 +285,9 @@ LF_DEVICE QueryTile query_tile_of(const Desc &d, int tile_rows) {
 // innermost. A pair weighs the keys that its tile sees, without their rounding to key tiles,
 // and kPairKeys for what it takes whatever its keys are: min(a + step x, cap) for tile x of a
 // sequence, so that sums over x have a closed form. The blocks take equal ranges of weight.
-// (kPairKeys by what pairs take apart from their keys: 8192 rows and four prompts of up to 2039, heads of
-// 128, us with 32, 64, 256 and 512 of them: 649, 629, 571, 572 and 190, 190, 174, 180; other kinds of steps
-// within 3 % all along.)
+// (kPairKeys by what pairs take apart from their keys, us with 64, 256 and 512 of them: 8192 rows of heads of 128
+// 619, 564 and 566, four prompts of up to 2039 rows 174, 158 and 163, of heads of 64 114, 105 and 110, windows of
+// 1021 146, 150 and 152; few rows behind a cache, 1209 to 2545 of heads of 256 and one prompt of 1506 within 2 %.)
 constexpr int kPairKeys = 256;
 struct Weights {
   int64_t a, step, cap, rising;  // rising: the tiles that weigh less than cap
@@ -367,13 +367,14 @@ LF_DEVICE PromptKeys keys_of(const Desc &d, const QueryTile &q, const Prompt &p,
 // Where weight u cuts a pair of [begin, begin + weight) with `tiles` key tiles: at a multiple
 // of `cut` of them, so that no part is shorter (but a pair itself may be). Does not fall as u rises.
 // (Shorter parts cost their beginning, end and place in the join, longer ones equal ranges. us with 8 and 16:
-// windows of 1021 172 and 161, four prompts 174 and 178, heads of 256 180 and 189.)
+// windows of 1021 150 and 135, four prompts of heads of 128 158 and 167, of 64 105 and 116, heads of 256 170 and
+// 178, 8192 rows alike.)
 constexpr int kCut = 8;
 // In steps of little work (share, a block's weight, below 8 tiles of 64 keys) long pairs are cut at every fourth
-// tile instead. us with 8 and 4: 69 rows behind 3244 tokens, 28/4 heads of 128, 50 and 39; 3 prompts of 8 rows
-// behind 6566, 16/2, 42 and 32; 2 of 14 behind 40776, 5/1 of 64, 40 and 35; beyond it windows of 1021 156 and 166,
-// pairs of up to 24 tiles (1506 rows of 8 heads of 64) 35 and 42, tiles of 32 keys (1209 rows, 16/8 heads of 256)
-// 69 and 102.
+// tile instead. us with 8 and 4: 69 rows behind 3244 tokens, 28/4 heads of 128, 47 and 34; 3 prompts of 8 rows
+// behind 6566, 16/2, 41 and 30; 2 of 14 behind 40776, 5/1 of 64, 36 and 32. Cut at 4 beyond that (when the rule was
+// made, before later steps): windows of 1021 156 and 166, pairs of up to 24 tiles (1506 rows of 8 heads of 64) 35 and
+// 42, tiles of 32 keys (1209 rows, 16/8 heads of 256) 69 and 102.
 LF_DEVICE int cut_tiles(int64_t share, int tile_keys) { return tile_keys == 64 && share < kCut * 64 ? kCut / 2 : kCut; }
 LF_DEVICE int cut_of(int64_t u, int64_t begin, int64_t weight, int tiles, int cut = kCut) {
   if (u <= begin) return 0;

@@ -21,18 +21,18 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 //
 // Weights are rounded to bf16 once, for the second product, and their sum is of the rounded ones, so
 // that equal values come out equal. A weight is off by up to 2^-8 of itself, as a value of out is: for values
-// without a common part the errors are as large as out's own rounding (1.9e-3 of out in all against 64
-// bits, 1.6e-3 where only out is rounded). A second bf16 term would take that away for half as many
+// without a common part the errors are as large as out's own rounding (1.7e-3 to 2.4e-3 of out in all against
+// 64 bits, more the more keys; 1.6e-3 to 1.7e-3 where only out is rounded). A second bf16 term would take that away for half as many
 // products again.
 //
 // Matrix products bound it, with the softmax close behind: of a tile of heads of 128 a wave has 32 products,
 // 1024 cycles of the matrix unit, and some 190 vector instructions, 900 of the vector unit. 8192 rows, 32/8 heads
-// of 128: 551 us, 1.00 PFLOP/s of 1.39 that an 8192^3 product reaches; 49 % of the cycles of the matrix
-// units at the 1.9 GHz that the card holds under it, LDS reads 19-25 % without conflicts. By steps: waves
+// of 128: 555-570 us, 0.97-0.99 PFLOP/s of 1.39 that an 8192^3 product reaches, at the 1.9 GHz that the card holds
+// under it; under the counters matrix units 47 % of the cycles, LDS reads 23 % without conflicts. By steps: waves
 // of 16 rows with tiles through registers 1652 us; two groups of waves with 32 rows and loads that go
 // straight to LDS 696; operands read ahead and code of their own for the groups 584; a third stage of
 // tiles 551. Loads issued by the second group instead of the first: 591 at the time of 554. Tiles of 32 keys
-// for heads of 256, whose sums and queries take 192 registers of a lane: 177 us for 2045 rows.
+// for heads of 256, whose sums and queries take 192 registers of a lane: 170 us for 2045 rows behind 2500 tokens each.
 template <int D>
 struct Prompts {
   static constexpr int kWaves = 8, kThreads = 64 * kWaves, kBlocks = 256;
@@ -232,7 +232,7 @@ LF_DEVICE float weighted(float v, float weight) { return fabsf(v) == INFINITY ? 
 // too, for ones with scores so large that their differences need the scores rounded as the maximum is, and
 // for tables with pages outside the cache. Here only the keys that it counts enter. Lanes c and
 // c + 32 hold the halves of row c. Apart from the kernel's registers, and slow, which such rows bear: a
-// prompt of 8192 rows that all hold a NaN takes 208 ms, 380 times as long as without.
+// prompt of 8192 rows that all hold a NaN takes 233 ms, 400 times as long as without.
 struct CarefulRow {
   const uint16_t *q;
   const uint8_t *kc, *vc;
