@@ -143,8 +143,10 @@ LF_DEVICE void finish(const Sync &s, int total, int steps, Flag &flag) {
 
 // 16 bytes stored through the XCD's L2 (the cache policy of an agent-scope
 // atomic store), for outputs that blocks on other XCDs read in this launch.
+// (Its data registers may be written again two wait states later, which the
+// compiler does not see to behind an asm.)
 LF_DEVICE void store16_through(void *p, u32x4 v) {
-  asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(v) : "memory");
+  asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
 }
 
 }  // namespace phase

@@ -90,3 +90,26 @@ def test_memory_instructions_wait_for_scalars_that_vector_instructions_wrote(ker
                     flagged.append(f"{name}+{address - ins[0][0]:#x}: {mnemonic} {operands} behind {at[1]} {at[2]}")
     assert seen > 1000
     assert not flagged, f"{len(flagged)}: " + "\n".join(flagged[:20])
+
+
+def test_data_of_wide_stores_is_not_written_before_it_is_read(kernels):
+    """A store of more than 8 bytes a lane reads its data registers late: a vector instruction may write them two wait
+    states after it."""
+    seen, flagged = 0, []
+    for name, ins in kernels.items():
+        before = predecessors(ins)
+        for i, (address, mnemonic, operands, _) in enumerate(ins):
+            tokens = isa._operands(operands)
+            written = isa._regs(tokens[0]) if mnemonic.startswith("v_") and tokens else set()
+
+            def stores(m, ops):
+                if not re.match(r"(global|flat|scratch|buffer)_store_dwordx[34]$", m):
+                    return False
+                return isa._regs(isa._operands(ops)[0 if m.startswith("buffer") else 1].split()[0]) & written
+            if written:
+                seen += 1
+                at = too_early(ins, before, i, 2, stores)
+                if at is not None:
+                    flagged.append(f"{name}+{address - ins[0][0]:#x}: {mnemonic} {operands} behind {at[1]} {at[2]}")
+    assert seen > 1000
+    assert not flagged, f"{len(flagged)}: " + "\n".join(flagged[:20])
