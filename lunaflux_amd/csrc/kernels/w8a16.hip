@@ -416,6 +416,12 @@ __device__ void w8a16_kernel(const int32_t *counts, const uint16_t *x, const uin
             asm volatile("" : "+v"(acc[mt][i]));
           }
         }
+      } else {
+        // A product's result may be read eight wait states behind it. Where the
+        // loop ends, the compiler does not count them over the branches to the
+        // epilogue's first read, and left six; with these two there are eight.
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 1");
       }
       if (kl + D < nkt) load_tiles<NW>(strip, kt0 + kl + D, lane, b[d]);
     }

@@ -113,3 +113,42 @@ def test_data_of_wide_stores_is_not_written_before_it_is_read(kernels):
                     flagged.append(f"{name}+{address - ins[0][0]:#x}: {mnemonic} {operands} behind {at[1]} {at[2]}")
     assert seen > 1000
     assert not flagged, f"{len(flagged)}: " + "\n".join(flagged[:20])
+
+
+def test_mfma_results_are_not_read_early_on_any_way(kernels):
+    """The wait states from each matrix instruction to the first vector read of its result, on every way through any
+    number of branches, are at least the fewest that the compiler places inside a block."""
+    needed, flagged = {}, []
+    for ins in kernels.values():
+        for i, (_, mnemonic, operands, _) in enumerate(ins):
+            if not mnemonic.startswith("v_mfma"):
+                continue
+            result, waited = isa._regs(isa._operands(operands)[0]), 0
+            for _, m, ops, target in ins[i + 1:i + 40]:
+                if target is not None or m == "s_endpgm":
+                    break
+                if result & isa._reads(m, ops):
+                    needed[mnemonic] = min(needed.get(mnemonic, 99), waited)
+                    break
+                if m.startswith("v_mfma") and result & isa._regs(isa._operands(ops)[0]):
+                    break
+                waited += isa._waits(m, ops)
+    assert needed
+    for name, ins in kernels.items():
+        before = predecessors(ins)
+        for i, (address, mnemonic, operands, _) in enumerate(ins):
+            reads = isa._reads(mnemonic, operands)
+            todo, seen = [(p, 0) for p in before[i]] if reads else [], set()
+            while todo:
+                at, waited = todo.pop()
+                m, ops = ins[at][1:3]
+                written = isa._regs(isa._operands(ops)[0]) if m.startswith("v_") else set()
+                if m.startswith("v_mfma") and reads & written:
+                    if waited < needed.get(m, 8):
+                        flagged.append(f"{name}+{address - ins[0][0]:#x}: {mnemonic} {operands} {waited} < {needed.get(m, 8)} behind {m}")
+                    continue
+                waited += isa._waits(m, ops)
+                if waited < 20 and not reads <= written and (at, waited) not in seen:
+                    seen.add((at, waited))
+                    todo += [(p, waited) for p in before[at]]
+    assert not flagged, f"{len(flagged)}, of {needed}: " + "\n".join(flagged[:20])
