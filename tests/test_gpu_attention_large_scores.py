@@ -18,15 +18,16 @@ def rt():
 
 @pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("magnitude", [2.0 ** 20, 2.0 ** 29, 2.0 ** 31, 2.0 ** 36])
-def test_equal_scores_average_the_values(rt, dim, magnitude, window, sinks):
+@pytest.mark.parametrize("cache", ["bf16", "e4m3", "e4m3_blocks"])
+@pytest.mark.parametrize("magnitude", [2.0 ** 20, 2.0 ** 29, 2.0 ** 31, 2.0 ** 36, 2.0 ** 44])
+def test_equal_scores_average_the_values(rt, dim, magnitude, window, sinks, cache):
     """Keys are alike, so each row's weights are, bit by bit. Bound as for prompts, of twice as many terms."""
     rng = np.random.default_rng(int(np.log2(magnitude)) + dim)
     before = [0, 1, 31, 32, 70, 900]
     s = st.make_step(rt, rng, rows=[1] * 6, before=before, prefill=0, query_heads=16, kv_heads=1, head_dim=dim, page=16,
-                     window=window, sinks=sinks)
-    same_keys(rt, rng, s, synth.bf16_bits(np.float32(magnitude / dim)))
-    q = np.ones((6, 16, dim), np.float32) * (1 + np.arange(96).reshape(6, 16, 1) / 128).astype(np.float32)
+                     cache=cache, window=window, sinks=sinks)
+    same_keys(s)
+    q = np.full((6, 16, dim), magnitude / dim, np.float32) * (1 + np.arange(96).reshape(6, 16, 1) / 128).astype(np.float32)
     op, out = st.bind(rt, s, synth.bf16_bits(q), prompts=False)
     op.launch(rt.stream, synchronous=True)
     got = synth.bf16_values(st.read(s, out)).astype(np.float64)

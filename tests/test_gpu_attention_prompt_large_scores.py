@@ -15,29 +15,32 @@ def rt():
     return fp8.ProjectionRuntime(0)
 
 
-def same_keys(rt, rng, s, value):
-    """All keys of the cache the same bf16 values."""
-    codes, _ = s.codes(s.host["k"])
+def same_keys(s):
+    """All keys of the cache the same values: ones, in steps of 2^-6 or of a head's scale over codes."""
+    codes, table = s.codes(s.host["k"])
     for i in range(len(s.rows)):
         for j in range(s.before[i] + s.rows[i]):
             page, slot = s.place(i, j)
+            if table is not None:
+                table[page, slot // s.desc.block_tokens] = 2.0 ** -6
             for h in range(s.desc.kv_heads):
                 at = s.element(page, h, slot)
-                codes[at:at + s.desc.head_dim] = value
+                codes[at:at + s.desc.head_dim] = synth.bf16_bits(np.float32(1.0)) if s.kind == "bf16" else 0x38
     s.device["k"].copy_from_host(s.host["k"])
 
 
 # rows from a first token on (one key), and ones cut between blocks
 @pytest.mark.parametrize("rows,before,dim", [([70], [0], 64), ([70], [0], 128), ([40], [100], 256), ([9], [3000], 64)])
 @pytest.mark.parametrize("sign", [1.0, -1.0])
-@pytest.mark.parametrize("magnitude", [2.0 ** 20, 2.0 ** 29, 2.0 ** 31, 2.0 ** 36])
-def test_equal_scores_average_the_values(rt, rows, before, dim, sign, magnitude):
+@pytest.mark.parametrize("cache", ["bf16", "e4m3", "e4m3_blocks"])
+@pytest.mark.parametrize("magnitude", [2.0 ** 20, 2.0 ** 29, 2.0 ** 31, 2.0 ** 36, 2.0 ** 44])
+def test_equal_scores_average_the_values(rt, rows, before, dim, sign, magnitude, cache):
     """Keys are alike, so each row's weights are, bit by bit, whatever its score; rows differ in theirs. Bound: sums of
     n fp32 terms, numerator and denominator (their weights are the same bf16 values), the quotient, the rounding to bf16."""
     rng = np.random.default_rng(int(np.log2(magnitude)) + dim)
-    s = st.make_step(rt, rng, rows=rows, before=before, query_heads=2, kv_heads=1, head_dim=dim, page=16)
-    same_keys(rt, rng, s, synth.bf16_bits(np.float32(magnitude / dim)))
-    q = np.ones((s.desc.max_tokens, 2, dim), np.float32) * sign
+    s = st.make_step(rt, rng, rows=rows, before=before, query_heads=2, kv_heads=1, head_dim=dim, page=16, cache=cache)
+    same_keys(s)
+    q = np.full((s.desc.max_tokens, 2, dim), sign * magnitude / dim, np.float32)
     q *= (1 + np.arange(2 * s.desc.max_tokens).reshape(-1, 2, 1) % 97 / 128).astype(np.float32)
     q = synth.bf16_bits(q)
     op, out = st.bind(rt, s, q)
